@@ -60,6 +60,11 @@ extern "C" {
 #define TVQ_FP8_REF 0 /* reference encoder, tv/quantization/types.tkv:154-191 (quirks kept) */
 #define TVQ_FP8_HW 1  /* hardware cvt.rn.satfinite (OCP E4M3), not the reference's          */
 
+/* ---- element types of the decoding operators */
+#define TVQ_TYPE_F32 0
+#define TVQ_TYPE_F16 1
+#define TVQ_TYPE_BF16 2
+
 /* ---- library / device */
 TVQ_API int tvq_version(void);
 /* Copies the last error message of the calling thread (NUL-terminated). */
@@ -398,6 +403,95 @@ TVQ_API int tvq_permute_cols(const float* src, float* dst, int64_t rows, int64_t
 TVQ_API int tvq_matmul_int4_grouped(const float* A, const uint8_t* packed_w, const float* bias, int64_t n_bias,
                                     float* Y, int64_t m, int64_t n, int64_t k, int64_t group_size,
                                     const float* scales_w, int64_t n_scales, const int64_t* perm);
+
+/* ================================================================ decoding
+ * A paged cache of keys and values, the attention of new tokens over it, beam
+ * search's choice of tokens and the reordering of the beams' caches.  No
+ * counterpart in the reference, whose attention recomputes every key on every
+ * call (gpt2_attention, tv/training/gpt2_ref.tkv:360-395).  Device buffers,
+ * asynchronous on `stream`; lengths, tables and parents are read on the
+ * device, so a decoding loop needs no host round trip.
+ *
+ * The cache of one layer is pages of `page` tokens: shape (host) = {pages,
+ * page, kv heads, head dim}, page a power of two in [8, 1024], head dim a
+ * multiple of 8 up to 128, values of `type` (F16 or BF16).  strides (host, in
+ * elements) = {k page, k token, k head, v page, v token, v head}, multiples
+ * of 8 (a token's head is contiguous; bases 16-byte aligned), so pages may be
+ * [page, heads, dim] or [heads, page, dim] inside, with gaps.  Sequence s holds
+ * ctx_len[s] tokens, token j in page table[s * table_stride + j / page], slot
+ * j % page; cols = columns of the table.  Its new rows are the packed rows
+ * cu[s] .. cu[s + 1] (cu NULL: one row each, n_rows = n_seq); row i of n sits
+ * at position ctx_len[s] - n + i.  Page numbers outside [0, pages) within a
+ * sequence's length record a device error (tvq_device_error: TVQ_ERR_INVALID)
+ * and are never dereferenced: append drops such a row, attention reads zeros.
+ * Packed rows of no sequence (outside [cu[0], cu[n_seq])) are dropped by
+ * append, and attention leaves their outputs as they are. */
+
+/* k, v rows [n_rows, kv heads, head dim] of src_type (F32, F16, BF16;
+ * src_strides (host) = {k token, k head, v token, v head, q token, q head} in
+ * elements, rows 16-byte aligned), rounded once to `type`, into the pages.  q
+ * (or NULL) [n_rows, q_heads, head dim] is rounded to q_out, contiguous. */
+TVQ_API int tvq_dev_paged_append(int type, int src_type, const void* k, const void* v, const void* q,
+                                 const int64_t* src_strides, int64_t q_heads, void* q_out, void* k_pages,
+                                 void* v_pages, const int64_t* shape, const int64_t* strides, const int32_t* table,
+                                 int64_t table_stride, int64_t cols, const int32_t* ctx_len, const int32_t* cu,
+                                 int64_t n_seq, int64_t n_rows, void* stream);
+/* out[row, h] = sum_j softmax_j(scale q[row, h] . k_j) v_j over the keys j <=
+ * position (and j > position - window if window > 0) of the row's sequence,
+ * kv head h / (q_heads / kv heads); q and out of `type`, q_strides (host) =
+ * {token, head}, out contiguous.  lse (or NULL) f32 [n_rows, q_heads] = ln
+ * sum_j exp(scale q . k_j).  A row without keys (at a negative position): out
+ * 0, lse -inf.  max_q: no sequence has more new rows (a host bound; the rows
+ * of a longer one are left as they are from there on).
+ * What lies in a page behind a sequence's end has no influence.  Products
+ * are formed in f32; the softmax's weights are rounded to `type` before
+ * they meet V (relative 2^-11 / 2^-8 each), its statistics stay f32.
+ * ws: at least tvq_paged_attention_workspace bytes, 256-byte aligned, used by
+ * one call at a time, zero before its first use (a call leaves it so). */
+TVQ_API int tvq_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t n_seq,
+                                          int64_t n_rows, int64_t max_q, int64_t* bytes);
+TVQ_API int tvq_dev_paged_attention(int type, const void* q, const int64_t* q_strides, int64_t q_heads,
+                                    const void* k_pages, const void* v_pages, const int64_t* shape,
+                                    const int64_t* strides, const int32_t* table, int64_t table_stride, int64_t cols,
+                                    const int32_t* ctx_len, const int32_t* cu, int64_t n_seq, int64_t n_rows,
+                                    int64_t max_q, float scale, int64_t window, void* out, float* lse, void* ws,
+                                    int64_t ws_bytes, void* stream);
+/* One step of beam search.  logits [batch * beams, vocab] of `type`, rows
+ * `stride` elements apart; scores f32 [batch * beams].  Each beam lists its
+ * `keep` largest logits (ties: lowest token; NaN counts as -inf), each with
+ * total = score + ((x - max) - ln sum exp(x - max)) in f32 (NaN counts as
+ * -inf); out: the `keep` best totals of a request's lists, descending, ties to
+ * the lower beam, then to the place in its list.  finished (or NULL) [batch *
+ * beams] bytes: a finished beam has the one continuation eos at no cost (its
+ * row counts as 0 at eos, -inf elsewhere).  keep <= 64, keep <= vocab, beams
+ * <= 64.  parents: the row batch * beams is numbered within its request (0 ..
+ * beams - 1).  ws as for attention, tvq_beam_select_workspace bytes. */
+TVQ_API int tvq_beam_select_workspace(int64_t batch, int64_t beams, int64_t keep, int64_t vocab, int64_t* bytes);
+TVQ_API int tvq_dev_beam_select(int type, const void* logits, int64_t stride, const float* scores,
+                                const uint8_t* finished, int64_t batch, int64_t beams, int64_t keep, int64_t vocab,
+                                int64_t eos, float* out_scores, int64_t* out_tokens, int32_t* out_parents, void* ws,
+                                int64_t ws_bytes, void* stream);
+/* Row r of the new tables continues row parents[r] of the old ones (-1: an
+ * empty row).  Full pages are shared; refs[pages] counts how often the tables
+ * (and whoever else keeps pages) hold each page.  Every row gets room for
+ * one more token: behind a full page a free page; a part-filled last page
+ * stays with the lowest new row that has it (if nobody but the old tables
+ * holds it), the other rows take a free page each and its filled tokens are
+ * copied there, in every layer, keys and values.  Free pages are those with
+ * refs 0 before the call, lowest number first, in row order.  Written:
+ * new_table [new_rows, cols] (unused entries -1), new_lens, new_refs (all
+ * apart from their inputs), status[2] = {pages taken, rows left without room:
+ * no free page or no column; their next entry is -1}.  The cache is [layers,
+ * pages, page, kv heads, dim]: shape (host) = {pages, page, kv heads, head
+ * dim, layers}, strides (host) = {k layer, page, token, head, v layer, page,
+ * token, head}, elements of 2 bytes; layers 0 moves tables only.  Rows <=
+ * 65535.  ws as for attention, tvq_beam_reorder_workspace bytes. */
+TVQ_API int tvq_beam_reorder_workspace(int64_t n_pages, int64_t rows, int64_t new_rows, int64_t* bytes);
+TVQ_API int tvq_dev_beam_reorder(const int32_t* table, int64_t table_stride, const int32_t* lens, int64_t rows,
+                                 int64_t cols, const int32_t* parents, int64_t new_rows, const int32_t* refs,
+                                 void* k_pages, void* v_pages, const int64_t* shape, const int64_t* strides,
+                                 int32_t* new_table, int32_t* new_lens, int32_t* new_refs, int32_t* status, void* ws,
+                                 int64_t ws_bytes, void* stream);
 
 /* ================================================================ sessions
  * Device-resident GPT-2-shaped INT8 PTQ stack: embeddings, n_layers blocks of

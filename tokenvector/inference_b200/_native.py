@@ -25,6 +25,7 @@ TVQ_ERR_HANDLE = -6
 ACT_NONE, ACT_RELU, ACT_GELU_TANH, ACT_GELU_ERF = 0, 1, 2, 6
 FP8_REF, FP8_HW = 0, 1
 GEMM_I8, GEMM_F8 = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 
 P = C.c_void_p
 i64, i32, f32 = C.c_int64, C.c_int, C.c_float
@@ -107,6 +108,14 @@ SIGNATURES = {
     "tvq_dequantize_int4_grouped": (i32, [P, P, i64, i64, i64, P, i64, P]),
     "tvq_permute_cols": (i32, [P, P, i64, i64, P, i64, i32]),
     "tvq_matmul_int4_grouped": (i32, [P, P, P, i64, P, i64, i64, i64, i64, P, i64, P]),
+    "tvq_dev_paged_append": (i32, [i32, i32, P, P, P, P, i64, P, P, P, P, P, P, i64, i64, P, P, i64, i64, P]),
+    "tvq_paged_attention_workspace": (i32, [i64, i64, i64, i64, i64, i64, P]),
+    "tvq_dev_paged_attention": (i32, [i32, P, P, i64, P, P, P, P, P, i64, i64, P, P, i64, i64, i64, f32, i64, P, P, P,
+                                      i64, P]),
+    "tvq_beam_select_workspace": (i32, [i64, i64, i64, i64, P]),
+    "tvq_dev_beam_select": (i32, [i32, P, i64, P, P, i64, i64, i64, i64, i64, P, P, P, P, i64, P]),
+    "tvq_beam_reorder_workspace": (i32, [i64, i64, i64, P]),
+    "tvq_dev_beam_reorder": (i32, [P, i64, P, i64, i64, P, i64, P, P, P, P, P, P, P, P, P, P, i64, P]),
     "tvq_session_hidden": (i32, [i64, P]),
     "tvq_quantize_linear": (i32, [P, P, i64, i64, i64, P, i64, i64]),
     "tvq_dequantize_linear": (i32, [P, P, i64, i64, i64, P, i64, i64]),

@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "tvq_common.cuh"
+#include "tvq_decode.h"
 #include "tvq_kernels.h"
 
 namespace tvq {
@@ -103,6 +104,10 @@ int check_device_error(cudaStream_t st) {
         }
         if (h == DEVERR_BAD_INDEX) {
             set_error(TVQ_ERR_INVALID, "index out of range (a permutation entry outside [0, cols))");
+            return TVQ_ERR_INVALID;
+        }
+        if (h == DEVERR_BAD_PAGE) {
+            set_error(TVQ_ERR_INVALID, "page number outside the cache within a sequence's length");
             return TVQ_ERR_INVALID;
         }
         set_error(TVQ_ERR_TIMEOUT, "device-side wait timed out (code " + std::to_string(h) + ")");
@@ -1482,6 +1487,299 @@ int tvq_matmul_int4_grouped(const float* A, const uint8_t* packed_w, const float
     STEP(tvq_dev_matmul_int4_grouped(dA, dW, dB, dY, m, n, k, group_size, dS, dP, H.st()));
     TVQ_CUDA(cudaMemcpyAsync(Y, dY, sizeof(float) * m * n, cudaMemcpyDeviceToHost, H.st()));
     return check_device_error(H.st());
+    TVQ_CATCH
+}
+
+// ================================================================ decoding
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The cache's shape and strides into `c`: sizes within int32 where the kernels
+// index with it, everything 16-byte aligned.
+int paged_view(tvq::PagedView& c, int type, void* k, void* v, const int64_t* shape, const int64_t* strides,
+               const int32_t* table, int64_t table_stride, int64_t cols, const int32_t* ctx, const int32_t* cu,
+               int64_t n_seq, int64_t n_rows) {
+    TVQ_CHECK(type == TVQ_TYPE_F16 || type == TVQ_TYPE_BF16, TVQ_ERR_INVALID, "the cache holds F16 or BF16");
+    TVQ_CHECK(shape && strides, TVQ_ERR_INVALID, "null shape or strides");
+    TVQ_CHECK(n_seq >= 0 && n_rows >= 0 && cols >= 0 && shape[0] >= 0, TVQ_ERR_INVALID, "negative size");
+    TVQ_CHECK(shape[1] >= 8 && shape[1] <= 1024 && (shape[1] & (shape[1] - 1)) == 0, TVQ_ERR_UNSUPPORTED,
+              "page must be a power of two in [8, 1024]");
+    TVQ_CHECK(shape[2] >= 1 && shape[2] <= 65535, TVQ_ERR_INVALID, "kv heads out of range");
+    TVQ_CHECK(shape[3] >= 8 && shape[3] <= 128 && shape[3] % 8 == 0, TVQ_ERR_UNSUPPORTED,
+              "head dim must be a multiple of 8 up to 128");
+    TVQ_CHECK(n_seq < (1 << 24) && n_rows < (1ll << 31) && shape[0] < (1ll << 31) && cols < (1ll << 31) &&
+                  cols * shape[1] < (1ll << 31),
+              TVQ_ERR_UNSUPPORTED, "too many sequences, rows, pages or table columns");
+    TVQ_CHECK(cu || n_rows == n_seq, TVQ_ERR_SIZE, "without cu every sequence has one row");
+    TVQ_CHECK(table_stride >= cols, TVQ_ERR_SIZE, "table_stride smaller than the table's columns");
+    if (n_rows > 0) {
+        TVQ_CHECK(n_seq > 0 && table && ctx && (shape[0] == 0 || (k && v)), TVQ_ERR_INVALID, "null buffer");
+        TVQ_CHECK(aligned16(k) && aligned16(v), TVQ_ERR_UNSUPPORTED, "pages must be 16-byte aligned");
+        for (int i = 0; i < 6; i++)
+            TVQ_CHECK(strides[i] >= 0 && strides[i] % 8 == 0, TVQ_ERR_UNSUPPORTED,
+                      "cache strides must be non-negative multiples of 8 elements");
+    }
+    c.type = type;
+    c.k = k;
+    c.v = v;
+    c.n_pages = shape[0];
+    c.page = static_cast<int>(shape[1]);
+    while ((1 << c.page_log2) < c.page) c.page_log2++;
+    c.kv_heads = static_cast<int>(shape[2]);
+    c.dim = static_cast<int>(shape[3]);
+    c.k_page = strides[0];
+    c.k_tok = strides[1];
+    c.k_head = strides[2];
+    c.v_page = strides[3];
+    c.v_tok = strides[4];
+    c.v_head = strides[5];
+    c.table = table;
+    c.table_stride = table_stride;
+    c.n_cols = static_cast<int>(cols);
+    c.ctx = ctx;
+    c.cu = cu;
+    c.n_seq = static_cast<int>(n_seq);
+    c.n_rows = static_cast<int>(n_rows);
+    return TVQ_OK;
+}
+
+int check_ws(const void* ws, int64_t have, int64_t need) {
+    TVQ_CHECK(have >= need, TVQ_ERR_SIZE, "workspace too small");
+    TVQ_CHECK(need == 0 || (ws && (reinterpret_cast<uintptr_t>(ws) & 255) == 0), TVQ_ERR_INVALID,
+              "workspace null or not 256-byte aligned");
+    return TVQ_OK;
+}
+
+int select_args(tvq::BeamSelectArgs& a, int64_t batch, int64_t beams, int64_t keep, int64_t vocab) {
+    TVQ_CHECK(batch >= 0 && beams >= 0 && keep >= 0 && vocab >= 0, TVQ_ERR_INVALID, "negative size");
+    TVQ_CHECK(beams >= 1 && beams <= 64 && keep >= 1 && keep <= 64, TVQ_ERR_UNSUPPORTED,
+              "beams and keep must be in [1, 64]");
+    TVQ_CHECK(keep <= vocab, TVQ_ERR_SIZE, "keep larger than the vocabulary");
+    TVQ_CHECK(vocab < (1ll << 31) - 65536 && batch < (1ll << 24), TVQ_ERR_UNSUPPORTED,
+              "vocabulary or batch too large");
+    a.batch = static_cast<int>(batch);
+    a.beams = static_cast<int>(beams);
+    a.keep = static_cast<int>(keep);
+    a.vocab = static_cast<int>(vocab);
+    return TVQ_OK;
+}
+
+}  // namespace
+
+int tvq_dev_paged_append(int type, int src_type, const void* k, const void* v, const void* q,
+                         const int64_t* src_strides, int64_t q_heads, void* q_out, void* k_pages, void* v_pages,
+                         const int64_t* shape, const int64_t* strides, const int32_t* table, int64_t table_stride,
+                         int64_t cols, const int32_t* ctx_len, const int32_t* cu, int64_t n_seq, int64_t n_rows,
+                         void* stream) {
+    TVQ_TRY
+    AppendArgs a;
+    STEP(paged_view(a.c, type, k_pages, v_pages, shape, strides, table, table_stride, cols, ctx_len, cu, n_seq, n_rows));
+    TVQ_CHECK(src_type == TVQ_TYPE_F32 || src_type == TVQ_TYPE_F16 || src_type == TVQ_TYPE_BF16, TVQ_ERR_INVALID,
+              "unknown source type");
+    TVQ_CHECK(src_strides, TVQ_ERR_INVALID, "null strides");
+    TVQ_CHECK(q_heads >= 0 && q_heads <= 65535, TVQ_ERR_INVALID, "q heads out of range");
+    if (n_rows == 0) return TVQ_OK;
+    TVQ_CHECK(k && v && (!q || q_out), TVQ_ERR_INVALID, "null buffer");
+    TVQ_CHECK(aligned16(k) && aligned16(v) && aligned16(q) && aligned16(q_out), TVQ_ERR_UNSUPPORTED,
+              "rows must be 16-byte aligned");
+    const int64_t unit = src_type == TVQ_TYPE_F32 ? 4 : 8;
+    for (int i = 0; i < (q ? 6 : 4); i++)
+        TVQ_CHECK(src_strides[i] >= 0 && src_strides[i] % unit == 0, TVQ_ERR_UNSUPPORTED,
+                  "row strides must be non-negative multiples of 16 bytes");
+    a.src_type = src_type;
+    a.k = k;
+    a.v = v;
+    a.q = q_heads ? q : nullptr;
+    a.k_tok = src_strides[0];
+    a.k_head = src_strides[1];
+    a.v_tok = src_strides[2];
+    a.v_head = src_strides[3];
+    if (a.q) {
+        a.q_tok = src_strides[4];
+        a.q_head = src_strides[5];
+    }
+    a.q_heads = static_cast<int>(q_heads);
+    a.q_out = q_out;
+    return launch_paged_append(a, static_cast<cudaStream_t>(stream));
+    TVQ_CATCH
+}
+
+int tvq_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t n_seq, int64_t n_rows,
+                                  int64_t max_q, int64_t* bytes) {
+    TVQ_TRY
+    TVQ_CHECK(bytes, TVQ_ERR_INVALID, "null pointer");
+    TVQ_CHECK(kv_heads >= 1 && kv_heads <= 65535 && q_heads >= 1 && q_heads <= 65535 && q_heads % kv_heads == 0,
+              TVQ_ERR_INVALID, "q heads must be a multiple of the kv heads");
+    TVQ_CHECK(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, TVQ_ERR_UNSUPPORTED,
+              "head dim must be a multiple of 8 up to 128");
+    TVQ_CHECK(n_seq >= 0 && n_rows >= 0 && max_q >= 0, TVQ_ERR_INVALID, "negative size");
+    TVQ_CHECK(n_seq < (1 << 24) && n_rows < (1ll << 31), TVQ_ERR_UNSUPPORTED, "too many sequences or rows");
+    PagedAttnArgs a;
+    a.c.kv_heads = static_cast<int>(kv_heads);
+    a.c.dim = static_cast<int>(head_dim);
+    a.c.n_seq = static_cast<int>(n_seq);
+    a.c.n_rows = static_cast<int>(n_rows);
+    a.q_heads = static_cast<int>(q_heads);
+    a.max_q = static_cast<int>(std::min<int64_t>(max_q, n_rows));
+    return paged_attention_workspace(a, bytes);
+    TVQ_CATCH
+}
+
+int tvq_dev_paged_attention(int type, const void* q, const int64_t* q_strides, int64_t q_heads, const void* k_pages,
+                            const void* v_pages, const int64_t* shape, const int64_t* strides, const int32_t* table,
+                            int64_t table_stride, int64_t cols, const int32_t* ctx_len, const int32_t* cu,
+                            int64_t n_seq, int64_t n_rows, int64_t max_q, float scale, int64_t window, void* out,
+                            float* lse, void* ws, int64_t ws_bytes, void* stream) {
+    TVQ_TRY
+    PagedAttnArgs a;
+    STEP(paged_view(a.c, type, const_cast<void*>(k_pages), const_cast<void*>(v_pages), shape, strides, table,
+                    table_stride, cols, ctx_len, cu, n_seq, n_rows));
+    TVQ_CHECK(q_heads >= 1 && q_heads <= 65535 && q_heads % a.c.kv_heads == 0, TVQ_ERR_INVALID,
+              "q heads must be a multiple of the kv heads");
+    TVQ_CHECK(max_q >= 0 && window >= 0, TVQ_ERR_INVALID, "negative max_q or window");
+    TVQ_CHECK(n_rows * q_heads < (1ll << 31), TVQ_ERR_UNSUPPORTED, "too many rows");
+    if (n_rows == 0) return TVQ_OK;
+    TVQ_CHECK(q && out && q_strides, TVQ_ERR_INVALID, "null buffer");
+    TVQ_CHECK(aligned16(q) && aligned16(out) && q_strides[0] >= 0 && q_strides[0] % 8 == 0 && q_strides[1] >= 0 &&
+                  q_strides[1] % 8 == 0,
+              TVQ_ERR_UNSUPPORTED, "q and out must be 16-byte aligned, q strides multiples of 8 elements");
+    a.q = q;
+    a.q_tok = q_strides[0];
+    a.q_head = q_strides[1];
+    a.q_heads = static_cast<int>(q_heads);
+    a.max_q = static_cast<int>(std::min<int64_t>(max_q, n_rows));
+    a.window = static_cast<int>(std::min<int64_t>(window, (1ll << 31) - 1));
+    a.scale = scale;
+    a.out = out;
+    a.lse = lse;
+    int64_t need = 0;
+    STEP(paged_attention_workspace(a, &need));
+    STEP(check_ws(ws, ws_bytes, need));
+    a.ws = ws;
+    a.ws_bytes = ws_bytes;
+    return launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+    TVQ_CATCH
+}
+
+int tvq_beam_select_workspace(int64_t batch, int64_t beams, int64_t keep, int64_t vocab, int64_t* bytes) {
+    TVQ_TRY
+    TVQ_CHECK(bytes, TVQ_ERR_INVALID, "null pointer");
+    BeamSelectArgs a;
+    STEP(select_args(a, batch, beams, keep, vocab));
+    return beam_select_workspace(a, bytes);
+    TVQ_CATCH
+}
+
+int tvq_dev_beam_select(int type, const void* logits, int64_t stride, const float* scores, const uint8_t* finished,
+                        int64_t batch, int64_t beams, int64_t keep, int64_t vocab, int64_t eos, float* out_scores,
+                        int64_t* out_tokens, int32_t* out_parents, void* ws, int64_t ws_bytes, void* stream) {
+    TVQ_TRY
+    BeamSelectArgs a;
+    TVQ_CHECK(type == TVQ_TYPE_F32 || type == TVQ_TYPE_F16 || type == TVQ_TYPE_BF16, TVQ_ERR_INVALID,
+              "unknown logits type");
+    STEP(select_args(a, batch, beams, keep, vocab));
+    TVQ_CHECK(stride >= vocab, TVQ_ERR_SIZE, "logits rows overlap (stride smaller than the vocabulary)");
+    TVQ_CHECK(!finished || (eos >= 0 && eos < vocab), TVQ_ERR_INVALID, "finished beams need eos within the vocabulary");
+    if (batch == 0) return TVQ_OK;
+    TVQ_CHECK(logits && scores && out_scores && out_tokens && out_parents, TVQ_ERR_INVALID, "null buffer");
+    TVQ_CHECK((reinterpret_cast<uintptr_t>(logits) & (type == TVQ_TYPE_F32 ? 3 : 1)) == 0, TVQ_ERR_UNSUPPORTED,
+              "logits not aligned to their type");
+    a.type = type;
+    a.logits = logits;
+    a.stride = stride;
+    a.scores = scores;
+    a.finished = finished;
+    a.eos = static_cast<int>(eos);
+    a.out_scores = out_scores;
+    a.out_tokens = out_tokens;
+    a.out_parents = out_parents;
+    int64_t need = 0;
+    STEP(beam_select_workspace(a, &need));
+    STEP(check_ws(ws, ws_bytes, need));
+    a.ws = ws;
+    a.ws_bytes = ws_bytes;
+    return launch_beam_select(a, static_cast<cudaStream_t>(stream));
+    TVQ_CATCH
+}
+
+int tvq_beam_reorder_workspace(int64_t n_pages, int64_t rows, int64_t new_rows, int64_t* bytes) {
+    TVQ_TRY
+    TVQ_CHECK(bytes, TVQ_ERR_INVALID, "null pointer");
+    TVQ_CHECK(n_pages >= 0 && rows >= 0 && new_rows >= 0, TVQ_ERR_INVALID, "negative size");
+    TVQ_CHECK(n_pages < (1ll << 31) && rows <= 65535 && new_rows <= 65535, TVQ_ERR_UNSUPPORTED,
+              "too many pages or rows");
+    BeamReorderArgs a;
+    a.n_pages = n_pages;
+    a.rows = static_cast<int>(rows);
+    a.new_rows = static_cast<int>(new_rows);
+    return beam_reorder_workspace(a, bytes);
+    TVQ_CATCH
+}
+
+int tvq_dev_beam_reorder(const int32_t* table, int64_t table_stride, const int32_t* lens, int64_t rows, int64_t cols,
+                         const int32_t* parents, int64_t new_rows, const int32_t* refs, void* k_pages, void* v_pages,
+                         const int64_t* shape, const int64_t* strides, int32_t* new_table, int32_t* new_lens,
+                         int32_t* new_refs, int32_t* status, void* ws, int64_t ws_bytes, void* stream) {
+    TVQ_TRY
+    BeamReorderArgs a;
+    TVQ_CHECK(shape && strides, TVQ_ERR_INVALID, "null shape or strides");
+    TVQ_CHECK(rows >= 0 && new_rows >= 0 && cols >= 0 && shape[0] >= 0 && shape[4] >= 0, TVQ_ERR_INVALID,
+              "negative size");
+    TVQ_CHECK(rows <= 65535 && new_rows <= 65535 && shape[0] < (1ll << 31) && shape[4] <= 16383 &&
+                  cols * shape[1] < (1ll << 31) && cols < (1ll << 31),
+              TVQ_ERR_UNSUPPORTED, "too many rows, pages, layers or table columns");
+    TVQ_CHECK(shape[1] >= 8 && shape[1] <= 1024 && (shape[1] & (shape[1] - 1)) == 0, TVQ_ERR_UNSUPPORTED,
+              "page must be a power of two in [8, 1024]");
+    TVQ_CHECK(shape[2] >= 1 && shape[2] <= 65535, TVQ_ERR_INVALID, "kv heads out of range");
+    TVQ_CHECK(shape[3] >= 8 && shape[3] <= 128 && shape[3] % 8 == 0, TVQ_ERR_UNSUPPORTED,
+              "head dim must be a multiple of 8 up to 128");
+    TVQ_CHECK(table_stride >= cols, TVQ_ERR_SIZE, "table_stride smaller than the table's columns");
+    TVQ_CHECK((rows * cols == 0 || table) && (rows == 0 || lens) && (new_rows == 0 || (parents && new_lens)) &&
+                  (new_rows * cols == 0 || new_table) && (shape[0] == 0 || (refs && new_refs)) && status,
+              TVQ_ERR_INVALID, "null buffer");
+    TVQ_CHECK(new_table != table && new_lens != lens && (shape[0] == 0 || new_refs != refs), TVQ_ERR_INVALID,
+              "the new tables, lengths and counts must lie apart from the old ones");
+    if (shape[4] > 0 && shape[0] > 0) {
+        TVQ_CHECK(k_pages && v_pages, TVQ_ERR_INVALID, "null buffer");
+        TVQ_CHECK(aligned16(k_pages) && aligned16(v_pages), TVQ_ERR_UNSUPPORTED, "pages must be 16-byte aligned");
+        for (int i = 0; i < 8; i++)
+            TVQ_CHECK(strides[i] >= 0 && strides[i] % 8 == 0, TVQ_ERR_UNSUPPORTED,
+                      "cache strides must be non-negative multiples of 8 elements");
+    }
+    a.table = table;
+    a.table_stride = table_stride;
+    a.lens = lens;
+    a.rows = static_cast<int>(rows);
+    a.cols = static_cast<int>(cols);
+    a.parents = parents;
+    a.new_rows = static_cast<int>(new_rows);
+    a.refs = refs;
+    a.n_pages = shape[0];
+    a.new_table = new_table;
+    a.new_lens = new_lens;
+    a.new_refs = new_refs;
+    a.status = status;
+    a.k = k_pages;
+    a.v = v_pages;
+    a.page = static_cast<int>(shape[1]);
+    a.kv_heads = static_cast<int>(shape[2]);
+    a.dim = static_cast<int>(shape[3]);
+    a.layers = static_cast<int>(shape[4]);
+    a.k_layer = strides[0];
+    a.k_page = strides[1];
+    a.k_tok = strides[2];
+    a.k_head = strides[3];
+    a.v_layer = strides[4];
+    a.v_page = strides[5];
+    a.v_tok = strides[6];
+    a.v_head = strides[7];
+    int64_t need = 0;
+    STEP(beam_reorder_workspace(a, &need));
+    STEP(check_ws(ws, ws_bytes, need));
+    a.ws = ws;
+    a.ws_bytes = ws_bytes;
+    return launch_beam_reorder(a, static_cast<cudaStream_t>(stream));
     TVQ_CATCH
 }
 

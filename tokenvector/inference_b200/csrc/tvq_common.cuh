@@ -53,6 +53,7 @@ enum : int {
     DEVERR_TIMEOUT_ROWS = 5,  // a row copy of the per-channel quantizer
     DEVERR_TIMEOUT_TEST = 9,
     DEVERR_BAD_INDEX = 60,  // an index operand out of range (not a timeout)
+    DEVERR_BAD_PAGE = 62,   // a page number outside the cache within a sequence's length
     DEVERR_FIX_FULL = 61,   // more undecided int8 attention rows than the fix-up lists hold
 };
 

@@ -1,0 +1,193 @@
+// tvq_paged.cu -- the paged cache of a decoding loop: writing the keys and
+// values of new tokens into it, and the attention of those tokens over it.
+//
+// A sequence s owns n_s new rows (its chunk) and L_s tokens in the cache, the
+// new ones included; row i sits at position p = L_s - n_s + i.  Token j of s
+// lies in page table[s][j / P], slot j % P.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "tvq_common.cuh"
+#include "tvq_decode.h"
+
+namespace tvq {
+
+namespace {
+
+// ---------------------------------------------------------------- types
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// 8 consecutive elements: loaded as 16-byte words, rounded once to T
+template <typename T, typename S>
+__device__ __forceinline__ uint4 load8(const S* p) {
+    if constexpr (sizeof(S) == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        union { T t[8]; uint4 u; } r;
+        r.t[0] = from_f32<T>(a.x); r.t[1] = from_f32<T>(a.y); r.t[2] = from_f32<T>(a.z); r.t[3] = from_f32<T>(a.w);
+        r.t[4] = from_f32<T>(b.x); r.t[5] = from_f32<T>(b.y); r.t[6] = from_f32<T>(b.z); r.t[7] = from_f32<T>(b.w);
+        return r.u;
+    } else {
+        union { S s[8]; uint4 u; } a;
+        a.u = __ldg(reinterpret_cast<const uint4*>(p));
+        if constexpr (std::is_same<T, S>::value) return a.u;
+        union { T t[8]; uint4 u; } r;
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.t[i] = from_f32<T>(to_f32(a.s[i]));
+        return r.u;
+    }
+}
+
+// The sequence that packed row `row` belongs to (the last s with cu[s] <= row).
+__device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seq, int row) {
+    int lo = 0, hi = n_seq;  // cu[lo] <= row < cu[hi] (cu[n_seq] taken as the end)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(cu + mid) <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------- append
+// Bound: memory (each value is read once and written once).  One thread per
+// 8 values of one row.
+template <typename T, typename S>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int* err) {
+    griddep_wait();
+    const int row = blockIdx.y * 65535 + blockIdx.z;
+    if (row >= a.c.n_rows) return;
+    const int d8 = a.c.dim >> 3;
+    const int kv = a.c.kv_heads * d8, total = 2 * kv + (a.q ? a.q_heads * d8 : 0);
+    const int u = blockIdx.x * 256 + threadIdx.x;
+    if (u >= total) return;
+    if (u >= 2 * kv) {
+        const int h = (u - 2 * kv) / d8, c = (u - 2 * kv) - h * d8;
+        const uint4 x = load8<T>(static_cast<const S*>(a.q) + row * a.q_tok + h * a.q_head + c * 8);
+        reinterpret_cast<uint4*>(a.q_out)[(static_cast<int64_t>(row) * a.q_heads + h) * d8 + c] = x;
+        return;
+    }
+    const int s = a.c.cu ? seq_of_row(a.c.cu, a.c.n_seq, row) : row;
+    const int n = a.c.cu ? __ldg(a.c.cu + s + 1) - __ldg(a.c.cu + s) : 1;
+    const int i = a.c.cu ? row - __ldg(a.c.cu + s) : 0;
+    const int p = __ldg(a.c.ctx + s) - n + i;
+    if (i < 0 || i >= n || p < 0) return;  // a row before the cache's first token (or of no sequence) is dropped
+    const int col = p >> a.c.page_log2, slot = p & (a.c.page - 1);
+    const int pg = col < a.c.n_cols ? __ldg(a.c.table + s * a.c.table_stride + col) : -1;
+    if (static_cast<unsigned>(pg) >= static_cast<unsigned>(a.c.n_pages)) {
+        record_error(err, DEVERR_BAD_PAGE);
+        return;
+    }
+    const bool is_v = u >= kv;
+    const int w = is_v ? u - kv : u;
+    const int h = w / d8, c = w - h * d8;
+    if (is_v) {
+        const uint4 x = load8<T>(static_cast<const S*>(a.v) + row * a.v_tok + h * a.v_head + c * 8);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.c.v) + pg * a.c.v_page + slot * a.c.v_tok + h * a.c.v_head + c * 8) = x;
+    } else {
+        const uint4 x = load8<T>(static_cast<const S*>(a.k) + row * a.k_tok + h * a.k_head + c * 8);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.c.k) + pg * a.c.k_page + slot * a.c.k_tok + h * a.c.k_head + c * 8) = x;
+    }
+}
+
+// ---------------------------------------------------------------- attention
+// The plain kernel: one warp per (row, head), keys one after another, the
+// softmax's running maximum and sum in f32 (m' = max(m, s), l' = l 2^(m - m')
+// + 2^(s - m'), o' likewise), four values of the head dim per lane.
+template <typename T>
+__global__ void __launch_bounds__(128) paged_attention_row_kernel(const PagedAttnArgs a, int* err) {
+    griddep_wait();
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (unit >= static_cast<int64_t>(a.c.n_rows) * a.q_heads) return;
+    const int row = static_cast<int>(unit / a.q_heads), h = static_cast<int>(unit - static_cast<int64_t>(row) * a.q_heads);
+    const int hk = h / (a.q_heads / a.c.kv_heads);
+    const int s = a.c.cu ? seq_of_row(a.c.cu, a.c.n_seq, row) : row;
+    const int n = a.c.cu ? __ldg(a.c.cu + s + 1) - __ldg(a.c.cu + s) : 1;
+    const int i = a.c.cu ? row - __ldg(a.c.cu + s) : 0;
+    if (i < 0 || i >= n || i >= a.max_q) return;  // a row of no sequence
+    const int p = __ldg(a.c.ctx + s) - n + i;
+    const float scale2 = a.scale * 1.4426950408889634f;
+    float q[4], o[4] = {0, 0, 0, 0};
+    const int d0 = lane * 4;
+    const bool in = d0 < a.c.dim;
+    const T* qp = static_cast<const T*>(a.q) + row * a.q_tok + h * a.q_head + d0;
+    for (int c = 0; c < 4; c++) q[c] = in ? to_f32(qp[c]) * scale2 : 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const int first = a.window > 0 ? max(0, p - a.window + 1) : 0;
+    for (int j = first; j <= p; j++) {
+        const int col = j >> a.c.page_log2, slot = j & (a.c.page - 1);
+        const int pg = col < a.c.n_cols ? __ldg(a.c.table + s * a.c.table_stride + col) : -1;
+        float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
+        if (static_cast<unsigned>(pg) >= static_cast<unsigned>(a.c.n_pages)) {
+            record_error(err, DEVERR_BAD_PAGE);
+        } else if (in) {
+            const T* kp = static_cast<const T*>(a.c.k) + pg * a.c.k_page + slot * a.c.k_tok + hk * a.c.k_head + d0;
+            const T* vp = static_cast<const T*>(a.c.v) + pg * a.c.v_page + slot * a.c.v_tok + hk * a.c.v_head + d0;
+            for (int c = 0; c < 4; c++) { k[c] = to_f32(kp[c]); v[c] = to_f32(vp[c]); }
+        }
+        float x = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+        for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+        const float m2 = fmaxf(m, x);
+        const float f = m2 == -INFINITY ? 0.0f : exp2f(m - m2), e = m2 == -INFINITY ? 0.0f : exp2f(x - m2);
+        m = m2;
+        l = l * f + e;
+        for (int c = 0; c < 4; c++) o[c] = o[c] * f + e * v[c];
+    }
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    T* op = static_cast<T*>(a.out) + unit * a.c.dim + d0;
+    if (in)
+        for (int c = 0; c < 4; c++) op[c] = from_f32<T>(o[c] * inv);
+    if (lane == 0 && a.lse) a.lse[unit] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace
+
+int launch_paged_append(const AppendArgs& a, cudaStream_t st) {
+    int rc = 0;
+    DeviceState* ds = device_state(&rc);
+    if (!ds) return rc;
+    if (a.c.n_rows == 0) return TVQ_OK;
+    const int d8 = a.c.dim / 8;
+    const int64_t total = 2ll * a.c.kv_heads * d8 + (a.q ? static_cast<int64_t>(a.q_heads) * d8 : 0);
+    const dim3 grid(static_cast<unsigned>((total + 255) / 256), static_cast<unsigned>((a.c.n_rows + 65534) / 65535),
+                    static_cast<unsigned>(std::min(a.c.n_rows, 65535)));
+#define TVQ_APPEND(T, S) return launch_pdl(paged_append_kernel<T, S>, grid, dim3(256), 0, st, a, ds->d_error)
+    if (a.c.type == TVQ_TYPE_F16) {
+        if (a.src_type == TVQ_TYPE_F32) TVQ_APPEND(__half, float);
+        if (a.src_type == TVQ_TYPE_F16) TVQ_APPEND(__half, __half);
+        TVQ_APPEND(__half, __nv_bfloat16);
+    }
+    if (a.src_type == TVQ_TYPE_F32) TVQ_APPEND(__nv_bfloat16, float);
+    if (a.src_type == TVQ_TYPE_F16) TVQ_APPEND(__nv_bfloat16, __half);
+    TVQ_APPEND(__nv_bfloat16, __nv_bfloat16);
+#undef TVQ_APPEND
+}
+
+int paged_attention_workspace(const PagedAttnArgs&, int64_t* bytes) {
+    *bytes = 0;
+    return TVQ_OK;
+}
+
+int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
+    int rc = 0;
+    DeviceState* ds = device_state(&rc);
+    if (!ds) return rc;
+    if (a.c.n_rows == 0) return TVQ_OK;
+    const int64_t units = static_cast<int64_t>(a.c.n_rows) * a.q_heads;
+    const dim3 grid(static_cast<unsigned>((units + 3) / 4));
+    if (a.c.type == TVQ_TYPE_F16)
+        return launch_pdl(paged_attention_row_kernel<__half>, grid, dim3(128), 0, st, a, ds->d_error);
+    return launch_pdl(paged_attention_row_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a, ds->d_error);
+}
+
+}  // namespace tvq

@@ -1,0 +1,3 @@
+"""Decoding: a paged key/value cache, attention of new tokens over it, and beam search on the device."""
+from .beam import beam_reorder, beam_select  # noqa: F401
+from .paged import paged_append, paged_attention  # noqa: F401
