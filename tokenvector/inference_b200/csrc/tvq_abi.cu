@@ -1649,7 +1649,7 @@ int tvq_dev_paged_attention(int type, const void* q, const int64_t* q_strides, i
     a.q_head = q_strides[1];
     a.q_heads = static_cast<int>(q_heads);
     a.max_q = static_cast<int>(std::min<int64_t>(max_q, n_rows));
-    a.window = static_cast<int>(std::min<int64_t>(window, (1ll << 31) - 1));
+    a.window = static_cast<int>(std::min<int64_t>(window, 1 << 30));
     a.scale = scale;
     a.out = out;
     a.lse = lse;

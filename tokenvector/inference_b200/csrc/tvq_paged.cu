@@ -1,5 +1,5 @@
 // tvq_paged.cu -- the paged cache of a decoding loop: writing the keys and
-// values of new tokens into it, and the attention of those tokens over it.
+// values of new tokens into it.
 //
 // A sequence s owns n_s new rows (its chunk) and L_s tokens in the cache, the
 // new ones included; row i sits at position p = L_s - n_s + i.  Token j of s
@@ -99,57 +99,6 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, i
     }
 }
 
-// ---------------------------------------------------------------- attention
-// The plain kernel: one warp per (row, head), keys one after another, the
-// softmax's running maximum and sum in f32 (m' = max(m, s), l' = l 2^(m - m')
-// + 2^(s - m'), o' likewise), four values of the head dim per lane.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attention_row_kernel(const PagedAttnArgs a, int* err) {
-    griddep_wait();
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (unit >= static_cast<int64_t>(a.c.n_rows) * a.q_heads) return;
-    const int row = static_cast<int>(unit / a.q_heads), h = static_cast<int>(unit - static_cast<int64_t>(row) * a.q_heads);
-    const int hk = h / (a.q_heads / a.c.kv_heads);
-    const int s = a.c.cu ? seq_of_row(a.c.cu, a.c.n_seq, row) : row;
-    const int n = a.c.cu ? __ldg(a.c.cu + s + 1) - __ldg(a.c.cu + s) : 1;
-    const int i = a.c.cu ? row - __ldg(a.c.cu + s) : 0;
-    if (i < 0 || i >= n || i >= a.max_q) return;  // a row of no sequence
-    const int p = __ldg(a.c.ctx + s) - n + i;
-    const float scale2 = a.scale * 1.4426950408889634f;
-    float q[4], o[4] = {0, 0, 0, 0};
-    const int d0 = lane * 4;
-    const bool in = d0 < a.c.dim;
-    const T* qp = static_cast<const T*>(a.q) + row * a.q_tok + h * a.q_head + d0;
-    for (int c = 0; c < 4; c++) q[c] = in ? to_f32(qp[c]) * scale2 : 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    const int first = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    for (int j = first; j <= p; j++) {
-        const int col = j >> a.c.page_log2, slot = j & (a.c.page - 1);
-        const int pg = col < a.c.n_cols ? __ldg(a.c.table + s * a.c.table_stride + col) : -1;
-        float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-        if (static_cast<unsigned>(pg) >= static_cast<unsigned>(a.c.n_pages)) {
-            record_error(err, DEVERR_BAD_PAGE);
-        } else if (in) {
-            const T* kp = static_cast<const T*>(a.c.k) + pg * a.c.k_page + slot * a.c.k_tok + hk * a.c.k_head + d0;
-            const T* vp = static_cast<const T*>(a.c.v) + pg * a.c.v_page + slot * a.c.v_tok + hk * a.c.v_head + d0;
-            for (int c = 0; c < 4; c++) { k[c] = to_f32(kp[c]); v[c] = to_f32(vp[c]); }
-        }
-        float x = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-        for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        const float m2 = fmaxf(m, x);
-        const float f = m2 == -INFINITY ? 0.0f : exp2f(m - m2), e = m2 == -INFINITY ? 0.0f : exp2f(x - m2);
-        m = m2;
-        l = l * f + e;
-        for (int c = 0; c < 4; c++) o[c] = o[c] * f + e * v[c];
-    }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    T* op = static_cast<T*>(a.out) + unit * a.c.dim + d0;
-    if (in)
-        for (int c = 0; c < 4; c++) op[c] = from_f32<T>(o[c] * inv);
-    if (lane == 0 && a.lse) a.lse[unit] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-}
-
 }  // namespace
 
 int launch_paged_append(const AppendArgs& a, cudaStream_t st) {
@@ -171,23 +120,6 @@ int launch_paged_append(const AppendArgs& a, cudaStream_t st) {
     if (a.src_type == TVQ_TYPE_F16) TVQ_APPEND(__nv_bfloat16, __half);
     TVQ_APPEND(__nv_bfloat16, __nv_bfloat16);
 #undef TVQ_APPEND
-}
-
-int paged_attention_workspace(const PagedAttnArgs&, int64_t* bytes) {
-    *bytes = 0;
-    return TVQ_OK;
-}
-
-int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
-    int rc = 0;
-    DeviceState* ds = device_state(&rc);
-    if (!ds) return rc;
-    if (a.c.n_rows == 0) return TVQ_OK;
-    const int64_t units = static_cast<int64_t>(a.c.n_rows) * a.q_heads;
-    const dim3 grid(static_cast<unsigned>((units + 3) / 4));
-    if (a.c.type == TVQ_TYPE_F16)
-        return launch_pdl(paged_attention_row_kernel<__half>, grid, dim3(128), 0, st, a, ds->d_error);
-    return launch_pdl(paged_attention_row_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a, ds->d_error);
 }
 
 }  // namespace tvq
