@@ -147,11 +147,13 @@ SHAPES = [
     ([513], [513], 1, 1, 8, 8),
     ([140], [100], 2, 2, 128, 16),
     ([64], [4096], 16, 2, 128, 64),                     # few rows, many keys
+    ([1] * 30, [2000 + 37 * i for i in range(30)], 8, 4, 128, 16),  # many tiles for every SM
+    ([2] * 30, [4000 + 41 * i for i in range(30)], 4, 4, 64, 32),
 ]
 
 
 @pytest.mark.parametrize("kind", ["float16", "bfloat16"])
-@pytest.mark.parametrize("case", SHAPES, ids=lambda c: "-".join(str(x).replace(" ", "") for x in c)[:60])
+@pytest.mark.parametrize("case", SHAPES, ids=lambda c: "-".join(str(x).replace(" ", "") for x in c)[-60:])
 def test_attention_follows_its_definition(case, kind):
     s = make(*case, kind, seed=len(case[0]) + case[4], head_major=case[5] % 32 == 0, wide_table=5)
     want = definition(s)

@@ -1520,6 +1520,27 @@ int make_tma_f16_sw128(CUtensorMap* map, const void* ptr, int64_t rows, int64_t 
     return make_map(map, ptr, rows, cols, box_rows, 2, pitch);
 }
 
+int make_tma_16bit(CUtensorMap* map, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box) {
+    int rc = get_encoder();
+    if (rc) return rc;
+    cuuint64_t d[5], st[4];
+    cuuint32_t b[5], es[5] = {1, 1, 1, 1, 1};
+    for (int i = 0; i < rank; i++) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i > 0) st[i - 1] = dims[i] > 1 ? strides[i - 1] : 16;
+    }
+    const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+                                const_cast<void*>(ptr), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    TVQ_CHECK(r == CUDA_SUCCESS, TVQ_ERR_UNSUPPORTED,
+              "strides that a tensor map cannot hold (cuTensorMapEncodeTiled code " +
+                  std::to_string(static_cast<int>(r)) + ")");
+    return TVQ_OK;
+}
+
 int launch_gemm(const GemmArgs& g, cudaStream_t st) {
     TVQ_CHECK(g.m >= 0 && g.n >= 0 && g.k >= 0, TVQ_ERR_INVALID, "negative GEMM size");
     TVQ_CHECK(g.m < (1ll << 31) && g.n < (1ll << 31) && g.k < 133143, TVQ_ERR_UNSUPPORTED,

@@ -98,6 +98,11 @@ int make_tma_f32_sw128(CUtensorMap* map, const float* ptr, int64_t rows, int64_t
 // The same for fp16 [rows, cols]: box of 64 columns x box_rows rows.
 int make_tma_f16_sw128(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int box_rows,
                        int64_t pitch = 0);
+// Tensor map of 2-byte elements, 2 to 5 dimensions (innermost first; strides
+// in bytes of dimensions 1 ..), 128-byte swizzle.  Moved as bits: both f16
+// and bf16.  A dimension of one entry may have any stride.
+int make_tma_16bit(CUtensorMap* map, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box);
 // x = hi + lo with hi rounded to TF32 precision (10 explicit mantissa bits)
 int launch_split_tf32(const float* x, float* hi, float* lo, int64_t n, cudaStream_t st);
 // tvq_int4.cu: group-wise INT4 (int4.tkv).  zps == nullptr: symmetric

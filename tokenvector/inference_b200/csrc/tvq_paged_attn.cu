@@ -9,20 +9,20 @@
 // so the keys are read once and parts are joined at the end.  The query heads
 // that share a kv head are rows of one product: row r = i * group + g.
 //
-// attn_rows_kernel: sequences of at most 32 such rows (single tokens, a few
-// drafted ones).  Every key and value is used for at most 32 rows, so the
+// attn_rows_kernel: sequences of at most 16 such rows (single tokens, a few
+// drafted ones).  Every key and value is used for at most 16 rows, so the
 // bytes of the cache bound it, and what counts is that enough of them are in
 // flight and that every SM has the same share:
-//  - one CTA per SM; all 16-key tiles of all (sequence, kv head) pairs stand
+//  - one CTA per SM; all 32-key tiles of all (sequence, kv head) pairs stand
 //    in one line, and CTA c takes the c-th equal piece of it, whatever the
 //    lengths.  Every CTA finds its piece from the lengths on the device.
-//  - the eight warps of a CTA are pipelines of their own: warp w takes the
-//    tiles w, w + 8, ... of a pair, brings them through its own ring in
-//    shared memory (cp.async, no barrier), and keeps its own m, l, o.  The
-//    ring runs on across the ends of pairs, so the next pair's tiles are on
-//    their way while the warps join their parts of this one.
-//  - mma.sync m16n8k16 with the rows padded to 16 or 32: at D = 128 the two
-//    products take 64 of an SM's ~350 cycles per 16 KB of cache, so that the
+//  - two producer warps (keys, values) bring the piece's tiles through a 192 KB
+//    ring by TMA (a tile's pages are boxes of a {value, token, half, head,
+//    page} tensor map, so any strides will do), across the ends of pairs; six
+//    consumer warps take the tiles in turn, each with its own m, l, o, and join them at the end
+//    of a pair, while the next pair's tiles are on their way.
+//  - mma.sync m16n8k16 with the rows padded to 16: at D = 128 the products
+//    of a 16 KB tile take 128 of the ~650 cycles that its bytes take, so the
 //    wider tcgen05 tile (128 rows) would buy nothing here.
 //  - a pair that several CTAs share is joined by the one that finishes last
 //    (a counter per CTA in the workspace, zero between calls), in the order
@@ -34,14 +34,19 @@
 
 #include "tvq_common.cuh"
 #include "tvq_decode.h"
+#include "tvq_kernels.h"
 
 namespace tvq {
 
 namespace {
 
-constexpr int KT = 16;      // keys per tile
-constexpr int NW = 8;       // warps per CTA of the rows kernel
-constexpr int NTHR = NW * 32;
+constexpr int NW = 6;              // consumer warps of the rows kernel
+constexpr int NC = NW * 32;        // consumer threads
+constexpr int NTHR = NC + 64;      // and two producer warps
+constexpr int MAX_ROWS = 16;       // rows of a pair (new tokens x heads of the group)
+
+// device error codes: the wait that gave up first
+enum : int { DEVERR_PATTN_EMPTY = 71, DEVERR_PATTN_FULL = 72, DEVERR_PATTN_DRAIN = 73 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error ~2^-22, 2^-inf = 0
     float y;
@@ -62,15 +67,14 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 16 bytes global -> shared; zeros when !in (the address is then not read)
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
-    const int n = in ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// 5-D TMA tile load {value, token, half, head, page}; what lies outside is zero.
+__device__ __forceinline__ void tma_load_5d(const CUtensorMap* map, uint64_t* bar, uint32_t dst, int c0, int c1, int c2,
+                                            int c3, int c4) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+        : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -120,8 +124,9 @@ __device__ __forceinline__ Seq load_seq(const PagedView& c, int s) {
     return q;
 }
 
-// The 16-key tiles [first, end) that the rows of a sequence see together: one
-// at least, so that rows without keys are written too.
+// The tiles of KT keys [first, end) that the rows of a sequence see together:
+// one at least, so that rows without keys are written too.
+template <int KT>
 __device__ __forceinline__ int2 seq_tiles(const Seq& q, int window) {
     const int p0 = q.len - q.n;
     const int first = window > 0 ? max(0, p0 - window + 1) / KT : 0;
@@ -129,53 +134,77 @@ __device__ __forceinline__ int2 seq_tiles(const Seq& q, int window) {
 }
 
 // ---------------------------------------------------------------- few rows
-template <int DP, int MT>
+template <int DP>
 struct RowsCfg {
-    static constexpr int ROWB = DP * 2;                  // bytes of a key
-    static constexpr int STAGE = 2 * KT * ROWB;          // one tile: keys, then values
-    static constexpr int STAGES = DP == 128 ? 3 : 6;     // 192 KB of ring either way
-    static constexpr int RING = NW * STAGES * STAGE;
-    static constexpr int PART = 16 * DP * 4;             // one warp's o of 16 rows
-    static constexpr int OFF_PART = RING;                // [4][16][DP] f32
-    static constexpr int OFF_ML = OFF_PART + 4 * PART;   // float2 [MLB][NW][16 * MT]
-    static constexpr int MLB = DP == 128 && MT == 2 ? 1 : 2;  // two, as far as they fit: one barrier less
-    static constexpr int SMEM = OFF_ML + MLB * NW * 16 * MT * 8;
-    static constexpr int64_t SLOT = 16 * MT * (DP * 4 + 8);  // workspace bytes of one partial
+    static constexpr int KT = 32;                        // keys per tile
+    static constexpr int HALF = KT * 128;                // 64 values of a tile's keys, 128-byte swizzle
+    static constexpr int HALVES = DP / 64;
+    static constexpr int STAGE = 2 * HALVES * HALF;      // one tile: keys, then values
+    static constexpr int STAGES = 196608 / STAGE;        // 24 or 12
+    // A stage is always the same warp's, which waits for its phases one after
+    // another.  Were it to pass from warp to warp, one that is ahead could take
+    // the parity of the phase before last for that of the one it waits for.
+    static_assert(STAGES % NW == 0);
+    static constexpr int OFF_PART = STAGES * STAGE;      // [NW / 2][16][DP] f32
+    static constexpr int OFF_ML = OFF_PART + NW / 2 * 16 * DP * 4;     // float2 [2][NW][16]
+    static constexpr int OFF_BAR = OFF_ML + 2 * NW * 16 * 8;      // full[STAGES], empty[STAGES]
+    static constexpr int OFF_MISC = OFF_BAR + 2 * STAGES * 8;     // scan[NW + 2], last, at[2]
+    static constexpr int SMEM = OFF_MISC + 64;
+    static constexpr int64_t SLOT = 16 * (DP * 4 + 8);   // workspace bytes of one partial
 };
 
 struct RowsPlan {
     int* counters;   // [grid]
     uint8_t* parts;  // [grid][2] slots
     int min_tiles;   // no CTA gets a smaller piece
+    // One TMA load: `box` tokens (a power of two: a page, or a tile of a larger
+    // one) of 64 values, or of both halves (box_halves 2: 128 values and box =
+    // KT).  by_value: the head dim is no multiple of 64, the halves start at
+    // values 0 and 64 of one dimension that ends with the head dim.
+    int box, box_halves, by_value;
 };
 
-// Where a warp stands in its CTA's piece: a pair and a tile of it.
+// Where a walk over a CTA's piece stands: a pair and its tiles in the piece.
 struct Cursor {
     int s, hk;
-    int64_t left;  // tiles of the piece from this pair's first tile in it on
+    int64_t left;    // tiles of the piece from this pair's first one on
     Seq q;
-    int t, end;    // this warp's next tile, the end of the pair's tiles in the piece
-    int first;     // the pair's first tile in the piece
-    int2 all;      // the pair's tiles
+    int2 all;        // the pair's tiles
+    int first, end;  // those in the piece
 };
 
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(NTHR, 1) attn_rows_kernel(const PagedAttnArgs a, const RowsPlan plan, int* err) {
-    using C = RowsCfg<DP, MT>;
-    extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ int s_scan[NW];
-    __shared__ int64_t s_at[2];
-    __shared__ int s_last;
+template <typename T, int DP>
+__global__ void __launch_bounds__(NTHR, 1)
+    attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const PagedAttnArgs a, const RowsPlan plan, int* err) {
+    using C = RowsCfg<DP>;
+    constexpr int KT = C::KT;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+    uint64_t* empty = full + C::STAGES;
+    int* s_scan = reinterpret_cast<int*>(sm + C::OFF_MISC);
+    int* s_last = s_scan + NW + 2;
+    int64_t* s_at = reinterpret_cast<int64_t*>(s_scan + NW + 4);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.q_heads / a.c.kv_heads;
+    const int fit = MAX_ROWS / group;  // new rows of a sequence that this kernel takes
+    if (tid == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(full + i, 2);
+            mbar_init(empty + i, 1);
+        }
+        fence_barrier_init();
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+    }
     griddep_wait();
 
     // ---- this CTA's piece of the line of tiles
     auto weight = [&](int s) -> int {
         if (s >= a.c.n_seq) return 0;
         const Seq q = load_seq(a.c, s);
-        if (q.n == 0 || q.n > 16 * MT / group) return 0;
-        const int2 t = seq_tiles(q, a.window);
+        if (q.n == 0 || q.n > fit) return 0;
+        const int2 t = seq_tiles<KT>(q, a.window);
         return t.y - t.x;
     };
     auto scan = [&](int x, int* all) {  // inclusive, over the CTA
@@ -187,7 +216,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_rows_kernel(const PagedAttnArgs 
         if (lane == 31) s_scan[warp] = x;
         __syncthreads();
         int sum = 0;
-        for (int w = 0; w < NW; w++) {
+        for (int w = 0; w < NW + 2; w++) {
             if (w < warp) x += s_scan[w];
             sum += s_scan[w];
         }
@@ -208,7 +237,7 @@ __global__ void __launch_bounds__(NTHR, 1) attn_rows_kernel(const PagedAttnArgs 
     if (begin >= stop) return;
     int64_t before = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += NTHR) {
-        int all;
+        int all = 0;
         int w = w0, inc = inc0;
         if (a.c.n_seq > NTHR) {
             w = weight(s0 + tid);
@@ -219,207 +248,226 @@ __global__ void __launch_bounds__(NTHR, 1) attn_rows_kernel(const PagedAttnArgs 
             s_at[0] = s0 + tid;
             s_at[1] = lo;
         }
-        if (a.c.n_seq > NTHR) before += all;
+        before += all;
     }
     __syncthreads();
 
     Cursor cur;
-    cur.s = static_cast<int>(s_at[0]);
-    const int64_t in_seq = begin - s_at[1];
-    auto enter = [&](Cursor& c, int skip) {  // c.s, c.hk, c.left set; the pair's tiles from `skip` on
-        c.all = seq_tiles(c.q, a.window);
-        c.first = c.all.x + skip;
-        c.end = static_cast<int>(min(static_cast<int64_t>(c.all.y), c.first + c.left));
-        c.t = c.first + warp;
+    auto enter = [&](int skip) {  // cur.s, hk, left and q set: the pair's tiles from `skip` on
+        cur.all = seq_tiles<KT>(cur.q, a.window);
+        cur.first = cur.all.x + skip;
+        cur.end = static_cast<int>(min(static_cast<int64_t>(cur.all.y), cur.first + cur.left));
     };
-    auto next_pair = [&](Cursor& c) {  // false: the piece is done
-        c.left -= c.end - c.first;
-        if (c.left <= 0) return false;
-        if (++c.hk == a.c.kv_heads) {
-            c.hk = 0;
+    auto next_pair = [&]() {  // false: the piece is done
+        cur.left -= cur.end - cur.first;
+        if (cur.left <= 0) return false;
+        if (++cur.hk == a.c.kv_heads) {
+            cur.hk = 0;
             do {
-                c.q = load_seq(a.c, ++c.s);
-            } while (c.q.n == 0 || c.q.n > 16 * MT / group);
+                cur.q = load_seq(a.c, ++cur.s);
+            } while (cur.q.n == 0 || cur.q.n > fit);
         }
-        enter(c, 0);
+        enter(0);
         return true;
     };
+    cur.s = static_cast<int>(s_at[0]);
     cur.q = load_seq(a.c, cur.s);
     cur.left = stop - begin;
     {
-        const int2 t = seq_tiles(cur.q, a.window);
+        const int64_t in_seq = begin - s_at[1];
+        const int2 t = seq_tiles<KT>(cur.q, a.window);
         cur.hk = static_cast<int>(in_seq / (t.y - t.x));
-        enter(cur, static_cast<int>(in_seq - static_cast<int64_t>(cur.hk) * (t.y - t.x)));
+        enter(static_cast<int>(in_seq - static_cast<int64_t>(cur.hk) * (t.y - t.x)));
     }
 
-    // ---- the warp's ring: tiles are issued STAGES - 1 ahead, one group each
-    Cursor ahead = cur;
-    bool more = true;
-    uint8_t* ring = sm + warp * (C::STAGES * C::STAGE);
-    const uint32_t ring_u = smem_u32(ring);
-    int page = -1;  // of the tile's first (even lanes) or second (odd lanes) eight keys
-    auto look = [&]() {  // the next tile with work, and its page
-        while (more && ahead.t >= ahead.end) more = next_pair(ahead);
-        if (!more) return;
-        const int col = (ahead.t * KT + (lane & 1) * 8) >> a.c.page_log2;
-        page = col < a.c.n_cols ? __ldg(a.c.table + ahead.s * a.c.table_stride + col) : -1;
-    };
-    auto issue = [&](int stage) {
-        if (more) {
-            const uint32_t dst = ring_u + stage * C::STAGE;
-            constexpr int CH = C::ROWB / 16;  // 16-byte pieces of a key
-            const int c = lane % CH;
-            const int64_t kh = ahead.hk * a.c.k_head + c * 8, vh = ahead.hk * a.c.v_head + c * 8;
-#pragma unroll
-            for (int i = 0; i < KT * CH / 32; i++) {
-                const int r = lane / CH + i * (32 / CH);
-                const int j = ahead.t * KT + r;
-                const int pg = __shfl_sync(0xffffffffu, page, r >> 3);
-                const bool ok = static_cast<unsigned>(pg) < static_cast<unsigned>(a.c.n_pages);
-                if (!ok && j < ahead.q.len) record_error(err, DEVERR_BAD_PAGE);
-                const bool in = ok && j < ahead.q.len && c * 8 < a.c.dim;
-                const int slot = j & (a.c.page - 1);
-                const T* k = static_cast<const T*>(a.c.k) + (in ? pg * a.c.k_page + slot * a.c.k_tok + kh : 0);
-                const T* v = static_cast<const T*>(a.c.v) + (in ? pg * a.c.v_page + slot * a.c.v_tok + vh : 0);
-                const uint32_t o = dst + r * C::ROWB + ((c ^ (r & 7)) << 4);
-                cp16(o, k, in);
-                cp16(o + KT * C::ROWB, v, in);
+    if (warp >= NW) {
+        // ------------------------------------------------ producers: keys, values
+        // lane i looks up the page of the i-th load of a window of 32 loads
+        const bool is_v = warp > NW;
+        const CUtensorMap* map = is_v ? &tmV : &tmK;
+        const uint32_t base = smem_u32(sm) + (is_v ? C::HALVES * C::HALF : 0);
+        const int per_tile = KT / plan.box, loads_h = C::HALVES / plan.box_halves;
+        int n = 0, stage = 0, phase = 1;  // tiles issued; the ring's place and the empty barriers' parity
+        bool ok = true;
+        do {
+            const int loads = (cur.end - cur.first) * per_tile;
+            for (int l0 = 0; ok && l0 < loads; l0 += 32) {
+                const int j = cur.first * KT + (l0 + lane) * plan.box;
+                int page = -1;
+                if (l0 + lane < loads && j < cur.q.len) {
+                    const int col = j >> a.c.page_log2;
+                    if (col < a.c.n_cols) page = __ldg(a.c.table + cur.s * a.c.table_stride + col);
+                    // (a page past the cache's end is outside the tensor map: zeros)
+                    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.n_pages)) {
+                        record_error(err, DEVERR_BAD_PAGE);
+                        page = -1;
+                    }
+                }
+                const int here = min(32, loads - l0);
+                for (int i = 0; i < here; i += per_tile) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(empty + stage, phase, err, DEVERR_PATTN_EMPTY));
+                    if (!ok) break;
+                    uint64_t* bar = full + stage;
+                    if (lane == 0) mbar_arrive_expect_tx(bar, C::STAGE / 2);
+                    for (int b = 0; b < per_tile; b++) {
+                        const int pg = __shfl_sync(0xffffffffu, page, i + b);
+                        const int slot = (cur.first * KT + (l0 + i + b) * plan.box) & (a.c.page - 1);
+                        if (lane == 0) {
+                            const uint32_t dst = base + stage * C::STAGE + b * plan.box * 128;
+                            for (int h = 0; h < loads_h; h++)
+                                tma_load_5d(map, bar, dst + h * C::HALF, plan.by_value ? h * 64 : 0, slot,
+                                            plan.by_value ? 0 : h, cur.hk, pg);
+                        }
+                    }
+                    n++;
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
             }
-            ahead.t += NW;
-        }
-        cp_commit();
-        look();
-    };
-    look();
-#pragma unroll
-    for (int i = 0; i < C::STAGES - 1; i++) issue(i);
-    int stage = 0, fill = C::STAGES - 1;
+        } while (ok && next_pair());
+        // every load lands before the CTA may end
+        if (lane == 0)
+            for (int i = max(0, n - C::STAGES); i < n; i++)
+                mbar_wait(full + i % C::STAGES, (i / C::STAGES) & 1, nullptr, DEVERR_PATTN_DRAIN);
+        return;
+    }
 
+    // ---------------------------------------------------- consumers
     const float scale2 = a.scale * 1.4426950408889634f;
     const int g = lane >> 2, quad = lane & 3;
-    int parity = 0;
-    for (bool go = true; go; go = next_pair(cur), parity ^= C::MLB - 1) {
+    int parity = 0, n0 = 0;  // n0: the pair's first tile in the order of the ring
+    int turn = warp, stage = warp % C::STAGES, phase = 0;  // this warp's next tile there
+    bool ok = true;
+    for (bool go = true; go; n0 += cur.end - cur.first, go = next_pair(), parity ^= 1) {
         // ---- the pair's rows as A fragments
         const int rows = cur.q.n * group;
-        uint32_t qf[MT][DP / 16][4];
-        int pos[MT][2];  // of this thread's two rows in each block of 16 (below 0: sees nothing)
+        uint32_t qf[DP / 16][4];
+        int pos[2];  // of this thread's two rows (below 0: sees nothing)
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int hf = 0; hf < 2; hf++) {
+            const int r = g + hf * 8;
+            const int i = r / group, gi = r - i * group;
+            const bool in = r < rows;
+            pos[hf] = in ? cur.q.len - cur.q.n + i : -1;
+            const T* q = static_cast<const T*>(a.q) + (in ? (cur.q.row0 + i) * a.q_tok + (cur.hk * group + gi) * a.q_head : 0);
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                const int r = mt * 16 + g + hf * 8;
-                const int i = r / group, gi = r - i * group;
-                const bool in = r < rows;
-                pos[mt][hf] = in ? cur.q.len - cur.q.n + i : -1;
-                const T* q = static_cast<const T*>(a.q) + (in ? (cur.q.row0 + i) * a.q_tok + (cur.hk * group + gi) * a.q_head : 0);
+            for (int kk = 0; kk < DP / 16; kk++)
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; kk++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int d = kk * 16 + e * 8 + quad * 2;
-                        qf[mt][kk][e * 2 + hf] = in && d < a.c.dim ? __ldg(reinterpret_cast<const uint32_t*>(q + d)) : 0u;
-                    }
-            }
-        float m[MT][2], l[MT][2], o[MT][DP / 8][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < DP / 8; n++) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.0f;
+                for (int e = 0; e < 2; e++) {
+                    const int d = kk * 16 + e * 8 + quad * 2;
+                    qf[kk][e * 2 + hf] = in && d < a.c.dim ? __ldg(reinterpret_cast<const uint32_t*>(q + d)) : 0u;
+                }
         }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[DP / 8][4];
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
-        for (; cur.t < cur.end; cur.t += NW) {
-            cp_wait<C::STAGES - 2>();
-            __syncwarp();  // the tile is there for every lane, and every lane is done with the one before
-            issue(fill);
-            const uint32_t ks = ring_u + stage * C::STAGE, vs = ks + KT * C::ROWB;
-            float sc[MT][2][4];
+        for (const int n1 = n0 + cur.end - cur.first; turn < n1; turn += NW) {
+            const int t = cur.first + turn - n0;
+            if (ok) ok = mbar_wait(full + stage, phase, err, DEVERR_PATTN_FULL);
+            const uint32_t ks = smem_u32(sm) + stage * C::STAGE, vs = ks + C::HALVES * C::HALF;
+            if ((t + 1) * KT > cur.q.len) {
+                // the values behind the sequence's end may be anything, and 0 x NaN is NaN: zeros
+                const int from = max(0, cur.q.len - t * KT);
+                for (int i = from * 8 + lane; i < KT * 8; i += 32)
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+                    for (int h = 0; h < C::HALVES; h++)
+                        *reinterpret_cast<uint4*>(sm + stage * C::STAGE + (C::HALVES + h) * C::HALF + i * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            float sc[KT / 8][4];
 #pragma unroll
-                for (int n = 0; n < 2; n++) sc[mt][n][0] = sc[mt][n][1] = sc[mt][n][2] = sc[mt][n][3] = 0.0f;
+            for (int n = 0; n < KT / 8; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
             {
                 const int r = ((lane >> 4) << 3) + (lane & 7), cc = (lane >> 3) & 1;
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; kk++) {
-                    uint32_t b[4];
-                    ldsm4(ks + r * C::ROWB + (((kk * 2 + cc) ^ (r & 7)) << 4), b);
+                    const uint32_t half = ks + (kk / 4) * C::HALF;
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        mma16816<T>(sc[mt][0], qf[mt][kk], b[0], b[1]);
-                        mma16816<T>(sc[mt][1], qf[mt][kk], b[2], b[3]);
+                    for (int n = 0; n < KT / 16; n++) {
+                        uint32_t b[4];
+                        ldsm4(half + (n * 16 + r) * 128 + ((((kk & 3) * 2 + cc) ^ (r & 7)) << 4), b);
+                        mma16816<T>(sc[2 * n], qf[kk], b[0], b[1]);
+                        mma16816<T>(sc[2 * n + 1], qf[kk], b[2], b[3]);
                     }
                 }
             }
-            uint32_t pf[MT][4];
-            const int j0 = cur.t * KT + quad * 2;
+            uint32_t pf[KT / 16][4];
+            const int j0 = t * KT + quad * 2;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int hf = 0; hf < 2; hf++) {
+                const int hi = pos[hf], lo = a.window > 0 ? hi - a.window : -1;  // keys in (lo, hi]
+                float x[KT / 4], top = -INFINITY;
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    const int hi = pos[mt][hf], lo = a.window > 0 ? hi - a.window : -1;  // keys in (lo, hi]
-                    float x[4], top = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int j = j0 + (e >> 1) * 8 + (e & 1);
-                        const float y = sc[mt][e >> 1][hf * 2 + (e & 1)] * scale2;
-                        x[e] = j <= hi && j > lo ? y : -INFINITY;
-                        top = fmaxf(top, x[e]);
-                    }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float m2 = fmaxf(m[mt][hf], top);
-                    const float base = m2 == -INFINITY ? 0.0f : m2;
-                    const float f = ex2(m[mt][hf] - base);
-                    m[mt][hf] = m2;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[e] = ex2(x[e] - base);
-                        sum += x[e];
-                    }
-                    l[mt][hf] = l[mt][hf] * f + sum;
-                    // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
-                    // rounding of the result; l sums them unrounded
-                    pf[mt][hf] = pack2<T>(x[0], x[1]);
-                    pf[mt][2 + hf] = pack2<T>(x[2], x[3]);
-#pragma unroll
-                    for (int n = 0; n < DP / 8; n++) {
-                        o[mt][n][hf * 2] *= f;
-                        o[mt][n][hf * 2 + 1] *= f;
-                    }
+                for (int e = 0; e < KT / 4; e++) {
+                    const int j = j0 + (e >> 1) * 8 + (e & 1);
+                    const float y = sc[e >> 1][hf * 2 + (e & 1)] * scale2;
+                    x[e] = j <= hi && j > lo ? y : -INFINITY;
+                    top = fmaxf(top, x[e]);
                 }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float m2 = fmaxf(m[hf], top);
+                const float base = m2 == -INFINITY ? 0.0f : m2;
+                const float f = ex2(m[hf] - base);
+                m[hf] = m2;
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < KT / 4; e++) {
+                    x[e] = ex2(x[e] - base);
+                    sum += x[e];
+                }
+                l[hf] = l[hf] * f + sum;
+                // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
+                // rounding of the result; l sums them unrounded
+#pragma unroll
+                for (int n = 0; n < KT / 16; n++) {
+                    pf[n][hf] = pack2<T>(x[4 * n], x[4 * n + 1]);
+                    pf[n][2 + hf] = pack2<T>(x[4 * n + 2], x[4 * n + 3]);
+                }
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++) {
+                    o[n][hf * 2] *= f;
+                    o[n][hf * 2 + 1] *= f;
+                }
+            }
             {
                 const int r = (((lane >> 3) & 1) << 3) + (lane & 7), cc = lane >> 4;
 #pragma unroll
                 for (int n = 0; n < DP / 16; n++) {
-                    uint32_t b[4];
-                    ldsm4_t(vs + r * C::ROWB + (((n * 2 + cc) ^ (r & 7)) << 4), b);
+                    const uint32_t half = vs + (n / 4) * C::HALF;
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        mma16816<T>(o[mt][2 * n], pf[mt], b[0], b[1]);
-                        mma16816<T>(o[mt][2 * n + 1], pf[mt], b[2], b[3]);
+                    for (int k = 0; k < KT / 16; k++) {
+                        uint32_t b[4];
+                        ldsm4_t(half + (k * 16 + r) * 128 + ((((n & 3) * 2 + cc) ^ (r & 7)) << 4), b);
+                        mma16816<T>(o[2 * n], pf[k], b[0], b[1]);
+                        mma16816<T>(o[2 * n + 1], pf[k], b[2], b[3]);
                     }
                 }
             }
-            if (++stage == C::STAGES) stage = 0;
-            if (++fill == C::STAGES) fill = 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + stage);
+            stage += NW;
+            if (stage >= C::STAGES) {
+                stage -= C::STAGES;
+                phase ^= 1;
+            }
         }
 
-        // ---- join the eight warps' parts
-        if constexpr (C::MLB == 1) __syncthreads();
-        float2* ml = reinterpret_cast<float2*>(sm + C::OFF_ML) + parity * NW * 16 * MT;
+        // ---- join the warps' parts
+        float2* ml = reinterpret_cast<float2*>(sm + C::OFF_ML) + parity * NW * 16;
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                float x = l[mt][hf];
-                x += __shfl_xor_sync(0xffffffffu, x, 1);
-                x += __shfl_xor_sync(0xffffffffu, x, 2);
-                if (quad == 0) ml[warp * 16 * MT + mt * 16 + g + hf * 8] = make_float2(m[mt][hf], x);
-            }
-        __syncthreads();
+        for (int hf = 0; hf < 2; hf++) {
+            float x = l[hf];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            if (quad == 0) ml[warp * 16 + g + hf * 8] = make_float2(m[hf], x);
+        }
+        named_bar_sync(1, NC);
         const bool whole = cur.first == cur.all.x && cur.end == cur.all.y;
         const int slot = cur.first == cur.all.x ? 1 : 0;  // a pair that goes on after this piece, or came into it
         uint8_t* part = plan.parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * C::SLOT;
@@ -427,102 +475,100 @@ __global__ void __launch_bounds__(NTHR, 1) attn_rows_kernel(const PagedAttnArgs 
         auto top_of = [&](int r) {
             float t = ml[r].x;
 #pragma unroll
-            for (int w = 1; w < NW; w++) t = fmaxf(t, ml[w * 16 * MT + r].x);
+            for (int w = 1; w < NW; w++) t = fmaxf(t, ml[w * 16 + r].x);
             return t;
         };
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
+        {
             float f[2];
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
-                const float t = top_of(mt * 16 + g + hf * 8);
-                f[hf] = t == -INFINITY ? 0.0f : ex2(m[mt][hf] - t);
+                const float t = top_of(g + hf * 8);
+                f[hf] = t == -INFINITY ? 0.0f : ex2(m[hf] - t);
             }
-            float* mine = buf + (warp & 3) * (16 * DP);
-            if (mt > 0) __syncthreads();  // the block before is read
-            if (warp >= 4) {
+            float* mine = buf + warp % (NW / 2) * (16 * DP);
+            if (warp >= NW / 2) {
 #pragma unroll
                 for (int n = 0; n < DP / 8; n++)
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++)
                         *reinterpret_cast<float2*>(mine + (g + hf * 8) * DP + n * 8 + quad * 2) =
-                            make_float2(o[mt][n][hf * 2] * f[hf], o[mt][n][hf * 2 + 1] * f[hf]);
+                            make_float2(o[n][hf * 2] * f[hf], o[n][hf * 2 + 1] * f[hf]);
             }
-            __syncthreads();
-            if (warp < 4) {
+            named_bar_sync(1, NC);
+            if (warp < NW / 2) {
 #pragma unroll
                 for (int n = 0; n < DP / 8; n++)
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++) {
                         float2* w = reinterpret_cast<float2*>(mine + (g + hf * 8) * DP + n * 8 + quad * 2);
                         const float2 y = *w;
-                        *w = make_float2(fmaf(o[mt][n][hf * 2], f[hf], y.x), fmaf(o[mt][n][hf * 2 + 1], f[hf], y.y));
+                        *w = make_float2(fmaf(o[n][hf * 2], f[hf], y.x), fmaf(o[n][hf * 2 + 1], f[hf], y.y));
                     }
             }
-            __syncthreads();
-            for (int e = tid; e < 16 * (DP / 4); e += NTHR) {
-                const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4, row = mt * 16 + r;
-                if (row >= rows || d >= a.c.dim) continue;
-                float4 y = *reinterpret_cast<const float4*>(buf + r * DP + d);
+            named_bar_sync(1, NC);
+        }
+        for (int e = tid; e < rows * (DP / 4); e += NC) {
+            const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4;
+            if (d >= a.c.dim) continue;
+            float4 y = *reinterpret_cast<const float4*>(buf + r * DP + d);
 #pragma unroll
-                for (int w = 1; w < 4; w++) {
-                    const float4 z = *reinterpret_cast<const float4*>(buf + w * 16 * DP + r * DP + d);
-                    y.x += z.x;
-                    y.y += z.y;
-                    y.z += z.z;
-                    y.w += z.w;
-                }
-                const float t = top_of(row);
-                float sum = 0.0f;
+            for (int w = 1; w < NW / 2; w++) {
+                const float4 z = *reinterpret_cast<const float4*>(buf + w * 16 * DP + r * DP + d);
+                y.x += z.x;
+                y.y += z.y;
+                y.z += z.z;
+                y.w += z.w;
+            }
+            const float t = top_of(r);
+            float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < NW; w++) {
-                    const float2 z = ml[w * 16 * MT + row];
-                    sum += t == -INFINITY ? 0.0f : z.y * ex2(z.x - t);
-                }
-                if (whole) {
-                    const int i = row / group, gi = row - i * group;
-                    const int64_t at = static_cast<int64_t>(cur.q.row0 + i) * a.q_heads + cur.hk * group + gi;
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.c.dim + d) =
-                        make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
-                    if (d == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (t + log2f(sum)) * 0.6931471805599453f;
-                } else {
-                    *reinterpret_cast<float4*>(part + (static_cast<int64_t>(row) * DP + d) * 4) = y;
-                    if (d == 0) *reinterpret_cast<float2*>(part + 16 * MT * DP * 4 + row * 8) = make_float2(t, sum);
-                }
+            for (int w = 0; w < NW; w++) {
+                const float2 z = ml[w * 16 + r];
+                sum += t == -INFINITY ? 0.0f : z.y * ex2(z.x - t);
+            }
+            if (whole) {
+                const int i = r / group, gi = r - i * group;
+                const int64_t at = static_cast<int64_t>(cur.q.row0 + i) * a.q_heads + cur.hk * group + gi;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.c.dim + d) =
+                    make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
+                if (d == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (t + log2f(sum)) * 0.6931471805599453f;
+            } else {
+                *reinterpret_cast<float4*>(part + (r * DP + d) * 4) = y;
+                if (d == 0) *reinterpret_cast<float2*>(part + 16 * DP * 4 + r * 8) = make_float2(t, sum);
             }
         }
         if (whole) continue;
 
         // ---- join the CTAs' parts: CTA c0 began the pair, c1 ends it
-        const int64_t at0 = begin + (stop - begin - cur.left) - (cur.first - cur.all.x);  // of the pair's first tile
+        const int64_t at0 = stop - cur.left - (cur.first - cur.all.x);  // the pair's first tile in the line
         const int c0 = static_cast<int>(at0 / per), c1 = static_cast<int>((at0 + cur.all.y - cur.all.x - 1) / per);
         __threadfence();
-        __syncthreads();
-        if (tid == 0) s_last = atomicAdd(plan.counters + c0, 1) == c1 - c0;
-        __syncthreads();
-        if (!s_last) continue;
+        named_bar_sync(1, NC);
+        if (tid == 0) *s_last = atomicAdd(plan.counters + c0, 1) == c1 - c0;
+        named_bar_sync(1, NC);
+        if (!*s_last) continue;
         __threadfence();
-        for (int e = tid; e < rows * (DP / 4); e += NTHR) {
-            const int row = e / (DP / 4), d = (e - row * (DP / 4)) * 4;
+        for (int e = tid; e < rows * (DP / 4); e += NC) {
+            const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4;
             if (d >= a.c.dim) continue;
             auto slot_of = [&](int c) { return plan.parts + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * C::SLOT; };
             float t = -INFINITY;
             for (int c = c0; c <= c1; c++)
-                t = fmaxf(t, __ldcg(reinterpret_cast<const float2*>(slot_of(c) + 16 * MT * DP * 4 + row * 8)).x);
+                t = fmaxf(t, __ldcg(reinterpret_cast<const float2*>(slot_of(c) + 16 * DP * 4 + r * 8)).x);
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float sum = 0.0f;
             for (int c = c0; c <= c1; c++) {
-                const float2 z = __ldcg(reinterpret_cast<const float2*>(slot_of(c) + 16 * MT * DP * 4 + row * 8));
+                const float2 z = __ldcg(reinterpret_cast<const float2*>(slot_of(c) + 16 * DP * 4 + r * 8));
                 const float f = t == -INFINITY ? 0.0f : ex2(z.x - t);
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(slot_of(c) + (static_cast<int64_t>(row) * DP + d) * 4));
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(slot_of(c) + (r * DP + d) * 4));
                 sum = fmaf(z.y, f, sum);
                 y.x = fmaf(x.x, f, y.x);
                 y.y = fmaf(x.y, f, y.y);
                 y.z = fmaf(x.z, f, y.z);
                 y.w = fmaf(x.w, f, y.w);
             }
-            const int i = row / group, gi = row - i * group;
+            const int i = r / group, gi = r - i * group;
             const int64_t at = static_cast<int64_t>(cur.q.row0 + i) * a.q_heads + cur.hk * group + gi;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.c.dim + d) =
@@ -531,7 +577,6 @@ __global__ void __launch_bounds__(NTHR, 1) attn_rows_kernel(const PagedAttnArgs 
         }
         if (tid == 0) plan.counters[c0] = 0;
     }
-    cp_wait<0>();
 }
 
 // ---------------------------------------------------------------- many rows
@@ -614,39 +659,58 @@ int paged_attention_workspace(const PagedAttnArgs& a, int64_t* bytes) {
     int rc = 0;
     DeviceState* ds = device_state(&rc);
     if (!ds) return rc;
-    const bool two = static_cast<int64_t>(a.max_q) * (a.q_heads / a.c.kv_heads) > 16;
-    const int64_t slot = a.c.dim > 64 ? (two ? RowsCfg<128, 2>::SLOT : RowsCfg<128, 1>::SLOT)
-                                      : (two ? RowsCfg<64, 2>::SLOT : RowsCfg<64, 1>::SLOT);
-    *bytes = kCounterBytes + 2ll * ds->sm_count * slot;
+    *bytes = kCounterBytes + 2ll * ds->sm_count * (a.c.dim > 64 ? RowsCfg<128>::SLOT : RowsCfg<64>::SLOT);
     return TVQ_OK;
 }
 
 namespace {
 
-template <typename T, int DP, int MT>
+// The cache as a {value, token, half, head, page} tensor map, boxes of 64
+// values x `box` tokens x `halves` (128-byte swizzle).  A head dim that is no
+// multiple of 64 stays one dimension, so that nothing behind it is read.
+int cache_map(CUtensorMap* map, const PagedView& c, const void* ptr, int64_t tok, int64_t head, int64_t page, int box,
+              int halves) {
+    const bool whole = c.dim % 64 == 0;
+    const uint64_t dims[5] = {static_cast<uint64_t>(whole ? 64 : c.dim), static_cast<uint64_t>(c.page),
+                              static_cast<uint64_t>(whole ? c.dim / 64 : 1), static_cast<uint64_t>(c.kv_heads),
+                              static_cast<uint64_t>(c.n_pages)};
+    const uint64_t strides[4] = {static_cast<uint64_t>(tok) * 2, 128, static_cast<uint64_t>(head) * 2,
+                                 static_cast<uint64_t>(page) * 2};
+    const uint32_t boxes[5] = {64, static_cast<uint32_t>(box), static_cast<uint32_t>(halves), 1, 1};
+    return make_tma_16bit(map, ptr, 5, dims, strides, boxes);
+}
+
+template <typename T, int DP>
 int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
-    using C = RowsCfg<DP, MT>;
-    static const cudaError_t attr = cudaFuncSetAttribute(attn_rows_kernel<T, DP, MT>,
-                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    using C = RowsCfg<DP>;
+    static const cudaError_t attr =
+        cudaFuncSetAttribute(attn_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     TVQ_CUDA(attr);
     RowsPlan plan;
     plan.counters = static_cast<int*>(a.ws);
     plan.parts = static_cast<uint8_t*>(a.ws) + kCounterBytes;
-    plan.min_tiles = NW;
-    return launch_pdl(attn_rows_kernel<T, DP, MT>, dim3(ds->sm_count), dim3(NTHR), C::SMEM, st, a, plan, ds->d_error);
+    plan.min_tiles = 4;
+    plan.box = std::min(a.c.page, C::KT);
+    plan.by_value = a.c.dim % 64 != 0;
+    plan.box_halves = a.c.dim == 128 && plan.box == C::KT ? 2 : 1;
+    CUtensorMap tmK, tmV;
+    int rc = cache_map(&tmK, a.c, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
+    if (rc) return rc;
+    rc = cache_map(&tmV, a.c, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
+    if (rc) return rc;
+    return launch_pdl(attn_rows_kernel<T, DP>, dim3(ds->sm_count), dim3(NTHR), C::SMEM, st, tmK, tmV, a, plan,
+                      ds->d_error);
 }
 
 template <typename T>
 int launch_attention(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     const int group = a.q_heads / a.c.kv_heads;
-    const bool two = static_cast<int64_t>(a.max_q) * group > 16;
-    int rc;
-    if (a.c.dim > 64) rc = two ? launch_rows<T, 128, 2>(a, ds, st) : launch_rows<T, 128, 1>(a, ds, st);
-    else rc = two ? launch_rows<T, 64, 2>(a, ds, st) : launch_rows<T, 64, 1>(a, ds, st);
-    if (rc || static_cast<int64_t>(a.max_q) * group <= 32) return rc;
+    int rc = TVQ_OK;
+    if (group <= MAX_ROWS) rc = a.c.dim > 64 ? launch_rows<T, 128>(a, ds, st) : launch_rows<T, 64>(a, ds, st);
+    if (rc || static_cast<int64_t>(a.max_q) * group <= MAX_ROWS) return rc;
     const int64_t units = static_cast<int64_t>(a.c.n_rows) * a.q_heads;
     return launch_pdl(paged_attention_row_kernel<T>, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(128), 0, st, a,
-                      32 / group, ds->d_error);
+                      MAX_ROWS / group, ds->d_error);
 }
 
 }  // namespace
@@ -655,6 +719,8 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     int rc = 0;
     DeviceState* ds = device_state(&rc);
     if (!ds) return rc;
+    TVQ_CHECK(ds->cc_major == 10, TVQ_ERR_UNSUPPORTED, "the paged attention needs an sm_100 device");
+    TVQ_CHECK(ds->sm_count * 4 <= kCounterBytes, TVQ_ERR_UNSUPPORTED, "more SMs than counters");
     if (a.c.n_rows == 0 || a.max_q == 0) return TVQ_OK;
     return a.c.type == TVQ_TYPE_F16 ? launch_attention<__half>(a, ds, st) : launch_attention<__nv_bfloat16>(a, ds, st);
 }
