@@ -447,7 +447,7 @@ TVQ_API int tvq_dev_paged_append(int type, int src_type, const void* k, const vo
  * are formed in f32; the softmax's weights are rounded to `type` before
  * they meet V (relative 2^-11 / 2^-8 each), its statistics stay f32.
  * ws: at least tvq_paged_attention_workspace bytes, 256-byte aligned, used by
- * one call at a time, zero before its first use (a call leaves it so). */
+ * one call at a time; nothing in it has to last from call to call. */
 TVQ_API int tvq_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t n_seq,
                                           int64_t n_rows, int64_t max_q, int64_t* bytes);
 TVQ_API int tvq_dev_paged_attention(int type, const void* q, const int64_t* q_strides, int64_t q_heads,

@@ -13,20 +13,22 @@
 // drafted ones).  Every key and value is used for at most 16 rows, so the
 // bytes of the cache bound it, and what counts is that enough of them are in
 // flight and that every SM has the same share:
-//  - one CTA per SM; all 32-key tiles of all (sequence, kv head) pairs stand
-//    in one line, and CTA c takes the c-th equal piece of it, whatever the
-//    lengths.  Every CTA finds its piece from the lengths on the device.
-//  - two producer warps (keys, values) bring the piece's tiles through a 192 KB
-//    ring by TMA (a tile's pages are boxes of a {value, token, half, head,
-//    page} tensor map, so any strides will do), across the ends of pairs; six
-//    consumer warps take the tiles in turn, each with its own m, l, o, and join them at the end
-//    of a pair, while the next pair's tiles are on their way.
-//  - mma.sync m16n8k16 with the rows padded to 16: at D = 128 the products
-//    of a 16 KB tile take 128 of the ~650 cycles that its bytes take, so the
-//    wider tcgen05 tile (128 rows) would buy nothing here.
-//  - a pair that several CTAs share is joined by the one that finishes last
-//    (a counter per CTA in the workspace, zero between calls), in the order
-//    of the parts, so results do not depend on who that is.
+//  - all tiles (8 KB of keys and values) of all (sequence, kv head) pairs
+//    stand in one line, which is cut into equal pieces, one for each of the
+//    eight warps of each SM, whatever the lengths.  Every CTA finds its pieces
+//    from the lengths on the device; neighbouring pieces go to different SMs.
+//  - a warp is a pipeline of its own: its tiles come through its own ring of
+//    three stages by TMA (a tile's pages are boxes of a {value, token, half,
+//    head, page} tensor map, so any strides will do), across the ends of
+//    pairs, and it keeps its own m, l, o.  192 KB are in flight on each SM,
+//    and nothing in the CTA waits for another warp.  (Eight warps that share
+//    each pair and join it in shared memory took ~4000 cycles a pair more,
+//    which doubled the time of many short sequences.)
+//  - mma.sync m16n8k16 with the rows padded to 16: a warp's tile takes ~1000
+//    cycles from ring to ring, and the eight together 125 a tile where its
+//    bytes take ~330, so the wider tcgen05 tile (128 rows) would buy nothing.
+//  - a pair that lies in one piece is written at once; the parts of the others
+//    go to the workspace in f32, and attn_join_kernel joins them in order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -40,19 +42,27 @@ namespace tvq {
 
 namespace {
 
-constexpr int NW = 6;              // consumer warps of the rows kernel
-constexpr int NC = NW * 32;        // consumer threads
-constexpr int NTHR = NC + 64;      // and two producer warps
+constexpr int NW = 8;              // warps of the rows kernel's CTA
+constexpr int NTHR = NW * 32;
 constexpr int MAX_ROWS = 16;       // rows of a pair (new tokens x heads of the group)
 
 // device error codes: the wait that gave up first
-enum : int { DEVERR_PATTN_EMPTY = 71, DEVERR_PATTN_FULL = 72, DEVERR_PATTN_DRAIN = 73 };
+enum : int { DEVERR_PATTN_FULL = 72 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error ~2^-22, 2^-inf = 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -136,27 +146,21 @@ __device__ __forceinline__ int2 seq_tiles(const Seq& q, int window) {
 // ---------------------------------------------------------------- few rows
 template <int DP>
 struct RowsCfg {
-    static constexpr int KT = 32;                        // keys per tile
+    static constexpr int KT = DP == 128 ? 16 : 32;       // keys per tile
     static constexpr int HALF = KT * 128;                // 64 values of a tile's keys, 128-byte swizzle
     static constexpr int HALVES = DP / 64;
-    static constexpr int STAGE = 2 * HALVES * HALF;      // one tile: keys, then values
-    static constexpr int STAGES = 196608 / STAGE;        // 24 or 12
-    // A stage is always the same warp's, which waits for its phases one after
-    // another.  Were it to pass from warp to warp, one that is ahead could take
-    // the parity of the phase before last for that of the one it waits for.
-    static_assert(STAGES % NW == 0);
-    static constexpr int OFF_PART = STAGES * STAGE;      // [NW / 2][16][DP] f32
-    static constexpr int OFF_ML = OFF_PART + NW / 2 * 16 * DP * 4;     // float2 [2][NW][16]
-    static constexpr int OFF_BAR = OFF_ML + 2 * NW * 16 * 8;      // full[STAGES], empty[STAGES]
-    static constexpr int OFF_MISC = OFF_BAR + 2 * STAGES * 8;     // scan[NW + 2], last, at[2]
-    static constexpr int SMEM = OFF_MISC + 64;
-    static constexpr int64_t SLOT = 16 * (DP * 4 + 8);   // workspace bytes of one partial
+    static constexpr int STAGE = 2 * HALVES * HALF;      // one tile, 8 KB: keys, then values
+    static constexpr int STAGES = 3;                     // of each warp
+    static constexpr int OFF_BAR = NW * STAGES * STAGE;  // full[NW][STAGES]
+    static constexpr int OFF_MISC = OFF_BAR + NW * STAGES * 8;  // int64 at[NW], int seq[NW], int scan[NW]
+    static constexpr int SMEM = OFF_MISC + NW * 16;
 };
 
 struct RowsPlan {
-    int* counters;   // [grid]
-    uint8_t* parts;  // [grid][2] slots
-    int min_tiles;   // no CTA gets a smaller piece
+    uint8_t* parts;  // [pieces][2]: f32 [rows_cap][DP], then float2 (m, l) [rows_cap]
+    int2* spans;     // [n_seq * kv_heads]: a pair's first and last piece
+    int rows_cap;    // no pair has more rows
+    int64_t slot;    // bytes of one part
     // One TMA load: `box` tokens (a power of two: a page, or a tile of a larger
     // one) of 64 values, or of both halves (box_halves 2: 128 values and box =
     // KT).  by_value: the head dim is no multiple of 64, the halves start at
@@ -164,7 +168,7 @@ struct RowsPlan {
     int box, box_halves, by_value;
 };
 
-// Where a walk over a CTA's piece stands: a pair and its tiles in the piece.
+// Where a walk over a piece stands: a pair and its tiles in the piece.
 struct Cursor {
     int s, hk;
     int64_t left;    // tiles of the piece from this pair's first one on
@@ -180,26 +184,24 @@ __global__ void __launch_bounds__(NTHR, 1)
     using C = RowsCfg<DP>;
     constexpr int KT = C::KT;
     extern __shared__ __align__(1024) uint8_t sm[];
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
-    uint64_t* empty = full + C::STAGES;
-    int* s_scan = reinterpret_cast<int*>(sm + C::OFF_MISC);
-    int* s_last = s_scan + NW + 2;
-    int64_t* s_at = reinterpret_cast<int64_t*>(s_scan + NW + 4);
+    int64_t* s_at = reinterpret_cast<int64_t*>(sm + C::OFF_MISC);
+    int* s_seq = reinterpret_cast<int*>(s_at + NW);
+    int* s_scan = s_seq + NW;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + warp * C::STAGES;
     const int group = a.q_heads / a.c.kv_heads;
     const int fit = MAX_ROWS / group;  // new rows of a sequence that this kernel takes
-    if (tid == 0) {
-        for (int i = 0; i < C::STAGES; i++) {
-            mbar_init(full + i, 2);
-            mbar_init(empty + i, 1);
-        }
+    if (lane == 0) {
+        for (int i = 0; i < C::STAGES; i++) mbar_init(full + i, 1);
         fence_barrier_init();
+    }
+    if (tid == 0) {
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
     griddep_wait();
 
-    // ---- this CTA's piece of the line of tiles
+    // ---- the pieces of the line of tiles
     auto weight = [&](int s) -> int {
         if (s >= a.c.n_seq) return 0;
         const Seq q = load_seq(a.c, s);
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (lane == 31) s_scan[warp] = x;
         __syncthreads();
         int sum = 0;
-        for (int w = 0; w < NW + 2; w++) {
+        for (int w = 0; w < NW; w++) {
             if (w < warp) x += s_scan[w];
             sum += s_scan[w];
         }
@@ -232,9 +234,8 @@ __global__ void __launch_bounds__(NTHR, 1)
         total += all;
     }
     total *= a.c.kv_heads;
-    const int64_t per = max(static_cast<int64_t>(plan.min_tiles), (total + gridDim.x - 1) / gridDim.x);
-    const int64_t begin = per * blockIdx.x, stop = min(total, begin + per);
-    if (begin >= stop) return;
+    const int64_t pieces = static_cast<int64_t>(gridDim.x) * NW;
+    const int64_t per = max(static_cast<int64_t>(1), (total + pieces - 1) / pieces);
     int64_t before = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += NTHR) {
         int all = 0;
@@ -244,113 +245,133 @@ __global__ void __launch_bounds__(NTHR, 1)
             inc = scan(w, &all);
         }
         const int64_t hi = (before + inc) * a.c.kv_heads, lo = hi - static_cast<int64_t>(w) * a.c.kv_heads;
-        if (begin >= lo && begin < hi) {
-            s_at[0] = s0 + tid;
-            s_at[1] = lo;
-        }
+        if (w > 0)
+            for (int i = 0; i < NW; i++) {
+                const int64_t at = per * (static_cast<int64_t>(i) * gridDim.x + blockIdx.x);
+                if (at >= lo && at < hi) {
+                    s_seq[i] = s0 + tid;
+                    s_at[i] = lo;
+                }
+            }
         before += all;
     }
     __syncthreads();
+    const int piece = warp * gridDim.x + blockIdx.x;
+    const int64_t begin = per * piece, stop = min(total, begin + per);
+    if (begin >= stop) return;
 
     Cursor cur;
-    auto enter = [&](int skip) {  // cur.s, hk, left and q set: the pair's tiles from `skip` on
-        cur.all = seq_tiles<KT>(cur.q, a.window);
-        cur.first = cur.all.x + skip;
-        cur.end = static_cast<int>(min(static_cast<int64_t>(cur.all.y), cur.first + cur.left));
+    auto enter = [&](Cursor& c, int skip) {  // s, hk, left and q set: the pair's tiles from `skip` on
+        c.all = seq_tiles<KT>(c.q, a.window);
+        c.first = c.all.x + skip;
+        c.end = static_cast<int>(min(static_cast<int64_t>(c.all.y), c.first + c.left));
     };
-    auto next_pair = [&]() {  // false: the piece is done
-        cur.left -= cur.end - cur.first;
-        if (cur.left <= 0) return false;
-        if (++cur.hk == a.c.kv_heads) {
-            cur.hk = 0;
+    auto next_pair = [&](Cursor& c) {  // false: the piece is done
+        c.left -= c.end - c.first;
+        if (c.left <= 0) return false;
+        if (++c.hk == a.c.kv_heads) {
+            c.hk = 0;
             do {
-                cur.q = load_seq(a.c, ++cur.s);
-            } while (cur.q.n == 0 || cur.q.n > fit);
+                c.q = load_seq(a.c, ++c.s);
+            } while (c.q.n == 0 || c.q.n > fit);
         }
-        enter(0);
+        enter(c, 0);
         return true;
     };
-    cur.s = static_cast<int>(s_at[0]);
+    cur.s = s_seq[warp];
     cur.q = load_seq(a.c, cur.s);
     cur.left = stop - begin;
     {
-        const int64_t in_seq = begin - s_at[1];
+        const int64_t in_seq = begin - s_at[warp];
         const int2 t = seq_tiles<KT>(cur.q, a.window);
         cur.hk = static_cast<int>(in_seq / (t.y - t.x));
-        enter(static_cast<int>(in_seq - static_cast<int64_t>(cur.hk) * (t.y - t.x)));
+        enter(cur, static_cast<int>(in_seq - static_cast<int64_t>(cur.hk) * (t.y - t.x)));
     }
 
-    if (warp >= NW) {
-        // ------------------------------------------------ producers: keys, values
-        // lane i looks up the page of the i-th load of a window of 32 loads
-        const bool is_v = warp > NW;
-        const CUtensorMap* map = is_v ? &tmV : &tmK;
-        const uint32_t base = smem_u32(sm) + (is_v ? C::HALVES * C::HALF : 0);
-        const int per_tile = KT / plan.box, loads_h = C::HALVES / plan.box_halves;
-        int n = 0, stage = 0, phase = 1;  // tiles issued; the ring's place and the empty barriers' parity
-        bool ok = true;
-        do {
-            const int loads = (cur.end - cur.first) * per_tile;
-            for (int l0 = 0; ok && l0 < loads; l0 += 32) {
-                const int j = cur.first * KT + (l0 + lane) * plan.box;
-                int page = -1;
-                if (l0 + lane < loads && j < cur.q.len) {
-                    const int col = j >> a.c.page_log2;
-                    if (col < a.c.n_cols) page = __ldg(a.c.table + cur.s * a.c.table_stride + col);
-                    // (a page past the cache's end is outside the tensor map: zeros)
-                    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.n_pages)) {
-                        record_error(err, DEVERR_BAD_PAGE);
-                        page = -1;
-                    }
+    // ---- the ring: tiles come in windows of 32 page lookups (lane i: the i-th
+    // box), the next window's under way while this one's tiles are issued
+    const int boxes = KT / plan.box;  // of a tile
+    struct Window {
+        int t, end, hk, len, page;
+    };
+    Cursor ahead = cur;
+    int ahead_t = cur.first;
+    bool more = true;
+    auto look = [&]() {
+        Window w;
+        w.t = ahead_t;
+        w.end = min(ahead.end, ahead_t + 32 / boxes);
+        w.hk = ahead.hk;
+        w.len = ahead.q.len;
+        w.page = 0;
+        if (!more) {
+            w.end = w.t;
+            return w;
+        }
+        const int j = w.t * KT + lane * plan.box;
+        if (j < w.end * KT && j < w.len) {
+            const int col = j >> a.c.page_log2;
+            w.page = col < a.c.n_cols ? __ldg(a.c.table + ahead.s * a.c.table_stride + col) : -1;
+        }
+        ahead_t = w.end;
+        if (ahead_t == ahead.end) {
+            more = next_pair(ahead);
+            ahead_t = ahead.first;
+        }
+        return w;
+    };
+    uint8_t* ring = sm + warp * (C::STAGES * C::STAGE);
+    int issued = 0;
+    Window win = look(), then = look();
+    int base_t = win.t;
+    auto issue = [&](int stage) {
+        if (win.t == win.end) {
+            win = then;
+            base_t = win.t;
+            if (win.t == win.end) return;  // all issued
+            then = look();
+        }
+        if (win.t == base_t && static_cast<unsigned>(win.page) >= static_cast<unsigned>(a.c.n_pages)) {
+            record_error(err, DEVERR_BAD_PAGE);
+            win.page = -1;  // outside the tensor map: zeros
+        }
+        const uint32_t dst = smem_u32(ring) + stage * C::STAGE;
+        if (lane == 0) mbar_arrive_expect_tx(full + stage, C::STAGE);
+        for (int b = 0; b < boxes; b++) {
+            const int pg = __shfl_sync(0xffffffffu, win.page, (win.t - base_t) * boxes + b);
+            const int slot = (win.t * KT + b * plan.box) & (a.c.page - 1);
+            if (lane == 0)
+                for (int h = 0; h < C::HALVES / plan.box_halves; h++) {
+                    const int x = plan.by_value ? h * 64 : 0, y = plan.by_value ? 0 : h;
+                    const uint32_t at = dst + h * C::HALF + b * plan.box * 128;
+                    tma_load_5d(&tmK, full + stage, at, x, slot, y, win.hk, pg);
+                    tma_load_5d(&tmV, full + stage, at + C::HALVES * C::HALF, x, slot, y, win.hk, pg);
                 }
-                const int here = min(32, loads - l0);
-                for (int i = 0; i < here; i += per_tile) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(empty + stage, phase, err, DEVERR_PATTN_EMPTY));
-                    if (!ok) break;
-                    uint64_t* bar = full + stage;
-                    if (lane == 0) mbar_arrive_expect_tx(bar, C::STAGE / 2);
-                    for (int b = 0; b < per_tile; b++) {
-                        const int pg = __shfl_sync(0xffffffffu, page, i + b);
-                        const int slot = (cur.first * KT + (l0 + i + b) * plan.box) & (a.c.page - 1);
-                        if (lane == 0) {
-                            const uint32_t dst = base + stage * C::STAGE + b * plan.box * 128;
-                            for (int h = 0; h < loads_h; h++)
-                                tma_load_5d(map, bar, dst + h * C::HALF, plan.by_value ? h * 64 : 0, slot,
-                                            plan.by_value ? 0 : h, cur.hk, pg);
-                        }
-                    }
-                    n++;
-                    if (++stage == C::STAGES) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                }
-            }
-        } while (ok && next_pair());
-        // every load lands before the CTA may end
-        if (lane == 0)
-            for (int i = max(0, n - C::STAGES); i < n; i++)
-                mbar_wait(full + i % C::STAGES, (i / C::STAGES) & 1, nullptr, DEVERR_PATTN_DRAIN);
-        return;
-    }
+        }
+        win.t++;
+        issued++;
+    };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < C::STAGES; i++) issue(i);
 
-    // ---------------------------------------------------- consumers
     const float scale2 = a.scale * 1.4426950408889634f;
     const int g = lane >> 2, quad = lane & 3;
-    int parity = 0, n0 = 0;  // n0: the pair's first tile in the order of the ring
-    int turn = warp, stage = warp % C::STAGES, phase = 0;  // this warp's next tile there
+    int stage = 0, phase = 0;
     bool ok = true;
-    for (bool go = true; go; n0 += cur.end - cur.first, go = next_pair(), parity ^= 1) {
+    for (bool go = true; go; go = next_pair(cur)) {
         // ---- the pair's rows as A fragments
         const int rows = cur.q.n * group;
         uint32_t qf[DP / 16][4];
-        int pos[2];  // of this thread's two rows (below 0: sees nothing)
+        int pos[2];     // of this thread's two rows (below 0: sees nothing)
+        int64_t at[2];  // their place in out (below 0: none)
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
             const int r = g + hf * 8;
             const int i = r / group, gi = r - i * group;
             const bool in = r < rows;
             pos[hf] = in ? cur.q.len - cur.q.n + i : -1;
+            at[hf] = in ? static_cast<int64_t>(cur.q.row0 + i) * a.q_heads + cur.hk * group + gi : -1;
             const T* q = static_cast<const T*>(a.q) + (in ? (cur.q.row0 + i) * a.q_tok + (cur.hk * group + gi) * a.q_head : 0);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; kk++)
@@ -364,17 +385,16 @@ __global__ void __launch_bounds__(NTHR, 1)
 #pragma unroll
         for (int n = 0; n < DP / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
-        for (const int n1 = n0 + cur.end - cur.first; turn < n1; turn += NW) {
-            const int t = cur.first + turn - n0;
-            if (ok) ok = mbar_wait(full + stage, phase, err, DEVERR_PATTN_FULL);
-            const uint32_t ks = smem_u32(sm) + stage * C::STAGE, vs = ks + C::HALVES * C::HALF;
+        for (int t = cur.first; t < cur.end; t++) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + stage, phase, err, DEVERR_PATTN_FULL));
+            const uint32_t ks = smem_u32(ring) + stage * C::STAGE, vs = ks + C::HALVES * C::HALF;
             if ((t + 1) * KT > cur.q.len) {
                 // the values behind the sequence's end may be anything, and 0 x NaN is NaN: zeros
                 const int from = max(0, cur.q.len - t * KT);
                 for (int i = from * 8 + lane; i < KT * 8; i += 32)
 #pragma unroll
                     for (int h = 0; h < C::HALVES; h++)
-                        *reinterpret_cast<uint4*>(sm + stage * C::STAGE + (C::HALVES + h) * C::HALF + i * 16) =
+                        *reinterpret_cast<uint4*>(ring + stage * C::STAGE + (C::HALVES + h) * C::HALF + i * 16) =
                             make_uint4(0u, 0u, 0u, 0u);
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -449,146 +469,127 @@ __global__ void __launch_bounds__(NTHR, 1)
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty + stage);
-            stage += NW;
-            if (stage >= C::STAGES) {
-                stage -= C::STAGES;
+            __syncwarp();  // every lane is done with the stage
+            if (ok) issue(stage);
+            if (++stage == C::STAGES) {
+                stage = 0;
                 phase ^= 1;
             }
         }
 
-        // ---- join the warps' parts
-        float2* ml = reinterpret_cast<float2*>(sm + C::OFF_ML) + parity * NW * 16;
+        // ---- the pair's end: written, or left for the join
+        const bool begins = cur.first == cur.all.x, whole = begins && cur.end == cur.all.y;
+        if (begins && lane == 0) {
+            const int64_t at0 = stop - cur.left;  // the pair's first tile in the line
+            plan.spans[static_cast<int64_t>(cur.s) * a.c.kv_heads + cur.hk] =
+                make_int2(piece, static_cast<int>((at0 + cur.all.y - cur.all.x - 1) / per));
+        }
+        uint8_t* part = plan.parts + (static_cast<int64_t>(piece) * 2 + (begins ? 1 : 0)) * plan.slot;
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
-            float x = l[hf];
-            x += __shfl_xor_sync(0xffffffffu, x, 1);
-            x += __shfl_xor_sync(0xffffffffu, x, 2);
-            if (quad == 0) ml[warp * 16 + g + hf * 8] = make_float2(m[hf], x);
-        }
-        named_bar_sync(1, NC);
-        const bool whole = cur.first == cur.all.x && cur.end == cur.all.y;
-        const int slot = cur.first == cur.all.x ? 1 : 0;  // a pair that goes on after this piece, or came into it
-        uint8_t* part = plan.parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * C::SLOT;
-        float* buf = reinterpret_cast<float*>(sm + C::OFF_PART);
-        auto top_of = [&](int r) {
-            float t = ml[r].x;
-#pragma unroll
-            for (int w = 1; w < NW; w++) t = fmaxf(t, ml[w * 16 + r].x);
-            return t;
-        };
-        {
-            float f[2];
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                const float t = top_of(g + hf * 8);
-                f[hf] = t == -INFINITY ? 0.0f : ex2(m[hf] - t);
-            }
-            float* mine = buf + warp % (NW / 2) * (16 * DP);
-            if (warp >= NW / 2) {
-#pragma unroll
-                for (int n = 0; n < DP / 8; n++)
-#pragma unroll
-                    for (int hf = 0; hf < 2; hf++)
-                        *reinterpret_cast<float2*>(mine + (g + hf * 8) * DP + n * 8 + quad * 2) =
-                            make_float2(o[n][hf * 2] * f[hf], o[n][hf * 2 + 1] * f[hf]);
-            }
-            named_bar_sync(1, NC);
-            if (warp < NW / 2) {
-#pragma unroll
-                for (int n = 0; n < DP / 8; n++)
-#pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        float2* w = reinterpret_cast<float2*>(mine + (g + hf * 8) * DP + n * 8 + quad * 2);
-                        const float2 y = *w;
-                        *w = make_float2(fmaf(o[n][hf * 2], f[hf], y.x), fmaf(o[n][hf * 2 + 1], f[hf], y.y));
-                    }
-            }
-            named_bar_sync(1, NC);
-        }
-        for (int e = tid; e < rows * (DP / 4); e += NC) {
-            const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4;
-            if (d >= a.c.dim) continue;
-            float4 y = *reinterpret_cast<const float4*>(buf + r * DP + d);
-#pragma unroll
-            for (int w = 1; w < NW / 2; w++) {
-                const float4 z = *reinterpret_cast<const float4*>(buf + w * 16 * DP + r * DP + d);
-                y.x += z.x;
-                y.y += z.y;
-                y.z += z.z;
-                y.w += z.w;
-            }
-            const float t = top_of(r);
-            float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float2 z = ml[w * 16 + r];
-                sum += t == -INFINITY ? 0.0f : z.y * ex2(z.x - t);
-            }
+            float sum = l[hf];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (at[hf] < 0) continue;
+            const int r = g + hf * 8;
             if (whole) {
-                const int i = r / group, gi = r - i * group;
-                const int64_t at = static_cast<int64_t>(cur.q.row0 + i) * a.q_heads + cur.hk * group + gi;
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.c.dim + d) =
-                    make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
-                if (d == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (t + log2f(sum)) * 0.6931471805599453f;
+                T* out = static_cast<T*>(a.out) + at[hf] * a.c.dim + quad * 2;
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++)
+                    if (n * 8 < a.c.dim)
+                        *reinterpret_cast<uint32_t*>(out + n * 8) = pack2<T>(o[n][hf * 2] * inv, o[n][hf * 2 + 1] * inv);
+                if (quad == 0 && a.lse)
+                    a.lse[at[hf]] = sum == 0.0f ? -INFINITY : (m[hf] + log2f(sum)) * 0.6931471805599453f;
             } else {
-                *reinterpret_cast<float4*>(part + (r * DP + d) * 4) = y;
-                if (d == 0) *reinterpret_cast<float2*>(part + 16 * DP * 4 + r * 8) = make_float2(t, sum);
+                float* out = reinterpret_cast<float*>(part) + r * DP + quad * 2;
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++)
+                    if (n * 8 < a.c.dim)
+                        *reinterpret_cast<float2*>(out + n * 8) = make_float2(o[n][hf * 2], o[n][hf * 2 + 1]);
+                if (quad == 0)
+                    *reinterpret_cast<float2*>(part + (static_cast<int64_t>(plan.rows_cap) * DP * 4 + r * 8)) =
+                        make_float2(m[hf], sum);
             }
         }
-        if (whole) continue;
+    }
+    // after a timeout: what this warp has in flight lands before the CTA may end
+    if (!ok)
+        for (int i = max(0, issued - C::STAGES); i < issued; i++)
+            mbar_wait(full + i % C::STAGES, (i / C::STAGES) & 1, nullptr, DEVERR_PATTN_FULL);
+}
 
-        // ---- join the CTAs' parts: CTA c0 began the pair, c1 ends it
-        const int64_t at0 = stop - cur.left - (cur.first - cur.all.x);  // the pair's first tile in the line
-        const int c0 = static_cast<int>(at0 / per), c1 = static_cast<int>((at0 + cur.all.y - cur.all.x - 1) / per);
-        __threadfence();
-        named_bar_sync(1, NC);
-        if (tid == 0) *s_last = atomicAdd(plan.counters + c0, 1) == c1 - c0;
-        named_bar_sync(1, NC);
-        if (!*s_last) continue;
-        __threadfence();
-        for (int e = tid; e < rows * (DP / 4); e += NC) {
-            const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4;
-            if (d >= a.c.dim) continue;
-            auto slot_of = [&](int c) { return plan.parts + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * C::SLOT; };
-            float t = -INFINITY;
-            for (int c = c0; c <= c1; c++)
-                t = fmaxf(t, __ldcg(reinterpret_cast<const float2*>(slot_of(c) + 16 * DP * 4 + r * 8)).x);
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float sum = 0.0f;
-            for (int c = c0; c <= c1; c++) {
-                const float2 z = __ldcg(reinterpret_cast<const float2*>(slot_of(c) + 16 * DP * 4 + r * 8));
-                const float f = t == -INFINITY ? 0.0f : ex2(z.x - t);
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(slot_of(c) + (r * DP + d) * 4));
-                sum = fmaf(z.y, f, sum);
-                y.x = fmaf(x.x, f, y.x);
-                y.y = fmaf(x.y, f, y.y);
-                y.z = fmaf(x.z, f, y.z);
-                y.w = fmaf(x.w, f, y.w);
+// The rows of pairs that lie in several pieces: out = sum 2^(m - M) o / L over
+// the parts, in their order.  One CTA per row at a time; four warps share the
+// parts, a lane has DP / 32 values.  Bound: latency (the parts are in L2).
+constexpr int JW = 4;
+template <typename T, int DP>
+__global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs a, const RowsPlan plan) {
+    constexpr int E = DP / 32;
+    __shared__ float s_o[JW][DP];
+    __shared__ float2 s_ml[JW];
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = a.q_heads / a.c.kv_heads;
+    const int64_t all = static_cast<int64_t>(a.c.n_seq) * a.c.kv_heads * plan.rows_cap;
+    for (int64_t u = blockIdx.x; u < all; u += gridDim.x) {
+        const int64_t pair = u / plan.rows_cap;
+        const int r = static_cast<int>(u - pair * plan.rows_cap);
+        const int s = static_cast<int>(pair / a.c.kv_heads), hk = static_cast<int>(pair - static_cast<int64_t>(s) * a.c.kv_heads);
+        const Seq q = load_seq(a.c, s);
+        if (q.n == 0 || q.n > MAX_ROWS / group || r >= q.n * group) continue;
+        const int2 span = plan.spans[pair];
+        if (span.x == span.y) continue;
+        float t = -INFINITY, sum = 0.0f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.0f;
+#pragma unroll 4
+        for (int c = span.x + warp; c <= span.y; c += JW) {
+            const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == span.x ? 1 : 0)) * plan.slot;
+            const float2 ml = *reinterpret_cast<const float2*>(part + (static_cast<int64_t>(plan.rows_cap) * DP * 4 + r * 8));
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = reinterpret_cast<const float*>(part)[r * DP + e * 32 + lane];
+            const float t2 = fmaxf(t, ml.x), base = t2 == -INFINITY ? 0.0f : t2;
+            const float f = ex2(t - base), w = ex2(ml.x - base);
+            t = t2;
+            sum = sum * f + ml.y * w;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = o[e] * f + x[e] * w;
+        }
+        if (lane == 0) s_ml[warp] = make_float2(t, sum);
+#pragma unroll
+        for (int e = 0; e < E; e++) s_o[warp][e * 32 + lane] = o[e];
+        __syncthreads();
+        if (warp == 0) {
+            float top = s_ml[0].x;
+#pragma unroll
+            for (int w = 1; w < JW; w++) top = fmaxf(top, s_ml[w].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+            sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < JW; w++) {
+                const float f = ex2(s_ml[w].x - base);
+                sum += s_ml[w].y * f;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] += s_o[w][e * 32 + lane] * f;
             }
             const int i = r / group, gi = r - i * group;
-            const int64_t at = static_cast<int64_t>(cur.q.row0 + i) * a.q_heads + cur.hk * group + gi;
+            const int64_t at = static_cast<int64_t>(q.row0 + i) * a.q_heads + hk * group + gi;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.c.dim + d) =
-                make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
-            if (d == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (t + log2f(sum)) * 0.6931471805599453f;
+            T* out = static_cast<T*>(a.out) + at * a.c.dim;
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (e * 32 + lane < a.c.dim) out[e * 32 + lane] = from_f32<T>(o[e] * inv);
+            if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
         }
-        if (tid == 0) plan.counters[c0] = 0;
+        __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------- many rows
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // The sequence that packed row `row` belongs to (the last s with cu[s] <= row).
 __device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seq, int row) {
     int lo = 0, hi = n_seq;  // cu[lo] <= row < cu[hi] (cu[n_seq] taken as the end)
@@ -651,7 +652,28 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const PagedAtt
     if (lane == 0 && a.lse) a.lse[unit] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-constexpr int64_t kCounterBytes = 4096;  // at the workspace's start: a counter per CTA of any kernel here
+}  // namespace
+
+namespace {
+
+int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
+
+// Workspace of the rows kernel: spans of all pairs, then two parts per piece.
+struct RowsSpace {
+    int64_t spans = 0, slot = 0, bytes = 0;
+    int rows_cap = 0;
+};
+RowsSpace rows_space(const PagedAttnArgs& a, int sms) {
+    RowsSpace w;
+    const int group = a.q_heads / a.c.kv_heads;
+    if (group > MAX_ROWS || a.max_q == 0) return w;
+    const int dp = a.c.dim > 64 ? 128 : 64;
+    w.rows_cap = std::min(MAX_ROWS / group, a.max_q) * group;
+    w.slot = up256(w.rows_cap * (dp * 4ll + 8));
+    w.spans = up256(8ll * a.c.n_seq * a.c.kv_heads);
+    w.bytes = w.spans + 2ll * sms * NW * w.slot;
+    return w;
+}
 
 }  // namespace
 
@@ -659,7 +681,7 @@ int paged_attention_workspace(const PagedAttnArgs& a, int64_t* bytes) {
     int rc = 0;
     DeviceState* ds = device_state(&rc);
     if (!ds) return rc;
-    *bytes = kCounterBytes + 2ll * ds->sm_count * (a.c.dim > 64 ? RowsCfg<128>::SLOT : RowsCfg<64>::SLOT);
+    *bytes = rows_space(a, ds->sm_count).bytes;
     return TVQ_OK;
 }
 
@@ -686,10 +708,12 @@ int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     static const cudaError_t attr =
         cudaFuncSetAttribute(attn_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     TVQ_CUDA(attr);
+    const RowsSpace w = rows_space(a, ds->sm_count);
     RowsPlan plan;
-    plan.counters = static_cast<int*>(a.ws);
-    plan.parts = static_cast<uint8_t*>(a.ws) + kCounterBytes;
-    plan.min_tiles = 4;
+    plan.spans = static_cast<int2*>(a.ws);
+    plan.parts = static_cast<uint8_t*>(a.ws) + w.spans;
+    plan.rows_cap = w.rows_cap;
+    plan.slot = w.slot;
     plan.box = std::min(a.c.page, C::KT);
     plan.by_value = a.c.dim % 64 != 0;
     plan.box_halves = a.c.dim == 128 && plan.box == C::KT ? 2 : 1;
@@ -698,8 +722,12 @@ int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     if (rc) return rc;
     rc = cache_map(&tmV, a.c, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
     if (rc) return rc;
-    return launch_pdl(attn_rows_kernel<T, DP>, dim3(ds->sm_count), dim3(NTHR), C::SMEM, st, tmK, tmV, a, plan,
-                      ds->d_error);
+    rc = launch_pdl(attn_rows_kernel<T, DP>, dim3(ds->sm_count), dim3(NTHR), C::SMEM, st, tmK, tmV, a, plan,
+                    ds->d_error);
+    if (rc) return rc;
+    const int64_t rows = static_cast<int64_t>(a.c.n_seq) * a.c.kv_heads * w.rows_cap;
+    return launch_pdl(attn_join_kernel<T, DP>, dim3(static_cast<unsigned>(std::min<int64_t>(rows, ds->sm_count * 16ll))),
+                      dim3(JW * 32), 0, st, a, plan);
 }
 
 template <typename T>
@@ -720,7 +748,6 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     DeviceState* ds = device_state(&rc);
     if (!ds) return rc;
     TVQ_CHECK(ds->cc_major == 10, TVQ_ERR_UNSUPPORTED, "the paged attention needs an sm_100 device");
-    TVQ_CHECK(ds->sm_count * 4 <= kCounterBytes, TVQ_ERR_UNSUPPORTED, "more SMs than counters");
     if (a.c.n_rows == 0 || a.max_q == 0) return TVQ_OK;
     return a.c.type == TVQ_TYPE_F16 ? launch_attention<__half>(a, ds, st) : launch_attention<__nv_bfloat16>(a, ds, st);
 }

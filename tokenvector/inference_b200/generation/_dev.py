@@ -49,17 +49,17 @@ _workspaces = {}
 
 def workspace(op, dev, nbytes):
     """Scratch of one operator on the current stream of `dev`: calls on one
-    stream follow each other, so they share it.  Zero when new; the operators
-    leave their counters in it zero.  Under stream capture every call gets
-    its own out of the graph's memory, zeroed in the graph."""
+    stream follow each other, so they share it (nothing in it lasts from
+    call to call).  Under stream capture every call gets its own out of the
+    graph's memory."""
     if nbytes == 0:
         return None
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
     key = (op, dev.index, torch.cuda.current_stream(dev).cuda_stream)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
-        buf = _workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+        buf = _workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     return buf
 
 
