@@ -24,6 +24,9 @@
 //    and nothing in the CTA waits for another warp.  (Eight warps that share
 //    each pair and join it in shared memory took ~4000 cycles a pair more,
 //    which doubled the time of many short sequences.)
+//  - two producer warps fill the eight rings, eight lanes for each, whichever
+//    has a free stage: a TMA load costs its thread ~200 cycles, which
+//    doubled a tile's time when the consumers issued their own.
 //  - mma.sync m16n8k16 with the rows padded to 16: a warp's tile takes ~1000
 //    cycles from ring to ring, and the eight together 125 a tile where its
 //    bytes take ~330, so the wider tcgen05 tile (128 rows) would buy nothing.
@@ -42,12 +45,12 @@ namespace tvq {
 
 namespace {
 
-constexpr int NW = 8;              // warps of the rows kernel's CTA
-constexpr int NTHR = NW * 32;
+constexpr int NW = 8;              // consumer warps of the rows kernel's CTA
+constexpr int NTHR = (NW + 2) * 32;  // and two producer warps, a ring for every eight lanes
 constexpr int MAX_ROWS = 16;       // rows of a pair (new tokens x heads of the group)
 
 // device error codes: the wait that gave up first
-enum : int { DEVERR_PATTN_FULL = 72 };
+enum : int { DEVERR_PATTN_EMPTY = 71, DEVERR_PATTN_FULL = 72 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error ~2^-22, 2^-inf = 0
     float y;
@@ -75,6 +78,26 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A bounded wait that a page number out of range (recorded in the same word,
+// and no reason to stop) does not cut short.
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, int* err) {
+    const bool ok = mbar_wait_for(bar, parity, nullptr, DEVERR_PATTN_FULL, TVQ_WAIT_LIMIT_NS);
+    if (!ok) record_error(err, DEVERR_PATTN_FULL);
+    return ok;
+}
+
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 // 5-D TMA tile load {value, token, half, head, page}; what lies outside is zero.
@@ -151,9 +174,9 @@ struct RowsCfg {
     static constexpr int HALVES = DP / 64;
     static constexpr int STAGE = 2 * HALVES * HALF;      // one tile, 8 KB: keys, then values
     static constexpr int STAGES = 3;                     // of each warp
-    static constexpr int OFF_BAR = NW * STAGES * STAGE;  // full[NW][STAGES]
-    static constexpr int OFF_MISC = OFF_BAR + NW * STAGES * 8;  // int64 at[NW], int seq[NW], int scan[NW]
-    static constexpr int SMEM = OFF_MISC + NW * 16;
+    static constexpr int OFF_BAR = NW * STAGES * STAGE;  // full[NW][STAGES], empty[NW][STAGES]
+    static constexpr int OFF_MISC = OFF_BAR + 2 * NW * STAGES * 8;  // int64 at[NW], int seq[NW], int scan[NW + 2]
+    static constexpr int SMEM = OFF_MISC + NW * 16 + 8;
 };
 
 struct RowsPlan {
@@ -188,18 +211,21 @@ __global__ void __launch_bounds__(NTHR, 1)
     int* s_seq = reinterpret_cast<int*>(s_at + NW);
     int* s_scan = s_seq + NW;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + warp * C::STAGES;
+    // whose ring this thread serves: its warp's, or eight lanes' of a producer warp
+    const int mine = warp < NW ? warp : (warp - NW) * 4 + (lane >> 3);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + mine * C::STAGES;
+    uint64_t* empty = full + NW * C::STAGES;
+    uint8_t* ring = sm + mine * (C::STAGES * C::STAGE);
     const int group = a.q_heads / a.c.kv_heads;
     const int fit = MAX_ROWS / group;  // new rows of a sequence that this kernel takes
-    if (lane == 0) {
-        for (int i = 0; i < C::STAGES; i++) mbar_init(full + i, 1);
-        fence_barrier_init();
-    }
     if (tid == 0) {
+        for (int i = 0; i < 2 * NW * C::STAGES; i++) mbar_init(reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + i, 1);
+        fence_barrier_init();
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
     griddep_wait();
+    griddep_launch();  // the join kernel's CTAs fit beside this one's and wait there
 
     // ---- the pieces of the line of tiles
     auto weight = [&](int s) -> int {
@@ -218,7 +244,7 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (lane == 31) s_scan[warp] = x;
         __syncthreads();
         int sum = 0;
-        for (int w = 0; w < NW; w++) {
+        for (int w = 0; w < NW + 2; w++) {
             if (w < warp) x += s_scan[w];
             sum += s_scan[w];
         }
@@ -256,9 +282,9 @@ __global__ void __launch_bounds__(NTHR, 1)
         before += all;
     }
     __syncthreads();
-    const int piece = warp * gridDim.x + blockIdx.x;
+    const int piece = mine * gridDim.x + blockIdx.x;
     const int64_t begin = per * piece, stop = min(total, begin + per);
-    if (begin >= stop) return;
+    if (warp < NW && begin >= stop) return;
 
     Cursor cur;
     auto enter = [&](Cursor& c, int skip) {  // s, hk, left and q set: the pair's tiles from `skip` on
@@ -278,83 +304,112 @@ __global__ void __launch_bounds__(NTHR, 1)
         enter(c, 0);
         return true;
     };
-    cur.s = s_seq[warp];
-    cur.q = load_seq(a.c, cur.s);
     cur.left = stop - begin;
-    {
-        const int64_t in_seq = begin - s_at[warp];
+    if (cur.left > 0) {
+        cur.s = s_seq[mine];
+        cur.q = load_seq(a.c, cur.s);
+        const int64_t in_seq = begin - s_at[mine];
         const int2 t = seq_tiles<KT>(cur.q, a.window);
         cur.hk = static_cast<int>(in_seq / (t.y - t.x));
         enter(cur, static_cast<int>(in_seq - static_cast<int64_t>(cur.hk) * (t.y - t.x)));
     }
 
-    // ---- the ring: tiles come in windows of 32 page lookups (lane i: the i-th
-    // box), the next window's under way while this one's tiles are issued
-    const int boxes = KT / plan.box;  // of a tile
-    struct Window {
-        int t, end, hk, len, page;
-    };
-    Cursor ahead = cur;
-    int ahead_t = cur.first;
-    bool more = true;
-    auto look = [&]() {
-        Window w;
-        w.t = ahead_t;
-        w.end = min(ahead.end, ahead_t + 32 / boxes);
-        w.hk = ahead.hk;
-        w.len = ahead.q.len;
-        w.page = 0;
-        if (!more) {
-            w.end = w.t;
+    if (warp >= NW) {
+        // ------------------------------------------------ producers
+        // Eight lanes for a ring.  Its tiles come in windows of eight page
+        // lookups (lane i: the i-th box), the next window's under way while this
+        // one's tiles are issued; each of the lanes issues one load of a tile.
+        const int boxes = KT / plan.box, loads_h = C::HALVES / plan.box_halves, ops = 2 * boxes * loads_h;
+        const int sub = lane & 7, lead = lane & 24;
+        const bool is_v = sub & 1, issues = sub < ops;
+        const int b = (sub >> 1) / loads_h, h = (sub >> 1) - b * loads_h;
+        const uint32_t dst = smem_u32(ring) + (is_v ? C::HALVES * C::HALF : 0) + h * C::HALF + b * plan.box * 128;
+        const CUtensorMap* map = is_v ? &tmV : &tmK;
+        const int x = plan.by_value ? h * 64 : 0, y = plan.by_value ? 0 : h;
+        struct Window {
+            int t, end, hk, page;
+        };
+        int next_t = cur.left > 0 ? cur.first : 0;
+        bool more = cur.left > 0;
+        auto look = [&]() {
+            Window w;
+            w.t = w.end = next_t;
+            w.hk = cur.hk;
+            w.page = 0;
+            if (!more) return w;
+            w.end = min(cur.end, next_t + 8 / boxes);
+            const int j = w.t * KT + sub * plan.box;
+            if (j < w.end * KT && j < cur.q.len) {
+                const int col = j >> a.c.page_log2;
+                w.page = col < a.c.n_cols ? __ldg(a.c.table + cur.s * a.c.table_stride + col) : -1;
+            }
+            next_t = w.end;
+            if (next_t == cur.end) {
+                more = next_pair(cur);
+                next_t = cur.first;
+            }
             return w;
-        }
-        const int j = w.t * KT + lane * plan.box;
-        if (j < w.end * KT && j < w.len) {
-            const int col = j >> a.c.page_log2;
-            w.page = col < a.c.n_cols ? __ldg(a.c.table + ahead.s * a.c.table_stride + col) : -1;
-        }
-        ahead_t = w.end;
-        if (ahead_t == ahead.end) {
-            more = next_pair(ahead);
-            ahead_t = ahead.first;
-        }
-        return w;
-    };
-    uint8_t* ring = sm + warp * (C::STAGES * C::STAGE);
-    int issued = 0;
-    Window win = look(), then = look();
-    int base_t = win.t;
-    auto issue = [&](int stage) {
-        if (win.t == win.end) {
-            win = then;
-            base_t = win.t;
-            if (win.t == win.end) return;  // all issued
-            then = look();
-        }
-        if (win.t == base_t && static_cast<unsigned>(win.page) >= static_cast<unsigned>(a.c.n_pages)) {
-            record_error(err, DEVERR_BAD_PAGE);
-            win.page = -1;  // outside the tensor map: zeros
-        }
-        const uint32_t dst = smem_u32(ring) + stage * C::STAGE;
-        if (lane == 0) mbar_arrive_expect_tx(full + stage, C::STAGE);
-        for (int b = 0; b < boxes; b++) {
-            const int pg = __shfl_sync(0xffffffffu, win.page, (win.t - base_t) * boxes + b);
-            const int slot = (win.t * KT + b * plan.box) & (a.c.page - 1);
-            if (lane == 0)
-                for (int h = 0; h < C::HALVES / plan.box_halves; h++) {
-                    const int x = plan.by_value ? h * 64 : 0, y = plan.by_value ? 0 : h;
-                    const uint32_t at = dst + h * C::HALF + b * plan.box * 128;
-                    tma_load_5d(&tmK, full + stage, at, x, slot, y, win.hk, pg);
-                    tma_load_5d(&tmV, full + stage, at + C::HALVES * C::HALF, x, slot, y, win.hk, pg);
+        };
+        auto checked = [&](Window w) {
+            if (static_cast<unsigned>(w.page) >= static_cast<unsigned>(a.c.n_pages)) {
+                record_error(err, DEVERR_BAD_PAGE);
+                w.page = -1;  // outside the tensor map: zeros
+            }
+            return w;
+        };
+        int n = 0, stage = 0, phase = 1, pos = 0;  // tiles issued, the ring's place, tiles of the window issued
+        Window win = look(), then = look();
+        if (win.t < win.end) win = checked(win);
+        bool ok = true;
+        uint32_t idle = 0;
+        uint64_t since = 0;
+        while (true) {
+            const bool has = win.t + pos < win.end;
+            if (!__any_sync(0xffffffffu, has)) break;
+            bool ready = has && mbar_test(empty + stage, phase);
+            ready = __shfl_sync(0xffffffffu, ready, lead);
+            const int pg = __shfl_sync(0xffffffffu, win.page, lead + ((pos * boxes + b) & 7));
+            if (ready) {
+                if (sub == 0) mbar_arrive_expect_tx(full + stage, C::STAGE);
+                if (issues)
+                    tma_load_5d(map, full + stage, dst + stage * C::STAGE, x,
+                                ((win.t + pos) * KT + b * plan.box) & (a.c.page - 1), y, win.hk, pg);
+                n++;
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
                 }
+                if (win.t + ++pos == win.end) {
+                    win = then;
+                    pos = 0;
+                    if (win.t < win.end) {
+                        win = checked(win);
+                        then = look();
+                    }
+                }
+            }
+            if (__any_sync(0xffffffffu, ready)) {
+                idle = 0;
+            } else if ((++idle & 63u) == 0u) {  // nothing free for a while: the bound of every wait here
+                if (idle == 64u) since = globaltimer_ns();
+                else ok = globaltimer_ns() - since < TVQ_WAIT_LIMIT_NS;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) {
+                    record_error(err, DEVERR_PATTN_EMPTY);
+                    break;
+                }
+            } else {
+                __nanosleep(32);
+            }
         }
-        win.t++;
-        issued++;
-    };
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < C::STAGES; i++) issue(i);
+        // every load lands before the CTA may end
+        if (sub == 0)
+            for (int i = max(0, n - C::STAGES); i < n; i++)
+                wait_full(full + i % C::STAGES, (i / C::STAGES) & 1, nullptr);
+        return;
+    }
 
+    // ---------------------------------------------------- consumers
     const float scale2 = a.scale * 1.4426950408889634f;
     const int g = lane >> 2, quad = lane & 3;
     int stage = 0, phase = 0;
@@ -386,7 +441,7 @@ __global__ void __launch_bounds__(NTHR, 1)
         for (int n = 0; n < DP / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
         for (int t = cur.first; t < cur.end; t++) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + stage, phase, err, DEVERR_PATTN_FULL));
+            if (ok) ok = __all_sync(0xffffffffu, wait_full(full + stage, phase, err));
             const uint32_t ks = smem_u32(ring) + stage * C::STAGE, vs = ks + C::HALVES * C::HALF;
             if ((t + 1) * KT > cur.q.len) {
                 // the values behind the sequence's end may be anything, and 0 x NaN is NaN: zeros
@@ -470,7 +525,7 @@ __global__ void __launch_bounds__(NTHR, 1)
                 }
             }
             __syncwarp();  // every lane is done with the stage
-            if (ok) issue(stage);
+            if (lane == 0) mbar_arrive(empty + stage);
             if (++stage == C::STAGES) {
                 stage = 0;
                 phase ^= 1;
@@ -513,69 +568,74 @@ __global__ void __launch_bounds__(NTHR, 1)
             }
         }
     }
-    // after a timeout: what this warp has in flight lands before the CTA may end
-    if (!ok)
-        for (int i = max(0, issued - C::STAGES); i < issued; i++)
-            mbar_wait(full + i % C::STAGES, (i / C::STAGES) & 1, nullptr, DEVERR_PATTN_FULL);
 }
 
 // The rows of pairs that lie in several pieces: out = sum 2^(m - M) o / L over
-// the parts, in their order.  One CTA per row at a time; four warps share the
-// parts, a lane has DP / 32 values.  Bound: latency (the parts are in L2).
-constexpr int JW = 4;
-template <typename T, int DP>
+// the parts, in their order.  SHARE of a CTA's eight warps take a row together
+// (each its own parts), a lane has DP / 32 values.  Bound: latency (the parts
+// are in L2), so a row's parts are spread over as many warps as there are.
+constexpr int JW = 8;
+template <typename T, int DP, int SHARE>
 __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs a, const RowsPlan plan) {
-    constexpr int E = DP / 32;
+    constexpr int E = DP / 32, ROWS = JW / SHARE;
     __shared__ float s_o[JW][DP];
     __shared__ float2 s_ml[JW];
-    griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.q_heads / a.c.kv_heads;
     const int64_t all = static_cast<int64_t>(a.c.n_seq) * a.c.kv_heads * plan.rows_cap;
-    for (int64_t u = blockIdx.x; u < all; u += gridDim.x) {
-        const int64_t pair = u / plan.rows_cap;
+    bool waited = false;
+    for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * ROWS; u0 < all; u0 += static_cast<int64_t>(gridDim.x) * ROWS) {
+        const int64_t u = u0 + warp / SHARE, pair = u / plan.rows_cap;
         const int r = static_cast<int>(u - pair * plan.rows_cap);
         const int s = static_cast<int>(pair / a.c.kv_heads), hk = static_cast<int>(pair - static_cast<int64_t>(s) * a.c.kv_heads);
-        const Seq q = load_seq(a.c, s);
-        if (q.n == 0 || q.n > MAX_ROWS / group || r >= q.n * group) continue;
-        const int2 span = plan.spans[pair];
-        if (span.x == span.y) continue;
+        Seq q{0, 0, 0};
+        if (u < all) q = load_seq(a.c, s);  // (the rows kernel started this one after its own wait: they are there)
+        if (!waited) griddep_wait();
+        waited = true;
+        int2 span = make_int2(0, 0);
+        if (q.n > 0 && q.n <= MAX_ROWS / group && r < q.n * group) span = plan.spans[pair];
+        const bool act = span.x != span.y;
         float t = -INFINITY, sum = 0.0f, o[E];
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] = 0.0f;
+        if (act)
 #pragma unroll 4
-        for (int c = span.x + warp; c <= span.y; c += JW) {
-            const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == span.x ? 1 : 0)) * plan.slot;
-            const float2 ml = *reinterpret_cast<const float2*>(part + (static_cast<int64_t>(plan.rows_cap) * DP * 4 + r * 8));
-            float x[E];
+            for (int c = span.x + warp % SHARE; c <= span.y; c += SHARE) {
+                const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == span.x ? 1 : 0)) * plan.slot;
+                const float2 ml = *reinterpret_cast<const float2*>(part + (static_cast<int64_t>(plan.rows_cap) * DP * 4 + r * 8));
+                float x[E];
 #pragma unroll
-            for (int e = 0; e < E; e++) x[e] = reinterpret_cast<const float*>(part)[r * DP + e * 32 + lane];
-            const float t2 = fmaxf(t, ml.x), base = t2 == -INFINITY ? 0.0f : t2;
-            const float f = ex2(t - base), w = ex2(ml.x - base);
-            t = t2;
-            sum = sum * f + ml.y * w;
+                for (int e = 0; e < E; e++) x[e] = reinterpret_cast<const float*>(part)[r * DP + e * 32 + lane];
+                const float t2 = fmaxf(t, ml.x), base = t2 == -INFINITY ? 0.0f : t2;
+                const float f = ex2(t - base), w = ex2(ml.x - base);
+                t = t2;
+                sum = sum * f + ml.y * w;
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] = o[e] * f + x[e] * w;
-        }
-        if (lane == 0) s_ml[warp] = make_float2(t, sum);
+                for (int e = 0; e < E; e++) o[e] = o[e] * f + x[e] * w;
+            }
+        if constexpr (SHARE > 1) {
+            if (lane == 0) s_ml[warp] = make_float2(t, sum);
 #pragma unroll
-        for (int e = 0; e < E; e++) s_o[warp][e * 32 + lane] = o[e];
-        __syncthreads();
-        if (warp == 0) {
-            float top = s_ml[0].x;
+            for (int e = 0; e < E; e++) s_o[warp][e * 32 + lane] = o[e];
+            __syncthreads();
+            const int w0 = warp - warp % SHARE;
+            t = s_ml[w0].x;
 #pragma unroll
-            for (int w = 1; w < JW; w++) top = fmaxf(top, s_ml[w].x);
-            const float base = top == -INFINITY ? 0.0f : top;
+            for (int w = 1; w < SHARE; w++) t = fmaxf(t, s_ml[w0 + w].x);
+            const float base = t == -INFINITY ? 0.0f : t;
             sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; e++) o[e] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < JW; w++) {
-                const float f = ex2(s_ml[w].x - base);
-                sum += s_ml[w].y * f;
+            for (int w = 0; w < SHARE; w++) {
+                const float f = ex2(s_ml[w0 + w].x - base);
+                sum += s_ml[w0 + w].y * f;
 #pragma unroll
-                for (int e = 0; e < E; e++) o[e] += s_o[w][e * 32 + lane] * f;
+                for (int e = 0; e < E; e++) o[e] += s_o[w0 + w][e * 32 + lane] * f;
             }
+            __syncthreads();
+        }
+        if (act && warp % SHARE == 0) {
             const int i = r / group, gi = r - i * group;
             const int64_t at = static_cast<int64_t>(q.row0 + i) * a.q_heads + hk * group + gi;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -583,10 +643,10 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 #pragma unroll
             for (int e = 0; e < E; e++)
                 if (e * 32 + lane < a.c.dim) out[e * 32 + lane] = from_f32<T>(o[e] * inv);
-            if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+            if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (t + log2f(sum)) * 0.6931471805599453f;
         }
-        __syncthreads();
     }
+    if (!waited) griddep_wait();
 }
 
 // ---------------------------------------------------------------- many rows
@@ -725,9 +785,13 @@ int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     rc = launch_pdl(attn_rows_kernel<T, DP>, dim3(ds->sm_count), dim3(NTHR), C::SMEM, st, tmK, tmV, a, plan,
                     ds->d_error);
     if (rc) return rc;
+    // One CTA of the join fits beside the rows kernel's on an SM.  Rows for all of them: eight warps a row;
+    // more rows: a warp each.
     const int64_t rows = static_cast<int64_t>(a.c.n_seq) * a.c.kv_heads * w.rows_cap;
-    return launch_pdl(attn_join_kernel<T, DP>, dim3(static_cast<unsigned>(std::min<int64_t>(rows, ds->sm_count * 16ll))),
-                      dim3(JW * 32), 0, st, a, plan);
+    if (rows <= ds->sm_count)
+        return launch_pdl(attn_join_kernel<T, DP, JW>, dim3(static_cast<unsigned>(rows)), dim3(JW * 32), 0, st, a, plan);
+    const int64_t ctas = std::min<int64_t>((rows + JW - 1) / JW, ds->sm_count * 8ll);
+    return launch_pdl(attn_join_kernel<T, DP, 1>, dim3(static_cast<unsigned>(ctas)), dim3(JW * 32), 0, st, a, plan);
 }
 
 template <typename T>
