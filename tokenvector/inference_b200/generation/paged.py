@@ -54,33 +54,65 @@ def _rows(t, heads, dim, name):
         raise ValueError("%s must be contiguous in its last dimension" % name)
 
 
-def paged_append(k, v, k_pages, v_pages, table, ctx_len, cu=None, *, q=None):
-    """Write the new rows k, v [rows, kv_heads, head_dim] (float32, float16 or
-    bfloat16; strided rows of a projection's output will do) into the cache,
-    rounded once to its type.  q [rows, heads, head_dim] of the same type as k
-    is rounded with them and returned contiguous (None without q).  ctx_len
-    counts the new tokens already."""
+_appends, _attentions = D.Forms(), D.Forms()
+
+
+def _append_form(k, v, k_pages, v_pages, table, ctx_len, cu, q):
     dev, kind, shape, strides = _cache(k_pages, v_pages, table, ctx_len, cu, k.shape[0])
     heads, dim = k_pages.shape[2:]
     _rows(k, heads, dim, "k")
     _rows(v, heads, dim, "v")
     if k.dtype not in D.TYPES or v.dtype is not k.dtype or v.shape[0] != k.shape[0]:
         raise ValueError("k and v must be float32, float16 or bfloat16 rows, alike")
-    q_out, q_heads, qs = None, 0, (0, 0)
+    q_heads, qs = 0, (0, 0)
     if q is not None:
         _rows(q, None, dim, "q")
         if q.dtype is not k.dtype or q.shape[0] != k.shape[0]:
             raise ValueError("q must have k's type and rows")
-        q_out = torch.empty(q.shape, dtype=k_pages.dtype, device=dev)
         q_heads, qs = q.shape[1], q.stride()[:2]
     D.check_dev(dev, k=k, v=v, q=q)
-    with torch.cuda.device(dev):
-        N.call("tvq_dev_paged_append", kind, D.TYPES[k.dtype], k.data_ptr(), v.data_ptr(),
-               q.data_ptr() if q_heads else None, D.i64s(*k.stride()[:2], *v.stride()[:2], *qs), q_heads,
-               q_out.data_ptr() if q_heads else None, k_pages.data_ptr(), v_pages.data_ptr(), shape, strides,
-               table.data_ptr(), table.stride(0), table.shape[1], ctx_len.data_ptr(),
-               D.ptr(cu), ctx_len.shape[0], k.shape[0], D.stream(dev))
+    return (dev, kind, D.TYPES[k.dtype], D.i64s(*k.stride()[:2], *v.stride()[:2], *qs), q_heads, shape, strides,
+            table.stride(0), table.shape[1], ctx_len.shape[0], k.shape[0])
+
+
+def paged_append(k, v, k_pages, v_pages, table, ctx_len, cu=None, *, q=None):
+    """Write the new rows k, v [rows, kv_heads, head_dim] (float32, float16 or
+    bfloat16; strided rows of a projection's output will do) into the cache,
+    rounded once to its type.  q [rows, heads, head_dim] of the same type as k
+    is rounded with them and returned contiguous (None without q).  ctx_len
+    counts the new tokens already."""
+    key = (D.form(k), D.form(v), D.form(k_pages), D.form(v_pages), D.form(table), D.form(ctx_len), D.form(cu),
+           D.form(q))
+    found = _appends.get(key) or _appends.keep(key, _append_form(k, v, k_pages, v_pages, table, ctx_len, cu, q))
+    dev, kind, source, src_strides, q_heads, shape, strides, table_stride, cols, seqs, n_rows = found
+    q_out = None if q is None else torch.empty(q.shape, dtype=k_pages.dtype, device=dev)
+    D.call("tvq_dev_paged_append", dev, kind, source, k.data_ptr(), v.data_ptr(), D.ptr(q), src_strides, q_heads,
+           D.ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(), shape, strides, table.data_ptr(), table_stride, cols,
+           ctx_len.data_ptr(), D.ptr(cu), seqs, n_rows, D.stream(dev))
     return q_out
+
+
+def _attention_form(q, k_pages, v_pages, table, ctx_len, cu, out, max_q, window):
+    n_rows = q.shape[0]
+    dev, kind, shape, strides = _cache(k_pages, v_pages, table, ctx_len, cu, n_rows)
+    kv_heads, dim = k_pages.shape[2:]
+    _rows(q, None, dim, "q")
+    heads = q.shape[1]
+    if q.dtype is not k_pages.dtype:
+        raise ValueError("q must have the cache's type")
+    if heads % kv_heads or heads == 0:
+        raise ValueError("q's heads must be a multiple of the cache's")
+    if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous()):
+        raise ValueError("out must be contiguous, with q's shape and type")
+    if window < 0:
+        raise ValueError("window must not be negative")
+    D.check_dev(dev, q=q, out=out)
+    most = (1 if cu is None else n_rows) if max_q is None else int(max_q)
+    seqs = ctx_len.shape[0]
+    with torch.cuda.device(dev):
+        need = D.needed("tvq_paged_attention_workspace", heads, kv_heads, dim, seqs, n_rows, most)
+    return (dev, kind, D.i64s(*q.stride()[:2]), heads, shape, strides, table.stride(0), table.shape[1], seqs, n_rows,
+            most, need, 1.0 / math.sqrt(dim))
 
 
 def paged_attention(q, k_pages, v_pages, table, ctx_len, cu=None, *, max_q=None, scale=None, window=0, out=None,
@@ -96,30 +128,17 @@ def paged_attention(q, k_pages, v_pages, table, ctx_len, cu=None, *, max_q=None,
     `out` if given: contiguous, q's shape and type), or (out, lse) with lse
     float32 [rows, heads], the natural logarithm of the softmax's
     denominators.  A row without keys gives 0 and -inf."""
-    n_rows = q.shape[0]
-    dev, kind, shape, strides = _cache(k_pages, v_pages, table, ctx_len, cu, n_rows)
-    kv_heads, dim = k_pages.shape[2:]
-    _rows(q, None, dim, "q")
-    heads = q.shape[1]
-    if q.dtype is not k_pages.dtype:
-        raise ValueError("q must have the cache's type")
-    if heads % kv_heads or heads == 0:
-        raise ValueError("q's heads must be a multiple of the cache's")
+    key = (D.form(q), D.form(k_pages), D.form(v_pages), D.form(table), D.form(ctx_len), D.form(cu), D.form(out),
+           max_q, window)
+    found = _attentions.get(key) or _attentions.keep(key, _attention_form(q, k_pages, v_pages, table, ctx_len, cu, out,
+                                                                          max_q, window))
+    dev, kind, q_strides, heads, shape, strides, table_stride, cols, seqs, n_rows, most, need, root = found
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
-        raise ValueError("out must be contiguous, with q's shape and type")
-    if window < 0:
-        raise ValueError("window must not be negative")
     lse = torch.empty((n_rows, heads), dtype=torch.float32, device=dev) if return_lse else None
-    D.check_dev(dev, q=q, out=out)
-    most = (1 if cu is None else n_rows) if max_q is None else int(max_q)
-    with torch.cuda.device(dev):
-        need = D.needed("tvq_paged_attention_workspace", heads, kv_heads, dim, ctx_len.shape[0], n_rows, most)
-        ws = D.workspace("paged_attention", dev, need)
-        N.call("tvq_dev_paged_attention", kind, q.data_ptr(), D.i64s(*q.stride()[:2]), heads, k_pages.data_ptr(),
-               v_pages.data_ptr(), shape, strides, table.data_ptr(), table.stride(0), table.shape[1],
-               ctx_len.data_ptr(), D.ptr(cu), ctx_len.shape[0], n_rows, most,
-               1.0 / math.sqrt(dim) if scale is None else scale, window, out.data_ptr(),
-               D.ptr(lse), D.ptr(ws), need, D.stream(dev))
+    stream = D.stream(dev)
+    ws = D.workspace("paged_attention", dev, stream, need)
+    D.call("tvq_dev_paged_attention", dev, kind, q.data_ptr(), q_strides, heads, k_pages.data_ptr(),
+           v_pages.data_ptr(), shape, strides, table.data_ptr(), table_stride, cols, ctx_len.data_ptr(), D.ptr(cu), seqs,
+           n_rows, most, root if scale is None else scale, window, out.data_ptr(), D.ptr(lse), D.ptr(ws), need, stream)
     return (out, lse) if return_lse else out
