@@ -36,6 +36,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "tvq_common.cuh"
 #include "tvq_decode.h"
@@ -58,8 +59,6 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error ~2^-22, 
     return y;
 }
 
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <typename T>
 __device__ __forceinline__ T from_f32(float x);
 template <>
@@ -650,66 +649,685 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 }
 
 // ---------------------------------------------------------------- many rows
-// The sequence that packed row `row` belongs to (the last s with cu[s] <= row).
-__device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seq, int row) {
-    int lo = 0, hi = n_seq;  // cu[lo] <= row < cu[hi] (cu[n_seq] taken as the end)
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(cu + mid) <= row) lo = mid;
-        else hi = mid;
+// attn_tile_kernel: sequences of more than 16 rows, on the tcgen05 tensor
+// cores.  A unit is two tiles of up to 128 rows (whole tokens: 128 / group of
+// them, with all heads of the group) of one (sequence, kv head), which share
+// the stream of 128-key tiles of K and V.  All (unit, key tile) stand in one
+// line that is cut into equal pieces, one for each SM, as above, so ragged
+// prompts, causal triangles and few rows over many keys all fill the GPU;
+// units cut by a piece's end are joined by attn_tile_join_kernel.
+//
+// Per tile t and key tile j, in tensor memory: S_t = Q_t K_j^T (128 x 128
+// f32), its softmax's weights P_t (16-bit, over S_t's columns), O_t += P_t V_j.
+//   warp 0       TMA: Q of a unit, then K_j, V_j through one ring
+//   warp 1       MMA issuer: for each j, PV_A(j-1), S_A(j), PV_B(j-1), S_B(j),
+//                so one tile's softmax runs under the other's products
+//   warp 2       tensor memory; zeros over the values behind a sequence's end
+//                (they may be anything, and 0 x NaN is NaN)
+//   warp 3       walks the piece and leaves the units for the others in shared
+//                memory, up to four ahead
+//   warps 4-7, 8-11  softmax of tile A, B: a thread has a row, all 128 keys
+// O stays relative to the row's first maximum until the running one exceeds it
+// by 2^8 (then O and l are scaled by the softmax warps): weights stay below
+// 2^8, exact enough in either 16-bit type, and nearly no tile is scaled twice.
+// A commit of S_t(j) covers PV_t(j-1), issued before it, so scaling O needs no
+// barrier of its own; and in-order execution of the products lets S_t(j)
+// overwrite P_t(j-1) right behind the product that reads it.
+// Bound: two products of 128 x 128 x D (2 x 512 cycles at D = 128) and 128 x
+// 128 exponentials (1024 cycles of the special-function units) per tile and j.
+constexpr int TM = 128, TKEYS = 128;
+constexpr int TTHR = 384;
+enum : int {
+    DEVERR_PTILE_EMPTY = 73, DEVERR_PTILE_Q = 74, DEVERR_PTILE_KV = 75, DEVERR_PTILE_P = 76, DEVERR_PTILE_S = 77,
+    DEVERR_PTILE_O = 78, DEVERR_PTILE_FIX = 79, DEVERR_PTILE_DRAIN = 80, DEVERR_PTILE_WORK = 81
+};
+
+template <int DP>
+struct TileCfg {
+    static constexpr int HALVES = DP / 64;
+    static constexpr int HALF = 128 * 128;               // 128 rows of 64 values, 128-byte swizzle
+    static constexpr int QT = HALVES * HALF;             // one tile of Q
+    static constexpr int STAGE = HALVES * HALF;          // 128 keys or values
+    static constexpr int STAGES = 163840 / STAGE;        // 5 or 10
+    static constexpr int OFF_RING = 2 * QT;
+    static constexpr int OFF_BAR = OFF_RING + STAGES * STAGE;
+    static constexpr int OFF_WORK = OFF_BAR + (2 * STAGES + 22) * 8;  // Work[4]
+    static constexpr int OFF_MISC = OFF_WORK + 4 * 96;   // int64 at, int seq, tmem
+    static constexpr int SMEM = OFF_MISC + 16;
+    static constexpr int64_t SLOT = 2 * TM * (DP * 4 + 8);
+    static constexpr uint32_t COL_S = 0, COL_O = 256, COLS = DP == 128 ? 512 : 512;
+};
+
+struct TilePlan {
+    uint8_t* parts;  // [grid][2] slots: f32 [256][DP], then float2 (m, l) [256]
+    int4* begun;     // [grid]: {s, hk, unit, last piece} of the unit that a piece begins and does not end (s -1: none)
+    int tokens;      // of a tile: 128 / group
+    int box, box_halves, by_value;  // as RowsPlan's, KT = 128
+    float scale2;    // log2(e) |scale|, not 0
+    int negative;
+};
+
+// A unit's tiles of rows: tokens [i0, i0 + cnt) each, key tiles [first, end).
+struct Unit {
+    int i0[2], cnt[2], first[2], end[2];
+    int f, e;  // of both
+};
+__device__ __forceinline__ Unit make_unit(const Seq& q, int u, int tokens, int window) {
+    Unit w;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        w.i0[t] = (2 * u + t) * tokens;
+        w.cnt[t] = max(0, min(tokens, q.n - w.i0[t]));
+        const int pa = q.len - q.n + w.i0[t], pb = pa + w.cnt[t] - 1;
+        w.first[t] = window > 0 ? max(0, pa - window + 1) / TKEYS : 0;
+        w.end[t] = max(w.first[t] + 1, (max(pb + 1, 0) + TKEYS - 1) / TKEYS);
+        if (w.cnt[t] == 0) w.first[t] = w.end[t] = 0;
     }
-    return lo;
+    w.f = w.first[0];
+    w.e = max(w.end[0], w.end[1]);
+    return w;
+}
+__device__ __forceinline__ int seq_units(const Seq& q, int tokens) { return (q.n + 2 * tokens - 1) / (2 * tokens); }
+
+// A unit's share of a CTA's piece: key tiles [a, b), of them [lo, hi) for each
+// row tile (lo >= hi: none).
+struct Work {
+    int hk, row0, n, len, a, b, more;
+    int whole, begins;  // the piece holds all of the unit's key tiles; the first of them
+    int i0[2], cnt[2], lo[2], hi[2];
+    int s, pad[4];
+};
+static_assert(sizeof(Work) == 88);
+
+// Q_t K_j^T with B transposed as given by idesc; A in tensor memory for P V.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// A B operand whose N runs along the rows of 128 bytes (V: [key][value]): groups
+// of 64 values HALF bytes apart, groups of 8 keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t group) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(group >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+__device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* bar, uint32_t dst, int c0, int c1, int c2,
+                                            int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// wait_full with a code
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* err, int code) {
+    const bool ok = mbar_wait_for(bar, parity, nullptr, code, TVQ_WAIT_LIMIT_NS);
+    if (!ok) record_error(err, code);
+    return ok;
 }
 
-// The plain kernel: one warp per (row, head), keys one after another, the
-// softmax's running maximum and sum in f32 (m' = max(m, s), l' = l 2^(m - m')
-// + 2^(s - m'), o' likewise), four values of the head dim per lane.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attention_row_kernel(const PagedAttnArgs a, int skip, int* err) {
-    griddep_wait();
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (unit >= static_cast<int64_t>(a.c.n_rows) * a.q_heads) return;
-    const int row = static_cast<int>(unit / a.q_heads), h = static_cast<int>(unit - static_cast<int64_t>(row) * a.q_heads);
-    const int hk = h / (a.q_heads / a.c.kv_heads);
-    const int s = a.c.cu ? seq_of_row(a.c.cu, a.c.n_seq, row) : row;
-    const int n = a.c.cu ? __ldg(a.c.cu + s + 1) - __ldg(a.c.cu + s) : 1;
-    const int i = a.c.cu ? row - __ldg(a.c.cu + s) : 0;
-    if (i < 0 || i >= n || i >= a.max_q) return;  // a row of no sequence
-    if (n <= skip) return;
-    const int p = __ldg(a.c.ctx + s) - n + i;
-    const float scale2 = a.scale * 1.4426950408889634f;
-    float q[4], o[4] = {0, 0, 0, 0};
-    const int d0 = lane * 4;
-    const bool in = d0 < a.c.dim;
-    const T* qp = static_cast<const T*>(a.q) + row * a.q_tok + h * a.q_head + d0;
-    for (int c = 0; c < 4; c++) q[c] = in ? to_f32(qp[c]) * scale2 : 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    const int first = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    for (int j = first; j <= p; j++) {
-        const int col = j >> a.c.page_log2, slot = j & (a.c.page - 1);
-        const int pg = col < a.c.n_cols ? __ldg(a.c.table + s * a.c.table_stride + col) : -1;
-        float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-        if (static_cast<unsigned>(pg) >= static_cast<unsigned>(a.c.n_pages)) {
-            record_error(err, DEVERR_BAD_PAGE);
-        } else if (in) {
-            const T* kp = static_cast<const T*>(a.c.k) + pg * a.c.k_page + slot * a.c.k_tok + hk * a.c.k_head + d0;
-            const T* vp = static_cast<const T*>(a.c.v) + pg * a.c.v_page + slot * a.c.v_tok + hk * a.c.v_head + d0;
-            for (int c = 0; c < 4; c++) { k[c] = to_f32(kp[c]); v[c] = to_f32(vp[c]); }
+template <typename T, int DP>
+__global__ void __launch_bounds__(TTHR, 1)
+    attn_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const PagedAttnArgs a, const TilePlan plan, int* err) {
+    using C = TileCfg<DP>;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint64_t* kv_full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+    uint64_t* kv_empty = kv_full + C::STAGES;
+    uint64_t* q_full = kv_empty + C::STAGES;  // [2] each
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* s_full = q_empty + 2;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_full = p_full + 2;
+    uint64_t* v_fixed = o_full + 2;
+    uint64_t* drain = v_fixed + 1;
+    uint64_t* w_full = drain + 1;  // [4] each
+    uint64_t* w_empty = w_full + 4;
+    uint64_t* v_last = w_empty + 4;  // the values to be fixed are on their way
+    Work* works = reinterpret_cast<Work*>(sm + C::OFF_WORK);
+    int64_t* s_at = reinterpret_cast<int64_t*>(sm + C::OFF_MISC);
+    int* s_seq = reinterpret_cast<int*>(s_at + 1);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(s_seq + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int group = a.q_heads / a.c.kv_heads;
+    const int fit = MAX_ROWS / group;  // new rows of a sequence that the rows kernel takes
+    if (tid == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(kv_full + i, 1);
+            mbar_init(kv_empty + i, 1);
         }
-        float x = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-        for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        const float m2 = fmaxf(m, x);
-        const float f = m2 == -INFINITY ? 0.0f : exp2f(m - m2), e = m2 == -INFINITY ? 0.0f : exp2f(x - m2);
-        m = m2;
-        l = l * f + e;
-        for (int c = 0; c < 4; c++) o[c] = o[c] * f + e * v[c];
+        for (int t = 0; t < 2; t++) {
+            mbar_init(q_full + t, 1);
+            mbar_init(q_empty + t, 1);
+            mbar_init(s_full + t, 1);
+            mbar_init(p_full + t, 4);
+            mbar_init(o_full + t, 1);
+        }
+        mbar_init(v_fixed, 1);
+        mbar_init(v_last, 1);
+        mbar_init(drain, 1);
+        for (int i = 0; i < 4; i++) {
+            mbar_init(w_full + i, 1);
+            mbar_init(w_empty + i, 11);  // TMA, MMA, fixing and eight softmax warps
+        }
+        fence_barrier_init();
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
     }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    T* op = static_cast<T*>(a.out) + unit * a.c.dim + d0;
-    if (in)
-        for (int c = 0; c < 4; c++) op[c] = from_f32<T>(o[c] * inv);
-    if (lane == 0 && a.lse) a.lse[unit] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    if (warp == 2) {
+        tmem_alloc(tmem_holder, C::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    griddep_wait();
+
+    // ---- the piece of the line of key tiles
+    auto weight = [&](int s) -> int64_t {  // of one kv head
+        if (s >= a.c.n_seq) return 0;
+        const Seq q = load_seq(a.c, s);
+        if (q.n <= fit) return 0;
+        int64_t sum = 0;
+        for (int u = 0; u < seq_units(q, plan.tokens); u++) {
+            const Unit w = make_unit(q, u, plan.tokens, a.window);
+            sum += w.e - w.f;
+        }
+        return sum;
+    };
+    auto scan = [&](int64_t x, int64_t* all) {  // inclusive, over the CTA (the ring's memory is free yet)
+        int64_t* buf = reinterpret_cast<int64_t*>(sm + C::OFF_RING);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) buf[warp] = x;
+        __syncthreads();
+        int64_t sum = 0;
+        for (int w = 0; w < TTHR / 32; w++) {
+            if (w < warp) x += buf[w];
+            sum += buf[w];
+        }
+        *all = sum;
+        return x;
+    };
+    int64_t total = 0, w0 = 0, inc0 = 0;
+    for (int s0 = 0; s0 < a.c.n_seq; s0 += TTHR) {
+        int64_t all;
+        w0 = weight(s0 + tid);
+        inc0 = scan(w0, &all);
+        total += all;
+    }
+    total *= a.c.kv_heads;
+    const int64_t per = max(static_cast<int64_t>(1), (total + gridDim.x - 1) / gridDim.x);
+    const int64_t begin = per * blockIdx.x, stop = min(total, begin + per);
+    int64_t before = 0;
+    for (int s0 = 0; s0 < a.c.n_seq; s0 += TTHR) {
+        int64_t all = 0, w = w0, inc = inc0;
+        if (a.c.n_seq > TTHR) {
+            w = weight(s0 + tid);
+            inc = scan(w, &all);
+        }
+        const int64_t hi = (before + inc) * a.c.kv_heads, lo = hi - w * a.c.kv_heads;
+        if (w > 0 && begin >= lo && begin < hi) {
+            *s_seq = s0 + tid;
+            *s_at = lo;
+        }
+        before += all;
+    }
+    fence_proxy_async_smem();  // (the scan's words in the ring, before TMA writes there)
+    __syncthreads();
+    bool ok = true;
+    // the k-th unit of the piece; false: there is none (or a wait gave up)
+    auto take = [&](int k) -> bool {
+        ok = ok && wait_bar(w_full + (k & 3), (k >> 2) & 1, err, DEVERR_PTILE_WORK);
+        return ok && works[k & 3].more;
+    };
+    auto done = [&](int k) {  // by one thread of a warp, once the warp needs nothing more of it
+        mbar_arrive(w_empty + (k & 3));
+    };
+    // a softmax thread holds a row of 128 scores: 256 x 208 + 128 x 88 registers of the 384 x 168 launched with
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 3) {
+            // ------------------------------------------------ the walk
+            if (lane == 0) {
+                int4 begun = make_int4(-1, 0, 0, 0);
+                int s = 0, hk = 0, u = 0, skip = 0, units = 0;
+                int64_t left = stop - begin;
+                Seq q{0, 0, 0};
+                if (left > 0) {
+                    s = *s_seq;
+                    q = load_seq(a.c, s);
+                    int64_t in = begin - *s_at, one = 0;  // one: tiles of one kv head
+                    units = seq_units(q, plan.tokens);
+                    for (int i = 0; i < units; i++) {
+                        const Unit w = make_unit(q, i, plan.tokens, a.window);
+                        one += w.e - w.f;
+                    }
+                    hk = static_cast<int>(in / one);
+                    in -= hk * one;
+                    for (u = 0; u < units; u++) {
+                        const Unit w = make_unit(q, u, plan.tokens, a.window);
+                        if (in < w.e - w.f) break;
+                        in -= w.e - w.f;
+                    }
+                    skip = static_cast<int>(in);
+                }
+                for (int k = 0;; k++) {
+                    ok = ok && wait_bar(w_empty + (k & 3), ((k >> 2) & 1) ^ 1, err, DEVERR_PTILE_WORK);
+                    if (!ok) break;
+                    Work& o = works[k & 3];
+                    o.more = left > 0;
+                    if (left > 0) {
+                        const Unit w = make_unit(q, u, plan.tokens, a.window);
+                        o.s = s;
+                        o.hk = hk;
+                        o.row0 = q.row0;
+                        o.n = q.n;
+                        o.len = q.len;
+                        o.a = w.f + skip;
+                        o.b = static_cast<int>(min(static_cast<int64_t>(w.e), o.a + left));
+                        o.begins = skip == 0;
+                        o.whole = skip == 0 && o.b == w.e;
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            o.i0[t] = w.i0[t];
+                            o.cnt[t] = w.cnt[t];
+                            o.lo[t] = max(w.first[t], o.a);
+                            o.hi[t] = min(w.end[t], o.b);
+                        }
+                        if (o.begins && !o.whole)
+                            begun = make_int4(s, hk, u, static_cast<int>((stop - left + w.e - w.f - 1) / per));
+                        left -= o.b - o.a;
+                        skip = 0;
+                        if (left > 0 && ++u == units) {
+                            u = 0;
+                            if (++hk == a.c.kv_heads) {
+                                hk = 0;
+                                do {
+                                    q = load_seq(a.c, ++s);
+                                } while (q.n <= fit);
+                                units = seq_units(q, plan.tokens);
+                            }
+                        }
+                    }
+                    mbar_arrive(w_full + (k & 3));
+                    if (!o.more) break;
+                }
+                plan.begun[blockIdx.x] = begun;
+            }
+            __syncwarp();
+        } else if (warp == 0) {
+            // ------------------------------------------------ TMA
+            const int boxes = TKEYS / plan.box, loads_h = C::HALVES / plan.box_halves, ops = boxes * loads_h;
+            const int b = lane / loads_h, h = lane - b * loads_h;
+            const bool issues = lane < ops;
+            const int x = plan.by_value ? h * 64 : 0, y = plan.by_value ? 0 : h;
+            const uint32_t ring = smem_u32(sm) + C::OFF_RING + h * C::HALF + b * plan.box * 128;
+            int n = 0, stage = 0, phase = 1, nq0 = 0, nq1 = 0;
+            for (int k = 0; __all_sync(0xffffffffu, take(k)); k++) {
+                const Work& w = works[k & 3];
+                const int hk = w.hk, len = w.len, end = w.b;
+                const int32_t* row = a.c.table + w.s * a.c.table_stride;
+                auto look = [&](int j) {
+                    const int key = j * TKEYS + b * plan.box;
+                    if (!issues || j >= end || key >= len) return 0;
+                    const int col = key >> a.c.page_log2;
+                    return col < a.c.n_cols ? __ldg(row + col) : -1;
+                };
+                int page = look(w.a);
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    int& nq = t ? nq1 : nq0;
+                    if (w.lo[t] >= w.hi[t]) continue;
+                    ok = ok && wait_bar(q_empty + t, (nq & 1) ^ 1, err, DEVERR_PTILE_EMPTY);
+                    if (ok && lane == 0) {
+                        mbar_arrive_expect_tx(q_full + t, C::HALVES * plan.tokens * group * 128);
+                        for (int i = 0; i < C::HALVES; i++)
+                            tma_load_4d(&tmQ, q_full + t, smem_u32(sm) + t * C::QT + i * C::HALF, plan.by_value ? i * 64 : 0,
+                                        plan.by_value ? 0 : i, hk * group, w.row0 + w.i0[t]);
+                    }
+                    if (ok) nq++;
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                for (int j = w.a; ok && j < end; j++) {
+                    int now = page;
+                    page = look(j + 1);
+                    if (static_cast<unsigned>(now) >= static_cast<unsigned>(a.c.n_pages)) {
+                        record_error(err, DEVERR_BAD_PAGE);
+                        now = -1;  // outside the tensor map: zeros
+                    }
+                    // (a box behind the sequence's end, of a page that is not its own, is not read either)
+                    if (j * TKEYS + b * plan.box >= len) now = -1;
+                    const int slot = (j * TKEYS + b * plan.box) & (a.c.page - 1);
+                    for (int v = 0; v < 2; v++) {
+                        ok = __all_sync(0xffffffffu, wait_bar(kv_empty + stage, phase, err, DEVERR_PTILE_EMPTY));
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(kv_full + stage, C::STAGE);
+                        __syncwarp();
+                        if (issues)
+                            tma_load_5d(v ? &tmV : &tmK, kv_full + stage, ring + stage * C::STAGE, x, slot, y, hk, now);
+                        n++;
+                        if (++stage == C::STAGES) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                    if (ok && (j + 1) * TKEYS > len && lane == 0) mbar_arrive(v_last);
+                }
+                __syncwarp();
+                if (lane == 0) done(k);
+            }
+            // every load lands before the CTA may end
+            if (lane == 0) {
+                for (int i = max(0, n - C::STAGES); i < n; i++)
+                    wait_bar(kv_full + i % C::STAGES, (i / C::STAGES) & 1, nullptr, DEVERR_PTILE_DRAIN);
+                if (nq0) wait_bar(q_full, (nq0 - 1) & 1, nullptr, DEVERR_PTILE_DRAIN);
+                if (nq1) wait_bar(q_full + 1, (nq1 - 1) & 1, nullptr, DEVERR_PTILE_DRAIN);
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            // ------------------------------------------------ MMA issuer
+            constexpr uint32_t ty = std::is_same<T, __half>::value ? 0u : 1u;
+            constexpr uint32_t idesc_s = (1u << 4) | (ty << 7) | (ty << 10) | (static_cast<uint32_t>(TKEYS >> 3) << 17) |
+                                         (static_cast<uint32_t>(TM >> 4) << 24);
+            constexpr uint32_t idesc_o = (1u << 4) | (ty << 7) | (ty << 10) | (1u << 16) |
+                                         (static_cast<uint32_t>(DP >> 3) << 17) | (static_cast<uint32_t>(TM >> 4) << 24);
+            const int ksteps = (a.c.dim + 15) / 16;
+            if (lane == 0) {
+                // the ring holds K_a, V_a, K_a+1, ...: step j uses V_{j-1} (stage sv) and K_j (stage sk)
+                int sk = 0, pk = 0, nq = 0, np = 0, nfix = 0;  // nq, np: a bit for each row tile's parity
+                for (int k = 0; take(k); k++) {
+                    const Work& w = works[k & 3];
+                    const int first = w.a, end = w.b, len = w.len;
+                    const int lo[2] = {w.lo[0], w.lo[1]}, hi[2] = {w.hi[0], w.hi[1]};
+                    int sv = 0, pv = 0;
+                    for (int j = first; ok && j <= end; j++) {
+                        const uint32_t ka = smem_u32(sm) + C::OFF_RING + sk * C::STAGE;
+                        const uint32_t va = smem_u32(sm) + C::OFF_RING + sv * C::STAGE;
+                        if (j > first) {
+                            ok = wait_bar(kv_full + sv, pv, err, DEVERR_PTILE_KV);
+                            if (ok && j * TKEYS > len) ok = wait_bar(v_fixed, nfix++ & 1, err, DEVERR_PTILE_FIX);
+                        }
+                        if (ok && j < end) ok = wait_bar(kv_full + sk, pk, err, DEVERR_PTILE_KV);
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            if (ok && j - 1 >= lo[t] && j - 1 < hi[t]) {
+                                ok = wait_bar(p_full + t, (np >> t) & 1, err, DEVERR_PTILE_P);
+                                np ^= 1 << t;
+                                if (!ok) break;
+                                tc_fence_after();
+#pragma unroll
+                                for (int i = 0; i < TKEYS / 16; i++)
+                                    umma_ts(tmem + C::COL_O + t * DP, tmem + C::COL_S + t * TKEYS + i * 8,
+                                            smem_desc_mn_sw128(va + i * 2048, C::HALF), idesc_o, (j - 1 > lo[t] || i > 0) ? 1u : 0u);
+                                if (j == hi[t]) umma_commit(o_full + t);
+                            }
+                            if (ok && j >= lo[t] && j < hi[t]) {
+                                if (j == lo[t]) {
+                                    ok = wait_bar(q_full + t, (nq >> t) & 1, err, DEVERR_PTILE_Q);
+                                    nq ^= 1 << t;
+                                    if (!ok) break;
+                                }
+                                const uint32_t qa = smem_u32(sm) + t * C::QT;
+                                for (int i = 0; i < ksteps; i++) {
+                                    const uint32_t off = (i >> 2) * C::HALF + (i & 3) * 32;
+                                    umma_f16(tmem + C::COL_S + t * TKEYS, smem_desc_k_sw128(qa + off),
+                                             smem_desc_k_sw128(ka + off), idesc_s, i > 0);
+                                }
+                                umma_commit(s_full + t);
+                                if (j == hi[t] - 1) umma_commit(q_empty + t);
+                            }
+                        }
+                        if (!ok) break;
+                        if (j > first) umma_commit(kv_empty + sv);
+                        if (j < end) {
+                            umma_commit(kv_empty + sk);
+                            sv = sk + 1;
+                            pv = pk;
+                            if (sv == C::STAGES) {
+                                sv = 0;
+                                pv ^= 1;
+                            }
+                            sk = sv + 1;
+                            pk = pv;
+                            if (sk == C::STAGES) {
+                                sk = 0;
+                                pk ^= 1;
+                            }
+                        }
+                    }
+                    done(k);
+                }
+                // all products are done before tensor memory is freed
+                umma_commit(drain);
+                wait_bar(drain, 0, err, DEVERR_PTILE_DRAIN);
+            }
+            __syncwarp();
+        } else if (warp == 2) {
+            // ------------------------------------------------ values behind a sequence's end
+            int n = 0, fixes = 0;  // ring entries before this unit's
+            for (int k = 0; __all_sync(0xffffffffu, take(k)); k++) {
+                const int first = works[k & 3].a, end = works[k & 3].b, len = works[k & 3].len;
+                if (end * TKEYS > len) {  // the last key tile has some
+                    const int ev = n + 2 * (end - 1 - first) + 1, sv = ev % C::STAGES;
+                    // (issued: the stage's barrier is in this phase, or past it; before, its parity would say nothing)
+                    ok = wait_bar(v_last, fixes++ & 1, err, DEVERR_PTILE_FIX);
+                    ok = __all_sync(0xffffffffu, ok && wait_bar(kv_full + sv, (ev / C::STAGES) & 1, err, DEVERR_PTILE_FIX));
+                    const int from = max(0, len - (end - 1) * TKEYS);
+                    uint8_t* v = sm + C::OFF_RING + sv * C::STAGE;
+                    if (ok)
+                        for (int i = from * 8 + lane; i < TKEYS * 8; i += 32)
+#pragma unroll
+                            for (int h = 0; h < C::HALVES; h++)
+                                *reinterpret_cast<uint4*>(v + h * C::HALF + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(v_fixed);
+                }
+                n += 2 * (end - first);
+                __syncwarp();
+                if (lane == 0) done(k);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ------------------------------------------------ softmax
+        const int t = (warp >> 2) - 1, wl = warp & 3;
+        const int row = wl * 32 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(wl * 32) << 16);
+        const uint32_t s_addr = lanes + C::COL_S + t * TKEYS, o_addr = lanes + C::COL_O + t * DP;
+        const float scale2 = plan.scale2;
+        const int ri = row / group, gi = row - ri * group;  // this row's token of the tile, its head of the group
+        int ns = 0, no = 0;
+        for (int k = 0; __all_sync(0xffffffffu, take(k)); k++) {
+            const Work& w = works[k & 3];
+            const int lo = w.lo[t], hi = w.hi[t];
+            const bool valid = ri < w.cnt[t];
+            // of the tile's rows: keys up to pmin are seen by all, keys up to pmax - window by none
+            const int pmin = w.len - w.n + w.i0[t], pmax = pmin + w.cnt[t] - 1;
+            const int pos = valid ? pmin + ri : -1;
+            float m = -INFINITY, l = 0.0f;  // m of the raw products
+            for (int j = lo; j < hi; j++) {
+                if (ok) ok = __all_sync(0xffffffffu, wait_bar(s_full + t, ns & 1, err, DEVERR_PTILE_S));
+                ns++;
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld32(s_addr + c * 32, s[c]);
+                tmem_ld_wait();
+                if (plan.negative) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int e = 0; e < 32; e++) s[c][e] ^= 0x80000000u;
+                }
+                const int k0 = j * TKEYS;
+                if (k0 + TKEYS - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window)) {
+                    const int top = pos - k0, bot = a.window > 0 ? top - a.window : -1;  // columns in (bot, top]
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (c * 32 + e > top || c * 32 + e <= bot) s[c][e] = 0xFF800000u;  // -inf
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int e = 0; e < 32; e++) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
+                const float tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // l == 0 and O == 0 as long as m is -inf: nothing to scale then
+                const bool grow = m != -INFINITY && (tile - m) * scale2 > 8.0f;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? ex2((m - tile) * scale2) : 1.0f;
+                    if (j > lo) {
+#pragma unroll
+                        for (int c = 0; c < DP / 16; c++) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + c * 16, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(o_addr + c * 16, o);
+                        }
+                    }
+                    l *= f;
+                    if (grow) m = tile;
+                }
+                if (m == -INFINITY) m = tile;
+                const float base = m == -INFINITY ? 0.0f : m * scale2;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
+                // rounding of the result; l sums them unrounded
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float x = ex2(fmaf(__uint_as_float(s[c][2 * e]), scale2, -base));
+                        const float y = ex2(fmaf(__uint_as_float(s[c][2 * e + 1]), scale2, -base));
+                        sum[e & 3] += x + y;
+                        p[e] = pack2<T>(x, y);
+                    }
+                    tmem_st16(s_addr + c * 16, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + t);
+            }
+            // ---- the tile's end
+            const bool whole = w.whole;
+            uint8_t* part = plan.parts + (static_cast<int64_t>(blockIdx.x) * 2 + w.begins) * C::SLOT;
+            const int64_t at = static_cast<int64_t>(w.row0 + w.i0[t] + ri) * a.q_heads + w.hk * group + gi;
+            if (lo < hi) {
+                if (ok) ok = __all_sync(0xffffffffu, wait_bar(o_full + t, no & 1, err, DEVERR_PTILE_O));
+                no++;
+                tc_fence_after();
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    tmem_ld32(o_addr + c * 32, o);
+                    tmem_ld_wait();
+                    if (!valid) continue;
+                    if (whole) {
+                        T* out = static_cast<T*>(a.out) + at * a.c.dim + c * 32;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (c * 32 + e * 8 >= a.c.dim) continue;
+                            uint4 v;
+                            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                x[i] = pack2<T>(__uint_as_float(o[e * 8 + 2 * i]) * inv, __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
+                            *reinterpret_cast<uint4*>(out + e * 8) = v;
+                        }
+                    } else {
+                        uint4* out = reinterpret_cast<uint4*>(part + ((t * TM + row) * DP + c * 32) * 4);
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            out[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                }
+                tc_fence_before();
+            }
+            if (valid && whole && a.lse)
+                a.lse[at] = l == 0.0f ? -INFINITY : (m * scale2 + log2f(l)) * 0.6931471805599453f;
+            if (valid && !whole)  // (a row tile without keys in the piece: m -inf)
+                *reinterpret_cast<float2*>(part + 2 * TM * DP * 4 + (t * TM + row) * 8) =
+                    make_float2(l == 0.0f ? -INFINITY : m * scale2, l);
+            __syncwarp();
+            if (lane == 0) done(k);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 2) tmem_dealloc(tmem, C::COLS);
+}
+
+// The rows of units that lie in several pieces, a warp each: as attn_join_kernel.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) attn_tile_join_kernel(const PagedAttnArgs a, const TilePlan plan) {
+    using C = TileCfg<DP>;
+    constexpr int E = DP / 32;
+    griddep_wait();
+    const int4 b = plan.begun[blockIdx.x];
+    if (b.x < 0) return;
+    const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int group = a.q_heads / a.c.kv_heads;
+    const Seq q = load_seq(a.c, b.x);
+    const int t = row >> 7, r = row & 127, i = r / group, gi = r - i * group;
+    const int tok = (2 * b.z + t) * plan.tokens + i;
+    if (i >= plan.tokens || tok >= q.n) return;
+    float m = -INFINITY, sum = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+#pragma unroll 4
+    for (int c = blockIdx.x; c <= b.w; c++) {
+        const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == static_cast<int>(blockIdx.x) ? 1 : 0)) * C::SLOT;
+        const float2 ml = *reinterpret_cast<const float2*>(part + 2 * TM * DP * 4 + row * 8);
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = reinterpret_cast<const float*>(part)[row * DP + e * 32 + lane];
+        const float m2 = fmaxf(m, ml.x), base = m2 == -INFINITY ? 0.0f : m2;
+        const float f = ex2(m - base), w = ex2(ml.x - base);
+        m = m2;
+        sum = sum * f + ml.y * w;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = ml.x == -INFINITY ? o[e] : o[e] * f + x[e] * w;  // (x is not written then)
+    }
+    const int64_t at = static_cast<int64_t>(q.row0 + tok) * a.q_heads + b.y * group + gi;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + at * a.c.dim;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (e * 32 + lane < a.c.dim) out[e * 32 + lane] = from_f32<T>(o[e] * inv);
+    if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
 }
 
 }  // namespace
@@ -735,13 +1353,25 @@ RowsSpace rows_space(const PagedAttnArgs& a, int sms) {
     return w;
 }
 
+// Workspace of the tile kernel, behind it: the pieces' units, two parts per piece.
+struct TileSpace {
+    int64_t begun = 0, bytes = 0;
+};
+TileSpace tile_space(const PagedAttnArgs& a, int sms) {
+    TileSpace w;
+    if (static_cast<int64_t>(a.max_q) * (a.q_heads / a.c.kv_heads) <= MAX_ROWS) return w;
+    w.begun = up256(16ll * sms);
+    w.bytes = w.begun + 2ll * sms * (a.c.dim > 64 ? TileCfg<128>::SLOT : TileCfg<64>::SLOT);
+    return w;
+}
+
 }  // namespace
 
 int paged_attention_workspace(const PagedAttnArgs& a, int64_t* bytes) {
     int rc = 0;
     DeviceState* ds = device_state(&rc);
     if (!ds) return rc;
-    *bytes = rows_space(a, ds->sm_count).bytes;
+    *bytes = rows_space(a, ds->sm_count).bytes + tile_space(a, ds->sm_count).bytes;
     return TVQ_OK;
 }
 
@@ -794,15 +1424,50 @@ int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     return launch_pdl(attn_join_kernel<T, DP, 1>, dim3(static_cast<unsigned>(ctas)), dim3(JW * 32), 0, st, a, plan);
 }
 
+template <typename T, int DP>
+int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
+    using C = TileCfg<DP>;
+    static const cudaError_t attr =
+        cudaFuncSetAttribute(attn_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    TVQ_CUDA(attr);
+    const int group = a.q_heads / a.c.kv_heads;
+    uint8_t* ws = static_cast<uint8_t*>(a.ws) + rows_space(a, ds->sm_count).bytes;
+    TilePlan plan;
+    plan.begun = reinterpret_cast<int4*>(ws);
+    plan.parts = ws + tile_space(a, ds->sm_count).begun;
+    plan.tokens = TM / group;
+    plan.box = std::min(a.c.page, TKEYS);
+    plan.by_value = a.c.dim % 64 != 0;
+    plan.box_halves = a.c.dim == 128 && plan.box == TKEYS ? 2 : 1;
+    plan.negative = a.scale < 0.0f;
+    plan.scale2 = std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // (0 x -inf would be NaN)
+    CUtensorMap tmQ, tmK, tmV;
+    const bool whole = a.c.dim % 64 == 0;
+    const uint64_t dims[4] = {static_cast<uint64_t>(whole ? 64 : a.c.dim), static_cast<uint64_t>(whole ? a.c.dim / 64 : 1),
+                              static_cast<uint64_t>(a.q_heads), static_cast<uint64_t>(a.c.n_rows)};
+    const uint64_t strides[3] = {128, static_cast<uint64_t>(a.q_head) * 2, static_cast<uint64_t>(a.q_tok) * 2};
+    const uint32_t box[4] = {64, 1, static_cast<uint32_t>(group), static_cast<uint32_t>(plan.tokens)};
+    int rc = make_tma_16bit(&tmQ, a.q, 4, dims, strides, box);
+    if (rc) return rc;
+    rc = cache_map(&tmK, a.c, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
+    if (rc) return rc;
+    rc = cache_map(&tmV, a.c, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
+    if (rc) return rc;
+    rc = launch_pdl(attn_tile_kernel<T, DP>, dim3(ds->sm_count), dim3(TTHR), C::SMEM, st, tmQ, tmK, tmV, a, plan,
+                    ds->d_error);
+    if (rc) return rc;
+    return launch_pdl(attn_tile_join_kernel<T, DP>, dim3(ds->sm_count, 2 * TM / 8), dim3(256), 0, st, a, plan);
+}
+
+// Each kernel takes the sequences of its side of 16 rows, told apart on the
+// device; max_q rules the tile kernel out for steps of few rows.
 template <typename T>
 int launch_attention(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     const int group = a.q_heads / a.c.kv_heads;
     int rc = TVQ_OK;
     if (group <= MAX_ROWS) rc = a.c.dim > 64 ? launch_rows<T, 128>(a, ds, st) : launch_rows<T, 64>(a, ds, st);
     if (rc || static_cast<int64_t>(a.max_q) * group <= MAX_ROWS) return rc;
-    const int64_t units = static_cast<int64_t>(a.c.n_rows) * a.q_heads;
-    return launch_pdl(paged_attention_row_kernel<T>, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(128), 0, st, a,
-                      MAX_ROWS / group, ds->d_error);
+    return a.c.dim > 64 ? launch_tiles<T, 128>(a, ds, st) : launch_tiles<T, 64>(a, ds, st);
 }
 
 }  // namespace
@@ -811,6 +1476,7 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     int rc = 0;
     DeviceState* ds = device_state(&rc);
     if (!ds) return rc;
+    TVQ_CHECK(a.q_heads / a.c.kv_heads <= TM, TVQ_ERR_UNSUPPORTED, "more than 128 query heads to a kv head");
     TVQ_CHECK(ds->cc_major == 10, TVQ_ERR_UNSUPPORTED, "the paged attention needs an sm_100 device");
     if (a.c.n_rows == 0 || a.max_q == 0) return TVQ_OK;
     return a.c.type == TVQ_TYPE_F16 ? launch_attention<__half>(a, ds, st) : launch_attention<__nv_bfloat16>(a, ds, st);
