@@ -463,8 +463,8 @@ TVQ_API int tvq_dev_paged_attention(int type, const void* q, const int64_t* q_st
  * -inf); out: the `keep` best totals of a request's lists, descending, ties to
  * the lower beam, then to the place in its list.  finished (or NULL) [batch *
  * beams] bytes: a finished beam has the one continuation eos at no cost (its
- * row counts as 0 at eos, -inf elsewhere).  keep <= 64, keep <= vocab, beams
- * <= 64.  parents: the row batch * beams is numbered within its request (0 ..
+ * row counts as 0 at eos, -inf elsewhere).  keep <= 64, keep <= vocab <= 2^20,
+ * beams <= 64, batch * beams <= 65535.  parents: the row batch * beams is numbered within its request (0 ..
  * beams - 1).  ws as for attention, tvq_beam_select_workspace bytes. */
 TVQ_API int tvq_beam_select_workspace(int64_t batch, int64_t beams, int64_t keep, int64_t vocab, int64_t* bytes);
 TVQ_API int tvq_dev_beam_select(int type, const void* logits, int64_t stride, const float* scores,

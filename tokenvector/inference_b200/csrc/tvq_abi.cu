@@ -1556,8 +1556,8 @@ int select_args(tvq::BeamSelectArgs& a, int64_t batch, int64_t beams, int64_t ke
     TVQ_CHECK(beams >= 1 && beams <= 64 && keep >= 1 && keep <= 64, TVQ_ERR_UNSUPPORTED,
               "beams and keep must be in [1, 64]");
     TVQ_CHECK(keep <= vocab, TVQ_ERR_SIZE, "keep larger than the vocabulary");
-    TVQ_CHECK(vocab < (1ll << 31) - 65536 && batch < (1ll << 24), TVQ_ERR_UNSUPPORTED,
-              "vocabulary or batch too large");
+    TVQ_CHECK(vocab <= (1 << 20) && batch * beams <= 65535, TVQ_ERR_UNSUPPORTED,
+              "vocabulary beyond 2^20 or more than 65535 rows");
     a.batch = static_cast<int>(batch);
     a.beams = static_cast<int>(beams);
     a.keep = static_cast<int>(keep);

@@ -32,90 +32,196 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_token(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
 
-// The logit as the selection sees it: NaN is a masked token; a finished beam
-// has only its end token.
-template <typename T>
-__device__ __forceinline__ float seen_logit(const T* row, int v, bool done, int eos) {
-    if (done) return v == eos ? 0.0f : -INFINITY;
-    const float x = to_f32(row[v]);
-    return x != x ? -INFINITY : x;
-}
-
-template <typename U>
-__device__ U block_max(U x, U* sm) {
-    for (int w = 16; w > 0; w >>= 1) {
-        const U y = __shfl_xor_sync(0xffffffffu, x, w);
-        x = x > y ? x : y;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = sm[0];
-    for (int i = 1; i < static_cast<int>(blockDim.x >> 5); i++) x = sm[i] > x ? sm[i] : x;
-    return x;
-}
-
-// The plain kernel of one row: its maximum, ln sum exp(x - max), then its
-// `keep` best one after another, each the largest key below the one before.
-template <typename T>
-__global__ void __launch_bounds__(256) select_row_kernel(const BeamSelectArgs a, uint64_t* keys, float2* stats) {
-    __shared__ uint64_t sm_k[8];
-    __shared__ float sm_f[8];
+// One slice of one row: its maximum m, sum exp(x - m), and its `keep` best
+// keys, best first.  Bound: memory, each logit is read once.  A thread keeps
+// its EPT logits in registers.  The keep-th largest of the threads' best keys
+// is a key that at least `keep` logits reach, and at most keep EPT (only the
+// `keep` threads at or above it hold any), so one pass collects all that can
+// count, whatever the values, and the collected are ranked by counting.
+// Slices of 8192 logits, or of 2048 while a step has too few rows to fill the
+// GPU with the larger ones.
+constexpr int ST = 256;
+template <typename T, int EPT>
+__global__ void __launch_bounds__(ST) select_slice_kernel(const BeamSelectArgs a, uint64_t* keys, float2* stats, int slices) {
+    constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC;
+    extern __shared__ __align__(16) uint64_t found[];  // [keep * EPT]
+    __shared__ __align__(16) uint64_t best[ST];
+    __shared__ uint64_t s_bar;
+    __shared__ float s_max, s_sum[ST / 32];
+    __shared__ int s_n;
     griddep_wait();
-    const int r = blockIdx.x;
+    const int r = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const T* row = static_cast<const T*>(a.logits) + r * a.stride;
+    // slices start at 16-byte boundaries; tokens outside the row carry numbers that
+    // rank (as unsigned) behind every token of it
+    const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int v0 = slice * (ST * EPT) - mis + tid * VEC;
     const bool done = a.finished && a.finished[r];
-    float m = -INFINITY;
-    for (int v = threadIdx.x; v < a.vocab; v += 256) m = fmaxf(m, seen_logit(row, v, done, a.eos));
-    m = block_max(m, sm_f);
-    float sum = 0.0f;
-    for (int v = threadIdx.x; v < a.vocab; v += 256) sum += expf(seen_logit(row, v, done, a.eos) - m);
-    for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm_f[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float t = 0.0f;
-        for (int i = 0; i < 8; i++) t += sm_f[i];
-        stats[r] = make_float2(m, logf(t));
-    }
-    uint64_t below = ~0ull;
-    for (int k = 0; k < a.keep; k++) {
-        uint64_t best = 0;
-        for (int v = threadIdx.x; v < a.vocab; v += 256) {
-            const uint64_t key = order_key(seen_logit(row, v, done, a.eos), v);
-            if (key < below && key > best) best = key;
+    if (tid == 0) s_n = 0;
+    float x[EPT];
+#pragma unroll
+    for (int c = 0; c < NV; c++) {
+        const int v = v0 + c * ST * VEC;
+        if (done) {  // its row counts as 0 at eos, -inf elsewhere
+#pragma unroll
+            for (int e = 0; e < VEC; e++) x[c * VEC + e] = v + e == a.eos ? 0.0f : -INFINITY;
+        } else if (v >= 0 && v + VEC <= a.vocab) {
+            union { T t[VEC]; uint4 u; } w;
+            w.u = __ldcs(reinterpret_cast<const uint4*>(row + v));
+#pragma unroll
+            for (int e = 0; e < VEC; e++) x[c * VEC + e] = to_f32(w.t[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                x[c * VEC + e] = v + e >= 0 && v + e < a.vocab ? to_f32(row[v + e]) : -INFINITY;
         }
-        below = block_max(best, sm_k);
-        if (threadIdx.x == 0) keys[static_cast<int64_t>(r) * a.keep + k] = below;
+    }
+    float bx = -INFINITY;
+    int bv = v0;
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+        const int v = v0 + i / VEC * ST * VEC + i % VEC;
+        x[i] = x[i] != x[i] ? -INFINITY : x[i];
+        // (a thread's first slot may lie before the row, where a later -inf of the row goes before it)
+        if (x[i] > bx || (x[i] == bx && bv < 0)) {
+            bx = x[i];
+            bv = v;
+        }
+    }
+    const uint64_t mine = order_key(bx, bv);
+    best[tid] = mine;
+    __syncthreads();
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < ST; i += 2) {
+        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(best + i);
+        above += (w.x > mine) + (w.y > mine);
+    }
+    if (above == 0) s_max = bx;
+    if (above == a.keep - 1) s_bar = mine;
+    __syncthreads();
+    const float m = s_max, bar_x = key_value(s_bar);
+    const uint32_t bar_v = key_token(s_bar);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+        const uint32_t v = v0 + i / VEC * ST * VEC + i % VEC;
+        sum += exp2f((x[i] - m) * 1.4426950408889634f);  // (the difference first: the maximum's term is 1)
+        if (x[i] > bar_x || (x[i] == bar_x && v <= bar_v)) found[atomicAdd(&s_n, 1)] = order_key(x[i], v);
+    }
+    if (m == -INFINITY) sum = 0.0f;
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
+    __syncthreads();
+    const int64_t at = static_cast<int64_t>(r) * slices + slice;
+    if (tid == 0) {
+        float t = 0.0f;
+        for (int i = 0; i < ST / 32; i++) t += s_sum[i];
+        stats[at] = make_float2(m, t);
+    }
+    const int n = s_n;
+    for (int i = tid; i < n; i += ST) {
+        const uint64_t key = found[i];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += found[j] > key;
+        if (rank < a.keep) keys[at * a.keep + rank] = key;
     }
 }
 
-// One request: the totals of its beams' lists, and the `keep` best of them.
-__global__ void __launch_bounds__(256) select_merge_kernel(const BeamSelectArgs a, const uint64_t* keys,
-                                                           const float2* stats) {
-    __shared__ uint64_t sm_k[8];
+// A candidate's place in its request's order: total, then the lower beam, then
+// its place in the beam's list.
+struct Place {
+    uint64_t hi, lo;
+    __device__ bool above(const Place& o) const { return hi > o.hi || (hi == o.hi && lo > o.lo); }
+};
+
+// One request: the `keep` best of its beams' slices' lists.  (A candidate that
+// is not among its beam's `keep` best has that many above it in any case.)
+// The same bar: the keep-th largest of the lists' heads, found among the
+// threads' best heads first, leaves candidates of at most `keep` lists.
+// Bound: latency; a few rounds through L2.
+__global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a, const uint64_t* keys,
+                                                          const float2* stats, int slices, int heads_cap) {
+    extern __shared__ __align__(16) uint8_t sm[];
+    Place* best = reinterpret_cast<Place*>(sm);  // [ST]
+    Place* heads = best + ST;                    // [heads_cap]
+    Place* found = heads + heads_cap;            // [min(lists, keep) keep]
+    __shared__ float s_score[64], s_max[64], s_z[64];
+    __shared__ Place s_bar;
+    __shared__ int s_n[2];
+    const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_wait();
-    const int b = blockIdx.x, n = a.beams * a.keep;
-    uint64_t below = ~0ull;
-    for (int k = 0; k < a.keep; k++) {
-        uint64_t best = 0;
-        for (int c = threadIdx.x; c < n; c += 256) {
-            const int r = b * a.beams + c / a.keep;
-            const float2 st = stats[r];
-            const float x = key_value(keys[static_cast<int64_t>(b) * n + c]);
-            float total = a.scores[r] + ((x - st.x) - st.y);
-            if (total != total) total = -INFINITY;
-            const uint64_t key = order_key(total, c);
-            if (key < below && key > best) best = key;
+    for (int w = warp; w < a.beams; w += ST / 32) {
+        const float2* st = stats + (static_cast<int64_t>(b) * a.beams + w) * slices;
+        float m = -INFINITY, sum = 0.0f;
+        for (int i = lane; i < slices; i += 32) m = fmaxf(m, st[i].x);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int i = lane; i < slices; i += 32) sum += st[i].y * expf(st[i].x - m);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+            s_score[w] = a.scores[b * a.beams + w];
+            s_max[w] = m;
+            s_z[w] = logf(sum);
         }
-        below = block_max(best, sm_k);
-        if (threadIdx.x == 0) {
-            const int c = static_cast<int>(key_token(below)), o = b * a.keep + k;
-            a.out_scores[o] = key_value(below);
-            a.out_tokens[o] = key_token(keys[static_cast<int64_t>(b) * n + c]);
-            a.out_parents[o] = c / a.keep;
+    }
+    if (tid < 2) s_n[tid] = 0;
+    __syncthreads();
+    const int lists = a.beams * slices;
+    const uint64_t* mine = keys + static_cast<int64_t>(b) * lists * a.keep;
+    auto place = [&](int list, int i) {
+        const int w = list / slices;
+        Place p;
+        p.lo = mine[static_cast<int64_t>(list) * a.keep + i];
+        float total = s_score[w] + ((key_value(p.lo) - s_max[w]) - s_z[w]);
+        if (total != total) total = -INFINITY;
+        p.hi = order_key(total, w);
+        return p;
+    };
+    auto rank_of = [](const Place* all, int n, const Place& p) {
+        int rank = 0;
+        for (int i = 0; i < n; i++) rank += all[i].above(p);
+        return rank;
+    };
+    Place top{0, 0};
+    for (int l = tid; l < lists; l += ST) {
+        const Place p = place(l, 0);
+        if (p.above(top)) top = p;
+    }
+    best[tid] = top;
+    if (tid == 0) s_bar = Place{0, 0};
+    __syncthreads();
+    const int threads = min(lists, ST);
+    if (tid < threads && rank_of(best, threads, top) == a.keep - 1) s_bar = top;
+    __syncthreads();
+    if (lists > ST) {  // the bar among all heads that reach the one among the threads'
+        Place bar = s_bar;
+        for (int l = tid; l < lists; l += ST) {
+            const Place p = place(l, 0);
+            if (!bar.above(p)) heads[atomicAdd(&s_n[1], 1)] = p;
         }
+        __syncthreads();
+        const int n = s_n[1];
+        for (int i = tid; i < n; i += ST)
+            if (rank_of(heads, n, heads[i]) == a.keep - 1) s_bar = heads[i];
+        __syncthreads();
+    }
+    const Place bar = s_bar;
+    for (int64_t c = tid; c < static_cast<int64_t>(lists) * a.keep; c += ST) {
+        const int l = static_cast<int>(c / a.keep);
+        const Place p = place(l, static_cast<int>(c - static_cast<int64_t>(l) * a.keep));
+        if (!bar.above(p)) found[atomicAdd(&s_n[0], 1)] = p;
+    }
+    __syncthreads();
+    const int n = s_n[0];
+    for (int i = tid; i < n; i += ST) {
+        const Place p = found[i];
+        const int rank = rank_of(found, n, p);
+        if (rank >= a.keep) continue;
+        const int o = b * a.keep + rank;
+        a.out_scores[o] = key_value(p.hi);
+        a.out_tokens[o] = key_token(p.lo);
+        a.out_parents[o] = key_token(p.hi);
     }
 }
 
@@ -255,23 +361,63 @@ int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
 }  // namespace
 
-int beam_select_workspace(const BeamSelectArgs& a, int64_t* bytes) {
+namespace {
+
+// Slices of a step's rows: 8192 logits each, 2048 while that leaves some of
+// the 148 SMs without one.
+constexpr int kSms = 148;
+struct Slices {
+    int ept, n, heads_cap, found_cap;
+    int64_t keys, bytes;  // of the workspace: the lists', all
+};
+Slices slices_of(const BeamSelectArgs& a) {
+    Slices s;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.beams;
-    *bytes = up256(rows * a.keep * 8) + up256(rows * 8);
+    // (a row may start up to 15 bytes behind a 16-byte boundary: 7 logits of 2 bytes)
+    auto count = [&](int ept) { return (a.vocab + 7 + ST * ept - 1) / (ST * ept); };
+    s.ept = rows * count(32) < kSms ? 8 : 32;
+    s.n = count(s.ept);
+    const int lists = a.beams * s.n;
+    s.heads_cap = lists > ST ? std::min(lists, a.keep * ((lists + ST - 1) / ST)) : 0;
+    s.found_cap = std::min(lists, a.keep) * a.keep;
+    s.keys = up256(rows * s.n * a.keep * 8);
+    s.bytes = s.keys + up256(rows * s.n * 8);
+    return s;
+}
+
+template <typename T, int EPT>
+int launch_slices(const BeamSelectArgs& a, const Slices& s, uint64_t* keys, float2* stats, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(s.n), static_cast<unsigned>(a.batch * a.beams));
+    return launch_pdl(select_slice_kernel<T, EPT>, grid, dim3(ST), static_cast<size_t>(a.keep) * EPT * 8, st, a, keys,
+                      stats, s.n);
+}
+
+template <typename T>
+int launch_select(const BeamSelectArgs& a, const Slices& s, cudaStream_t st) {
+    uint64_t* keys = static_cast<uint64_t*>(a.ws);
+    float2* stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.ws) + s.keys);
+    const int rc = s.ept == 8 ? launch_slices<T, 8>(a, s, keys, stats, st) : launch_slices<T, 32>(a, s, keys, stats, st);
+    if (rc) return rc;
+    const size_t smem = (ST + s.heads_cap + s.found_cap) * sizeof(Place);
+    static const cudaError_t attr =
+        cudaFuncSetAttribute(select_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    TVQ_CUDA(attr);
+    return launch_pdl(select_merge_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(ST), smem, st, a, keys, stats, s.n,
+                      s.heads_cap);
+}
+
+}  // namespace
+
+int beam_select_workspace(const BeamSelectArgs& a, int64_t* bytes) {
+    *bytes = slices_of(a).bytes;
     return TVQ_OK;
 }
 
 int launch_beam_select(const BeamSelectArgs& a, cudaStream_t st) {
-    const int64_t rows = static_cast<int64_t>(a.batch) * a.beams;
-    uint64_t* keys = static_cast<uint64_t*>(a.ws);
-    float2* stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.ws) + up256(rows * a.keep * 8));
-    int rc;
-    const dim3 grid(static_cast<unsigned>(rows));
-    if (a.type == TVQ_TYPE_F32) rc = launch_pdl(select_row_kernel<float>, grid, dim3(256), 0, st, a, keys, stats);
-    else if (a.type == TVQ_TYPE_F16) rc = launch_pdl(select_row_kernel<__half>, grid, dim3(256), 0, st, a, keys, stats);
-    else rc = launch_pdl(select_row_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a, keys, stats);
-    if (rc) return rc;
-    return launch_pdl(select_merge_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(256), 0, st, a, keys, stats);
+    const Slices s = slices_of(a);
+    if (a.type == TVQ_TYPE_F32) return launch_select<float>(a, s, st);
+    if (a.type == TVQ_TYPE_F16) return launch_select<__half>(a, s, st);
+    return launch_select<__nv_bfloat16>(a, s, st);
 }
 
 int beam_reorder_workspace(const BeamReorderArgs& a, int64_t* bytes) {
