@@ -17,6 +17,12 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
+__device__ __forceinline__ float ex2(float x) {  // 2^x, relative error ~2^-22, 2^-inf = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // ---------------------------------------------------------------- selection
 // A logit's place in its row's order as one 64-bit key: the value's bits,
 // made monotone, above; the complement of the token below, so that equal
@@ -32,40 +38,60 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_token(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
 
+// A float's bits in its order (-0 counts as 0).
+__device__ __forceinline__ uint32_t order_bits(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
 // One slice of one row: its maximum m, sum exp(x - m), and its `keep` best
-// keys, best first.  Bound: memory, each logit is read once.  A thread keeps
-// its EPT logits in registers.  The keep-th largest of the threads' best keys
-// is a key that at least `keep` logits reach, and at most keep EPT (only the
-// `keep` threads at or above it hold any), so one pass collects all that can
-// count, whatever the values, and the collected are ranked by counting.
+// keys, best first.  Bound: memory, each logit is read once (about ten instructions
+// a logit; 128 threads of 64 logits, since finding the bar is quadratic in the
+// threads: 256 of 32 took twice the time).  The keep-th largest of the threads'
+// best values is a bar that at least `keep` logits reach, and above which only
+// keep - 1 threads have any, so one pass collects all that can count and at
+// most keep EPT, unless many equal the bar; then those are taken by their
+// tokens, chunk by chunk.  The collected are ranked by counting.
 // Slices of 8192 logits, or of 2048 while a step has too few rows to fill the
 // GPU with the larger ones.
-constexpr int ST = 256;
+constexpr int SLT = 128;
 template <typename T, int EPT>
-__global__ void __launch_bounds__(ST) select_slice_kernel(const BeamSelectArgs a, uint64_t* keys, float2* stats, int slices) {
+__global__ void __launch_bounds__(SLT) select_slice_kernel(const BeamSelectArgs a, uint64_t* keys, float2* stats, int slices) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC;
     extern __shared__ __align__(16) uint64_t found[];  // [keep * EPT]
-    __shared__ __align__(16) uint64_t best[ST];
-    __shared__ uint64_t s_bar;
-    __shared__ float s_max, s_sum[ST / 32];
-    __shared__ int s_n;
+    __shared__ __align__(16) uint32_t best[SLT];
+    __shared__ uint32_t s_bar;
+    __shared__ float s_sum[SLT / 32];
+    __shared__ int s_n, s_scan[SLT / 32];
     griddep_wait();
     const int r = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const T* row = static_cast<const T*>(a.logits) + r * a.stride;
     // slices start at 16-byte boundaries; tokens outside the row carry numbers that
     // rank (as unsigned) behind every token of it
     const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    const int v0 = slice * (ST * EPT) - mis + tid * VEC;
-    const bool done = a.finished && a.finished[r];
-    if (tid == 0) s_n = 0;
-    float x[EPT];
+    const int begin = slice * (SLT * EPT) - mis, v0 = begin + tid * VEC;
+    const int64_t at = static_cast<int64_t>(r) * slices + slice;
+    uint64_t* out = keys + at * a.keep;
+    if (a.finished && a.finished[r]) {  // its row counts as 0 at eos, -inf elsewhere
+        const int first = max(begin, 0);
+        const bool has = a.eos >= first && a.eos < begin + SLT * EPT;
+        if (tid < a.keep) {
+            int v = first + tid - (has ? 1 : 0);
+            if (has && v >= a.eos) v++;
+            out[tid] = has && tid == 0 ? order_key(0.0f, a.eos) : order_key(-INFINITY, v);
+        }
+        if (tid == 0) stats[at] = has ? make_float2(0.0f, 1.0f) : make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    if (tid == 0) {
+        s_n = 0;
+        s_bar = 0xFFFFFFFFu;
+    }
+    float x[EPT], top = -INFINITY;
 #pragma unroll
     for (int c = 0; c < NV; c++) {
-        const int v = v0 + c * ST * VEC;
-        if (done) {  // its row counts as 0 at eos, -inf elsewhere
-#pragma unroll
-            for (int e = 0; e < VEC; e++) x[c * VEC + e] = v + e == a.eos ? 0.0f : -INFINITY;
-        } else if (v >= 0 && v + VEC <= a.vocab) {
+        const int v = v0 + c * SLT * VEC;
+        if (v >= 0 && v + VEC <= a.vocab) {
             union { T t[VEC]; uint4 u; } w;
             w.u = __ldcs(reinterpret_cast<const uint4*>(row + v));
 #pragma unroll
@@ -76,57 +102,99 @@ __global__ void __launch_bounds__(ST) select_slice_kernel(const BeamSelectArgs a
                 x[c * VEC + e] = v + e >= 0 && v + e < a.vocab ? to_f32(row[v + e]) : -INFINITY;
         }
     }
-    float bx = -INFINITY;
-    int bv = v0;
 #pragma unroll
     for (int i = 0; i < EPT; i++) {
-        const int v = v0 + i / VEC * ST * VEC + i % VEC;
-        x[i] = x[i] != x[i] ? -INFINITY : x[i];
-        // (a thread's first slot may lie before the row, where a later -inf of the row goes before it)
-        if (x[i] > bx || (x[i] == bx && bv < 0)) {
-            bx = x[i];
-            bv = v;
-        }
+        x[i] = fmaxf(x[i], -INFINITY);  // NaN counts as -inf
+        top = fmaxf(top, x[i]);
     }
-    const uint64_t mine = order_key(bx, bv);
+    const uint32_t mine = order_bits(top);
     best[tid] = mine;
     __syncthreads();
     int above = 0;
+    uint32_t most = 0;
 #pragma unroll 8
-    for (int i = 0; i < ST; i += 2) {
-        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(best + i);
-        above += (w.x > mine) + (w.y > mine);
+    for (int i = 0; i < SLT; i += 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(best + i);
+        above += (w.x > mine) + (w.y > mine) + (w.z > mine) + (w.w > mine);
+        most = max(max(most, max(w.x, w.y)), max(w.z, w.w));
     }
-    if (above == 0) s_max = bx;
-    if (above == a.keep - 1) s_bar = mine;
+    const uint32_t low = __reduce_min_sync(0xffffffffu, above < a.keep ? mine : 0xFFFFFFFFu);
+    if ((tid & 31) == 0) atomicMin(&s_bar, low);
     __syncthreads();
-    const float m = s_max, bar_x = key_value(s_bar);
-    const uint32_t bar_v = key_token(s_bar);
-    float sum = 0.0f;
+    const float m = key_value(static_cast<uint64_t>(most) << 32), bar = key_value(static_cast<uint64_t>(s_bar) << 32);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int cap = a.keep * EPT;
 #pragma unroll
     for (int i = 0; i < EPT; i++) {
-        const uint32_t v = v0 + i / VEC * ST * VEC + i % VEC;
-        sum += exp2f((x[i] - m) * 1.4426950408889634f);  // (the difference first: the maximum's term is 1)
-        if (x[i] > bar_x || (x[i] == bar_x && v <= bar_v)) found[atomicAdd(&s_n, 1)] = order_key(x[i], v);
+        sum[i & 3] += ex2((x[i] - base) * 1.4426950408889634f);  // (the difference first: the maximum's term is 1)
+        if (x[i] >= bar) {
+            const int n = atomicAdd(&s_n, 1);
+            if (n < cap) found[n] = order_key(x[i], v0 + i / VEC * SLT * VEC + i % VEC);
+        }
     }
-    if (m == -INFINITY) sum = 0.0f;
+    float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
+    for (int w = 16; w > 0; w >>= 1) all += __shfl_xor_sync(0xffffffffu, all, w);
+    if ((tid & 31) == 0) s_sum[tid >> 5] = all;
     __syncthreads();
-    const int64_t at = static_cast<int64_t>(r) * slices + slice;
     if (tid == 0) {
-        float t = 0.0f;
-        for (int i = 0; i < ST / 32; i++) t += s_sum[i];
-        stats[at] = make_float2(m, t);
+        all = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        stats[at] = make_float2(m, all);
     }
-    const int n = s_n;
-    for (int i = tid; i < n; i += ST) {
+    int n = s_n;
+    if (n > cap) {  // many equal the bar: those above it, then as many of them as are missing, lowest tokens first
+        __syncthreads();
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < EPT; i++)
+            if (x[i] > bar) found[atomicAdd(&s_n, 1)] = order_key(x[i], v0 + i / VEC * SLT * VEC + i % VEC);
+        __syncthreads();
+        n = s_n;
+        const int want = n + max(0, a.keep - n);
+#pragma unroll
+        for (int ch = 0; ch < NV; ch++) {
+            int cnt = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const int v = v0 + ch * SLT * VEC + e;
+                cnt += x[ch * VEC + e] == bar && v >= 0 && v < a.vocab;
+            }
+            int inc = cnt;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if ((tid & 31) >= o) inc += y;
+            }
+            __syncthreads();
+            if ((tid & 31) == 31) s_scan[tid >> 5] = inc;
+            __syncthreads();
+            int before = n + inc - cnt, total = 0;
+            for (int w = 0; w < SLT / 32; w++) {
+                if (w < (tid >> 5)) before += s_scan[w];
+                total += s_scan[w];
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const int v = v0 + ch * SLT * VEC + e;
+                if (x[ch * VEC + e] == bar && v >= 0 && v < a.vocab) {
+                    if (before < want) found[before] = order_key(bar, v);
+                    before++;
+                }
+            }
+            n = min(want, n + total);
+            if (n == want) break;
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += SLT) {
         const uint64_t key = found[i];
         int rank = 0;
         for (int j = 0; j < n; j++) rank += found[j] > key;
-        if (rank < a.keep) keys[at * a.keep + rank] = key;
+        if (rank < a.keep) out[rank] = key;
     }
+    // (a slice with fewer logits than `keep`: places behind every token's)
+    if (tid >= n && tid < a.keep) out[tid] = order_key(-INFINITY, 0x80000000u + tid);
 }
 
 // A candidate's place in its request's order: total, then the lower beam, then
@@ -141,6 +209,7 @@ struct Place {
 // The same bar: the keep-th largest of the lists' heads, found among the
 // threads' best heads first, leaves candidates of at most `keep` lists.
 // Bound: latency; a few rounds through L2.
+constexpr int ST = 256;
 __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a, const uint64_t* keys,
                                                           const float2* stats, int slices, int heads_cap) {
     extern __shared__ __align__(16) uint8_t sm[];
@@ -374,8 +443,8 @@ Slices slices_of(const BeamSelectArgs& a) {
     Slices s;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.beams;
     // (a row may start up to 15 bytes behind a 16-byte boundary: 7 logits of 2 bytes)
-    auto count = [&](int ept) { return (a.vocab + 7 + ST * ept - 1) / (ST * ept); };
-    s.ept = rows * count(32) < kSms ? 8 : 32;
+    auto count = [&](int ept) { return (a.vocab + 7 + SLT * ept - 1) / (SLT * ept); };
+    s.ept = rows * count(64) < kSms ? 16 : 64;
     s.n = count(s.ept);
     const int lists = a.beams * s.n;
     s.heads_cap = lists > ST ? std::min(lists, a.keep * ((lists + ST - 1) / ST)) : 0;
@@ -388,7 +457,7 @@ Slices slices_of(const BeamSelectArgs& a) {
 template <typename T, int EPT>
 int launch_slices(const BeamSelectArgs& a, const Slices& s, uint64_t* keys, float2* stats, cudaStream_t st) {
     const dim3 grid(static_cast<unsigned>(s.n), static_cast<unsigned>(a.batch * a.beams));
-    return launch_pdl(select_slice_kernel<T, EPT>, grid, dim3(ST), static_cast<size_t>(a.keep) * EPT * 8, st, a, keys,
+    return launch_pdl(select_slice_kernel<T, EPT>, grid, dim3(SLT), static_cast<size_t>(a.keep) * EPT * 8, st, a, keys,
                       stats, s.n);
 }
 
@@ -396,7 +465,7 @@ template <typename T>
 int launch_select(const BeamSelectArgs& a, const Slices& s, cudaStream_t st) {
     uint64_t* keys = static_cast<uint64_t*>(a.ws);
     float2* stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.ws) + s.keys);
-    const int rc = s.ept == 8 ? launch_slices<T, 8>(a, s, keys, stats, st) : launch_slices<T, 32>(a, s, keys, stats, st);
+    const int rc = s.ept == 16 ? launch_slices<T, 16>(a, s, keys, stats, st) : launch_slices<T, 64>(a, s, keys, stats, st);
     if (rc) return rc;
     const size_t smem = (ST + s.heads_cap + s.found_cap) * sizeof(Place);
     static const cudaError_t attr =
