@@ -16,6 +16,14 @@ namespace {
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error ~2^-22, 2^-inf = 0
     float y;
@@ -44,157 +52,236 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One slice of one row: its maximum m, sum exp(x - m), and its `keep` best
-// keys, best first.  Bound: memory, each logit is read once (about ten instructions
-// a logit; 128 threads of 64 logits, since finding the bar is quadratic in the
-// threads: 256 of 32 took twice the time).  The keep-th largest of the threads'
-// best values is a bar that at least `keep` logits reach, and above which only
-// keep - 1 threads have any, so one pass collects all that can count and at
-// most keep EPT, unless many equal the bar; then those are taken by their
-// tokens, chunk by chunk.  The collected are ranked by counting.
-// Slices of 8192 logits, or of 2048 while a step has too few rows to fill the
-// GPU with the larger ones.
-constexpr int SLT = 128;
-template <typename T, int EPT>
-__global__ void __launch_bounds__(SLT) select_slice_kernel(const BeamSelectArgs a, uint64_t* keys, float2* stats, int slices) {
-    constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC;
-    extern __shared__ __align__(16) uint64_t found[];  // [keep * EPT]
-    __shared__ __align__(16) uint32_t best[SLT];
-    __shared__ uint32_t s_bar;
+// Slices of the rows: each one's maximum m, sum exp(x - m), and its `keep`
+// best keys, best first.  Bound: memory, each logit is read once, as long as
+// the instructions stay below ~12 a logit; so a pass takes what one logit
+// needs and the rest is paid once a slice.  Six CTAs an SM go over the slices,
+// with a 32 KB buffer each that one bulk copy fills as soon as the slice before
+// has been looked through; between them there is always some at work.
+//   pass 1  the best value of every group of 4 threads (2 for keep > 32)
+//   bar     the keep-th largest of those 32 (64): at least `keep` logits reach it
+//   pass 2  the sum, and which logits reach the bar: hardly more than `keep`
+//           (22 of 5000 at keep 16); they are collected and ranked by counting
+// If more reach it than the list holds (many equal logits, or the best ones
+// side by side), the bar is raised to the keep-th largest value by bisection,
+// and those that equal it are taken by their tokens.
+constexpr int SLT = 128;                 // threads
+constexpr int SBUF = 32768;              // bytes of a slice
+constexpr int SMAX = SBUF / 4 - 8;       // logits of a slice, so that a thread has whole words of at most 64 in all
+constexpr int SCAP = 512;                // logits that reach the bar
+template <typename T>
+__global__ void __launch_bounds__(SLT) select_slice_kernel(const BeamSelectArgs a, uint64_t* keys, float2* stats,
+                                                           int slices, int width, int* err) {
+    constexpr int VEC = 16 / sizeof(T);
+    extern __shared__ __align__(128) uint8_t sm[];  // the slice, then found[SCAP]
+    uint64_t* found = reinterpret_cast<uint64_t*>(sm + SBUF);
+    __shared__ __align__(16) uint32_t best[64];
+    __shared__ __align__(8) uint64_t full;
     __shared__ float s_sum[SLT / 32];
     __shared__ int s_n, s_scan[SLT / 32];
+    const int tid = threadIdx.x, rows = a.batch * a.beams, items = rows * slices;
+    const int per = a.keep <= 32 ? 4 : 2;  // threads of a group
+    if (tid == 0) {
+        mbar_init(&full, 1);
+        fence_barrier_init();
+    }
+    __syncthreads();
     griddep_wait();
-    const int r = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
-    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    // slices start at 16-byte boundaries; tokens outside the row carry numbers that
-    // rank (as unsigned) behind every token of it
-    const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    const int begin = slice * (SLT * EPT) - mis, v0 = begin + tid * VEC;
-    const int64_t at = static_cast<int64_t>(r) * slices + slice;
-    uint64_t* out = keys + at * a.keep;
-    if (a.finished && a.finished[r]) {  // its row counts as 0 at eos, -inf elsewhere
-        const int first = max(begin, 0);
-        const bool has = a.eos >= first && a.eos < begin + SLT * EPT;
-        if (tid < a.keep) {
-            int v = first + tid - (has ? 1 : 0);
-            if (has && v >= a.eos) v++;
-            out[tid] = has && tid == 0 ? order_key(0.0f, a.eos) : order_key(-INFINITY, v);
-        }
-        if (tid == 0) stats[at] = has ? make_float2(0.0f, 1.0f) : make_float2(-INFINITY, 0.0f);
-        return;
-    }
-    if (tid == 0) {
-        s_n = 0;
-        s_bar = 0xFFFFFFFFu;
-    }
-    float x[EPT], top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < NV; c++) {
-        const int v = v0 + c * SLT * VEC;
-        if (v >= 0 && v + VEC <= a.vocab) {
-            union { T t[VEC]; uint4 u; } w;
-            w.u = __ldcs(reinterpret_cast<const uint4*>(row + v));
-#pragma unroll
-            for (int e = 0; e < VEC; e++) x[c * VEC + e] = to_f32(w.t[e]);
+    griddep_launch();  // the merge's CTAs get in place as the last slices run
+
+    // A slice: tokens [first, end) of row r, copied as the 16-byte words that hold them, as far as these lie
+    // within the logits (the rest of the first and last word of all is read one by one).
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(a.logits);
+    const uintptr_t hi = lo + ((rows - 1) * a.stride + a.vocab) * sizeof(T);
+    struct Slice {
+        int r, first, end;
+        uintptr_t from, word;  // address of token `first`; of the first word's start
+        bool done;
+    };
+    auto slice_of = [&](int item) {
+        Slice s;
+        s.r = item / slices;
+        s.first = (item - s.r * slices) * width;
+        s.end = min(a.vocab, s.first + width);
+        s.from = lo + (s.r * a.stride + s.first) * sizeof(T);
+        s.word = s.from & ~uintptr_t(15);
+        s.done = s.first >= s.end || (a.finished && a.finished[s.r]);
+        return s;
+    };
+    auto fetch = [&](const Slice& s) {  // by thread 0
+        if (s.done) return;
+        const uintptr_t a0 = s.word < lo ? s.word + 16 : s.word;
+        const uintptr_t past = (s.from + (s.end - s.first) * sizeof(T) + 15) & ~uintptr_t(15);
+        const uintptr_t a1 = past > hi ? past - 16 : past;
+        if (a1 > a0) {
+            mbar_arrive_expect_tx(&full, static_cast<uint32_t>(a1 - a0));
+            bulk_load(sm + (a0 - s.word), reinterpret_cast<const void*>(a0), static_cast<uint32_t>(a1 - a0), &full);
         } else {
-#pragma unroll
-            for (int e = 0; e < VEC; e++)
-                x[c * VEC + e] = v + e >= 0 && v + e < a.vocab ? to_f32(row[v + e]) : -INFINITY;
+            mbar_arrive(&full);
         }
+    };
+    uint32_t phase = 0;
+    Slice next{};
+    if (static_cast<int>(blockIdx.x) < items) {
+        next = slice_of(blockIdx.x);
+        if (tid == 0) fetch(next);
     }
-#pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        x[i] = fmaxf(x[i], -INFINITY);  // NaN counts as -inf
-        top = fmaxf(top, x[i]);
-    }
-    const uint32_t mine = order_bits(top);
-    best[tid] = mine;
-    __syncthreads();
-    int above = 0;
-    uint32_t most = 0;
-#pragma unroll 8
-    for (int i = 0; i < SLT; i += 4) {
-        const uint4 w = *reinterpret_cast<const uint4*>(best + i);
-        above += (w.x > mine) + (w.y > mine) + (w.z > mine) + (w.w > mine);
-        most = max(max(most, max(w.x, w.y)), max(w.z, w.w));
-    }
-    const uint32_t low = __reduce_min_sync(0xffffffffu, above < a.keep ? mine : 0xFFFFFFFFu);
-    if ((tid & 31) == 0) atomicMin(&s_bar, low);
-    __syncthreads();
-    const float m = key_value(static_cast<uint64_t>(most) << 32), bar = key_value(static_cast<uint64_t>(s_bar) << 32);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int cap = a.keep * EPT;
-#pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        sum[i & 3] += ex2((x[i] - base) * 1.4426950408889634f);  // (the difference first: the maximum's term is 1)
-        if (x[i] >= bar) {
-            const int n = atomicAdd(&s_n, 1);
-            if (n < cap) found[n] = order_key(x[i], v0 + i / VEC * SLT * VEC + i % VEC);
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const Slice s = next;
+        const bool more = item + static_cast<int>(gridDim.x) < items;
+        if (more) next = slice_of(item + gridDim.x);
+        uint64_t* out = keys + static_cast<int64_t>(item) * a.keep;
+        if (s.done) {  // a finished row counts as 0 at eos, -inf elsewhere
+            const bool has = a.eos >= s.first && a.eos < s.end;
+            if (tid < a.keep) {
+                int v = s.first + tid - (has ? 1 : 0);
+                if (has && v >= a.eos) v++;
+                // (a slice with fewer tokens than `keep`: places behind every token's)
+                const bool real = v < s.end;
+                out[tid] = has && tid == 0 ? order_key(0.0f, a.eos) : order_key(-INFINITY, real ? v : 0x80000000u + tid);
+            }
+            if (tid == 0) stats[item] = has ? make_float2(0.0f, 1.0f) : make_float2(-INFINITY, 0.0f);
+            if (more && tid == 0) fetch(next);
+            continue;
         }
-    }
-    float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) all += __shfl_xor_sync(0xffffffffu, all, w);
-    if ((tid & 31) == 0) s_sum[tid >> 5] = all;
-    __syncthreads();
-    if (tid == 0) {
-        all = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-        stats[at] = make_float2(m, all);
-    }
-    int n = s_n;
-    if (n > cap) {  // many equal the bar: those above it, then as many of them as are missing, lowest tokens first
-        __syncthreads();
+        const int skip = static_cast<int>((s.from - s.word) / sizeof(T));  // entry e of the buffer is token first - skip + e
+        const int count = s.end - s.first, words = (skip + count + VEC - 1) / VEC;
+        T* data = reinterpret_cast<T*>(sm);
+        if (!mbar_wait_for(&full, phase, nullptr, 0, TVQ_WAIT_LIMIT_NS)) record_error(err, DEVERR_TIMEOUT_ROWS);
+        phase ^= 1;
+        // the words that reach out of the slice: -inf there, and what the copy left out
+        if (tid < 2 * VEC) {
+            const int e = tid < VEC ? tid : (words - 1) * VEC + tid - VEC;
+            const bool in = e >= skip && e < skip + count;
+            const uintptr_t at = s.word + e / VEC * 16;
+            if (!in) data[e] = from_f32<T>(-INFINITY);
+            else if (at < lo || at + 16 > hi) data[e] = reinterpret_cast<const T*>(s.word)[e];
+            fence_proxy_async_smem();  // (before the next copy into the buffer)
+        }
         if (tid == 0) s_n = 0;
         __syncthreads();
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int w = tid; w < words; w += SLT) {
+            union { T t[VEC]; uint4 u; } x;
+            x.u = reinterpret_cast<const uint4*>(data)[w];
 #pragma unroll
-        for (int i = 0; i < EPT; i++)
-            if (x[i] > bar) found[atomicAdd(&s_n, 1)] = order_key(x[i], v0 + i / VEC * SLT * VEC + i % VEC);
-        __syncthreads();
-        n = s_n;
-        const int want = n + max(0, a.keep - n);
-#pragma unroll
-        for (int ch = 0; ch < NV; ch++) {
-            int cnt = 0;
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const int v = v0 + ch * SLT * VEC + e;
-                cnt += x[ch * VEC + e] == bar && v >= 0 && v < a.vocab;
-            }
-            int inc = cnt;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, inc, o);
-                if ((tid & 31) >= o) inc += y;
-            }
-            __syncthreads();
-            if ((tid & 31) == 31) s_scan[tid >> 5] = inc;
-            __syncthreads();
-            int before = n + inc - cnt, total = 0;
-            for (int w = 0; w < SLT / 32; w++) {
-                if (w < (tid >> 5)) before += s_scan[w];
-                total += s_scan[w];
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const int v = v0 + ch * SLT * VEC + e;
-                if (x[ch * VEC + e] == bar && v >= 0 && v < a.vocab) {
-                    if (before < want) found[before] = order_key(bar, v);
-                    before++;
-                }
-            }
-            n = min(want, n + total);
-            if (n == want) break;
+            for (int e = 0; e < VEC; e++) top = fmaxf(top, to_f32(x.t[e]));  // (NaN counts as -inf)
         }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        if (per == 4) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (tid % per == 0) best[tid / per] = order_bits(top);
         __syncthreads();
+        // every warp: a lane's place among the groups' tops, and the lowest of those that have fewer than
+        // `keep` above them
+        const int lane = tid & 31;
+        uint32_t low = 0xFFFFFFFFu, most = 0;
+        for (int g = lane; g < SLT / per; g += 32) {
+            const uint32_t mine = best[g];
+            int above = 0;
+#pragma unroll 8
+            for (int i = 0; i < SLT / per; i += 4) {
+                const uint4 w = *reinterpret_cast<const uint4*>(best + i);
+                above += (w.x > mine) + (w.y > mine) + (w.z > mine) + (w.w > mine);
+            }
+            if (above < a.keep) low = min(low, mine);
+            most = max(most, mine);
+        }
+        low = __reduce_min_sync(0xffffffffu, low);
+        most = __reduce_max_sync(0xffffffffu, most);
+        const float m = key_value(static_cast<uint64_t>(most) << 32);
+        float bar = key_value(static_cast<uint64_t>(low) << 32);
+        const float base = m == -INFINITY ? 0.0f : m;
+        const int v0 = s.first - skip;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint64_t hits = 0;  // which of the thread's logits reach the bar (collected one by one in the loop, each took ~400 cycles)
+#pragma unroll 2
+        for (int w = tid, k = 0; w < words; w += SLT, k += VEC) {
+            union { T t[VEC]; uint4 u; } x;
+            x.u = reinterpret_cast<const uint4*>(data)[w];
+            uint32_t some = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const float y = fmaxf(to_f32(x.t[e]), -INFINITY);
+                sum[e & 3] += ex2((y - base) * 1.4426950408889634f);  // (the difference first: the maximum's term is 1)
+                some |= y >= bar ? 1u << e : 0u;
+            }
+            hits |= static_cast<uint64_t>(some) << k;
+        }
+        if (bar == -INFINITY)  // (entries outside the slice are -inf there: none of its logits)
+            for (int w = tid, k = 0; w < words; w += SLT, k += VEC)
+                for (int e = 0; e < VEC; e++)
+                    if (static_cast<unsigned>(w * VEC + e - skip) >= static_cast<unsigned>(count)) hits &= ~(1ull << (k + e));
+        if (hits) {
+            for (int n = atomicAdd(&s_n, __popcll(hits)); hits && n < SCAP; hits &= hits - 1, n++) {
+                const int k = __ffsll(hits) - 1, e = (tid + k / VEC * SLT) * VEC + k % VEC;
+                found[n] = order_key(fmaxf(to_f32(data[e]), -INFINITY), v0 + e);
+            }
+        }
+        float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) all += __shfl_xor_sync(0xffffffffu, all, w);
+        if (lane == 0) s_sum[tid >> 5] = all;
+        __syncthreads();
+        if (tid == 0) stats[item] = make_float2(m, (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]));
+        int n = s_n;
+        if (n > SCAP) {
+            // the keep-th largest value: the highest that `keep` logits reach
+            auto value = [&](int e) { return fmaxf(to_f32(data[e]), -INFINITY); };
+            uint32_t below = low, least = most;  // `keep` reach `below`; the highest such is in [below, least]
+            while (below < least) {
+                const uint32_t mid = below + (least - below + 1) / 2;
+                int reach = 0;
+                for (int e = skip + tid; e < skip + count; e += SLT) reach += order_bits(value(e)) >= mid;
+                reach = __reduce_add_sync(0xffffffffu, reach);
+                __syncthreads();
+                if (lane == 0) s_scan[tid >> 5] = reach;
+                __syncthreads();
+                reach = 0;
+                for (int w = 0; w < SLT / 32; w++) reach += s_scan[w];
+                if (reach >= a.keep) below = mid;
+                else least = mid - 1;
+            }
+            bar = key_value(static_cast<uint64_t>(below) << 32);
+            // those above it, then as many that equal it as are missing, lowest tokens first
+            __syncthreads();
+            if (tid == 0) s_n = 0;
+            __syncthreads();
+            for (int e = skip + tid; e < skip + count; e += SLT) {
+                const float y = value(e);
+                if (y > bar) found[atomicAdd(&s_n, 1)] = order_key(y, v0 + e);
+            }
+            __syncthreads();
+            n = s_n;
+            const int want = max(n, a.keep);
+            for (int e0 = skip; e0 < skip + count && n < want; e0 += SLT) {
+                const int e = e0 + tid;
+                const bool same = e < skip + count && value(e) == bar;
+                const uint32_t votes = __ballot_sync(0xffffffffu, same);
+                __syncthreads();
+                if (lane == 0) s_scan[tid >> 5] = __popc(votes);
+                __syncthreads();
+                int place = n + __popc(votes & ((1u << lane) - 1)), total = 0;
+                for (int w = 0; w < SLT / 32; w++) {
+                    if (w < (tid >> 5)) place += s_scan[w];
+                    total += s_scan[w];
+                }
+                if (same && place < want) found[place] = order_key(bar, v0 + e);
+                n = min(want, n + total);
+            }
+            __syncthreads();
+        }
+        if (more && tid == 0) fetch(next);  // (nobody reads the buffer any more)
+        for (int i = tid; i < n; i += SLT) {
+            const uint64_t key = found[i];
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; j++) rank += found[j] > key;
+            if (rank < a.keep) out[rank] = key;
+        }
+        if (tid >= n && tid < a.keep) out[tid] = order_key(-INFINITY, 0x80000000u + tid);
+        __syncthreads();  // `found` and the counters are free
     }
-    for (int i = tid; i < n; i += SLT) {
-        const uint64_t key = found[i];
-        int rank = 0;
-        for (int j = 0; j < n; j++) rank += found[j] > key;
-        if (rank < a.keep) out[rank] = key;
-    }
-    // (a slice with fewer logits than `keep`: places behind every token's)
-    if (tid >= n && tid < a.keep) out[tid] = order_key(-INFINITY, 0x80000000u + tid);
 }
 
 // A candidate's place in its request's order: total, then the lower beam, then
@@ -208,11 +295,12 @@ struct Place {
 // is not among its beam's `keep` best has that many above it in any case.)
 // The same bar: the keep-th largest of the lists' heads, found among the
 // threads' best heads first, leaves candidates of at most `keep` lists.
-// Bound: latency; a few rounds through L2.
-constexpr int ST = 256;
+// Bound: latency, so what is read is asked for at once: all statistics, a
+// list's head and AHEAD candidates for each thread.
+constexpr int ST = 256, AHEAD = 4;
 __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a, const uint64_t* keys,
                                                           const float2* stats, int slices, int heads_cap) {
-    extern __shared__ __align__(16) uint8_t sm[];
+    extern __shared__ __align__(128) uint8_t sm[];
     Place* best = reinterpret_cast<Place*>(sm);  // [ST]
     Place* heads = best + ST;                    // [heads_cap]
     Place* found = heads + heads_cap;            // [min(lists, keep) keep]
@@ -220,54 +308,60 @@ __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a
     __shared__ Place s_bar;
     __shared__ int s_n[2];
     const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int lists = a.beams * slices, all = lists * a.keep;
     griddep_wait();
+    const uint64_t* mine = keys + static_cast<int64_t>(b) * all;
+    const uint64_t head = tid < lists ? mine[static_cast<int64_t>(tid) * a.keep] : 0;
+    uint64_t ahead[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) ahead[i] = tid + i * ST < all ? mine[tid + i * ST] : 0;
+    if (tid < 2) s_n[tid] = 0;
+    if (tid == 0) s_bar = Place{0, 0};
     for (int w = warp; w < a.beams; w += ST / 32) {
         const float2* st = stats + (static_cast<int64_t>(b) * a.beams + w) * slices;
-        float m = -INFINITY, sum = 0.0f;
-        for (int i = lane; i < slices; i += 32) m = fmaxf(m, st[i].x);
+        float2 one = lane < slices ? st[lane] : make_float2(-INFINITY, 0.0f);
+        const float score = a.scores[b * a.beams + w];
+        float m = one.x;
+        for (int i = lane + 32; i < slices; i += 32) m = fmaxf(m, st[i].x);
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int i = lane; i < slices; i += 32) sum += st[i].y * expf(st[i].x - m);
+        float sum = lane < slices ? one.y * expf(one.x - m) : 0.0f;
+        for (int i = lane + 32; i < slices; i += 32) sum += st[i].y * expf(st[i].x - m);
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
-            s_score[w] = a.scores[b * a.beams + w];
+            s_score[w] = score;
             s_max[w] = m;
             s_z[w] = logf(sum);
         }
     }
-    if (tid < 2) s_n[tid] = 0;
     __syncthreads();
-    const int lists = a.beams * slices;
-    const uint64_t* mine = keys + static_cast<int64_t>(b) * lists * a.keep;
-    auto place = [&](int list, int i) {
+    auto place = [&](uint64_t key, int list) {
         const int w = list / slices;
-        Place p;
-        p.lo = mine[static_cast<int64_t>(list) * a.keep + i];
-        float total = s_score[w] + ((key_value(p.lo) - s_max[w]) - s_z[w]);
+        float total = s_score[w] + ((key_value(key) - s_max[w]) - s_z[w]);
         if (total != total) total = -INFINITY;
-        p.hi = order_key(total, w);
-        return p;
+        return Place{order_key(total, w), key};
     };
-    auto rank_of = [](const Place* all, int n, const Place& p) {
+    auto rank_of = [](const Place* set, int n, const Place& p) {
         int rank = 0;
-        for (int i = 0; i < n; i++) rank += all[i].above(p);
+#pragma unroll 4
+        for (int i = 0; i < n; i++) rank += set[i].above(p);
         return rank;
     };
     Place top{0, 0};
-    for (int l = tid; l < lists; l += ST) {
-        const Place p = place(l, 0);
+    if (tid < lists) top = place(head, tid);
+    for (int l = tid + ST; l < lists; l += ST) {
+        const Place p = place(mine[static_cast<int64_t>(l) * a.keep], l);
         if (p.above(top)) top = p;
     }
     best[tid] = top;
-    if (tid == 0) s_bar = Place{0, 0};
     __syncthreads();
     const int threads = min(lists, ST);
     if (tid < threads && rank_of(best, threads, top) == a.keep - 1) s_bar = top;
     __syncthreads();
     if (lists > ST) {  // the bar among all heads that reach the one among the threads'
-        Place bar = s_bar;
+        const Place first = s_bar;
         for (int l = tid; l < lists; l += ST) {
-            const Place p = place(l, 0);
-            if (!bar.above(p)) heads[atomicAdd(&s_n[1], 1)] = p;
+            const Place p = place(mine[static_cast<int64_t>(l) * a.keep], l);
+            if (!first.above(p)) heads[atomicAdd(&s_n[1], 1)] = p;
         }
         __syncthreads();
         const int n = s_n[1];
@@ -276,11 +370,14 @@ __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a
         __syncthreads();
     }
     const Place bar = s_bar;
-    for (int64_t c = tid; c < static_cast<int64_t>(lists) * a.keep; c += ST) {
-        const int l = static_cast<int>(c / a.keep);
-        const Place p = place(l, static_cast<int>(c - static_cast<int64_t>(l) * a.keep));
+    auto collect = [&](uint64_t key, int c) {
+        const Place p = place(key, c / a.keep);
         if (!bar.above(p)) found[atomicAdd(&s_n[0], 1)] = p;
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+        if (tid + i * ST < all) collect(ahead[i], tid + i * ST);
+    for (int c = tid + AHEAD * ST; c < all; c += ST) collect(mine[c], c);
     __syncthreads();
     const int n = s_n[0];
     for (int i = tid; i < n; i += ST) {
@@ -432,20 +529,29 @@ int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
 namespace {
 
-// Slices of a step's rows: 8192 logits each, 2048 while that leaves some of
-// the 148 SMs without one.
-constexpr int kSms = 148;
+// Slices of a step's rows, for the six CTAs that go over them on each of the
+// 148 SMs: as few rounds of as narrow slices as will do, where a slice costs
+// what 3000 logits do besides its own (the two passes over its tops), and has
+// at least 2048.
+constexpr int kSms = 148, kSliceCtas = 6 * kSms, kSliceCost = 3000;
 struct Slices {
-    int ept, n, heads_cap, found_cap;
+    int n, width, heads_cap, found_cap;
     int64_t keys, bytes;  // of the workspace: the lists', all
 };
 Slices slices_of(const BeamSelectArgs& a) {
     Slices s;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.beams;
-    // (a row may start up to 15 bytes behind a 16-byte boundary: 7 logits of 2 bytes)
-    auto count = [&](int ept) { return (a.vocab + 7 + SLT * ept - 1) / (SLT * ept); };
-    s.ept = rows * count(64) < kSms ? 16 : 64;
-    s.n = count(s.ept);
+    const int least = (a.vocab + SMAX - 1) / SMAX;
+    int64_t cost = INT64_MAX;
+    s.n = least;
+    for (int n = least; n <= std::max(least, std::min(a.vocab / 2048, 3 * least + 24)); n++) {
+        const int64_t c = (rows * n + kSliceCtas - 1) / kSliceCtas * ((a.vocab + n - 1) / n + kSliceCost);
+        if (c < cost) {
+            cost = c;
+            s.n = n;
+        }
+    }
+    s.width = (a.vocab + s.n - 1) / s.n;
     const int lists = a.beams * s.n;
     s.heads_cap = lists > ST ? std::min(lists, a.keep * ((lists + ST - 1) / ST)) : 0;
     s.found_cap = std::min(lists, a.keep) * a.keep;
@@ -454,23 +560,21 @@ Slices slices_of(const BeamSelectArgs& a) {
     return s;
 }
 
-template <typename T, int EPT>
-int launch_slices(const BeamSelectArgs& a, const Slices& s, uint64_t* keys, float2* stats, cudaStream_t st) {
-    const dim3 grid(static_cast<unsigned>(s.n), static_cast<unsigned>(a.batch * a.beams));
-    return launch_pdl(select_slice_kernel<T, EPT>, grid, dim3(SLT), static_cast<size_t>(a.keep) * EPT * 8, st, a, keys,
-                      stats, s.n);
-}
-
 template <typename T>
 int launch_select(const BeamSelectArgs& a, const Slices& s, cudaStream_t st) {
+    int rc = 0;
+    DeviceState* ds = device_state(&rc);
+    if (!ds) return rc;
     uint64_t* keys = static_cast<uint64_t*>(a.ws);
     float2* stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.ws) + s.keys);
-    const int rc = s.ept == 16 ? launch_slices<T, 16>(a, s, keys, stats, st) : launch_slices<T, 64>(a, s, keys, stats, st);
+    static const cudaError_t attr2 =
+        cudaFuncSetAttribute(select_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    TVQ_CUDA(attr2);
+    const int64_t items = static_cast<int64_t>(a.batch) * a.beams * s.n;
+    rc = launch_pdl(select_slice_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(items, kSliceCtas))), dim3(SLT),
+                    static_cast<size_t>(SBUF + SCAP * 8), st, a, keys, stats, s.n, s.width, ds->d_error);
     if (rc) return rc;
     const size_t smem = (ST + s.heads_cap + s.found_cap) * sizeof(Place);
-    static const cudaError_t attr =
-        cudaFuncSetAttribute(select_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    TVQ_CUDA(attr);
     return launch_pdl(select_merge_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(ST), smem, st, a, keys, stats, s.n,
                       s.heads_cap);
 }
