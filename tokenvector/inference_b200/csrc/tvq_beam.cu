@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "tvq_common.cuh"
 #include "tvq_decode.h"
@@ -392,134 +393,229 @@ __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a
 }
 
 // ---------------------------------------------------------------- reordering
-// A copy that a row needs: page `src` -> page `dst` (or -1: none).
+// A copy that a row needs: `fill` tokens of page src to page dst.
 struct PageCopy {
     int src, dst, fill;
 };
+// What becomes of a new row: its parent's first `n` pages, and page `page` in
+// column `at` (at -1: none of its own; page -1: none to be had).
+struct RowPlan {
+    int parent, n, at, page;
+};
 
-__device__ int block_scan(int x, int* sm, int* total) {  // exclusive, 1024 threads
-    int inc = x;
+constexpr int RT = 1024;  // threads of a CTA
+// Exclusive sum over the CTA; counts in both halves of the word do not meet.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sm, uint32_t* total) {
+    uint32_t inc = x;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += y;
     }
     __syncthreads();
     if (lane == 31) sm[w] = inc;
     __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < 32; i++) {
-        if (i < w) before += sm[i];
-        all += sm[i];
+    uint32_t part = sm[lane];  // (32 warps)
+    const uint32_t own = part;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, part, o);
+        if (lane >= o) part += y;
     }
-    *total = all;
-    return before + inc - x;
+    *total = __shfl_sync(0xffffffffu, part, 31);
+    return __shfl_sync(0xffffffffu, part - own, w) + inc - x;
 }
 
-// Tables, lengths, counts and the list of copies, by one CTA.
-__global__ void __launch_bounds__(1024) reorder_tables_kernel(const BeamReorderArgs a, int* held, int* tails,
-                                                              int* freelist, PageCopy* copies, int* err) {
-    __shared__ int sm[32];
+// Every thread's writes to memory before are seen by every thread of the cluster after (through L2: read them with __ldcg).
+template <int RC>
+__device__ __forceinline__ void cluster_sync() {
+    if constexpr (RC == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Tables, lengths, counts and the list of copies.  A step's tables are a few
+// KB; what takes the time is the chain of reads that depend on one another, and
+// the atomics of one SM (one address a cycle), so a cluster of eight CTAs does
+// large ones (256 rows: 13 us, one CTA 25), and one CTA small ones, where a
+// barrier across the cluster costs more (4 rows: 6 us, the cluster 9); both in
+// four phases.  held[page]: how often
+// the old tables hold it; owner[page]: the lowest new row whose tail it is.
+template <int RC>
+__global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
+    reorder_tables_kernel(const BeamReorderArgs a, int* held, int* owner, int* freelist, RowPlan* rows, PageCopy* copies,
+                          int* n_copies, int* err) {
+    __shared__ uint32_t sm[32];
     griddep_wait();
-    const int t = threadIdx.x;
-    for (int64_t i = t; i < a.n_pages; i += 1024) {
+    griddep_launch();
+    constexpr int ALL = RC * RT;
+    const int t = threadIdx.x, g = blockIdx.x * RT + t;  // the cluster is the grid
+    const int log2 = __ffs(a.page) - 1;
+    auto used = [&](int len) { return min(a.cols, (len + a.page - 1) >> log2); };
+    // (row, column) of the entries g, g + ALL, ... of a table: one division, not one each
+    const int r_first = g / max(a.cols, 1), c_first = g - r_first * a.cols;
+    const int r_step = ALL / max(a.cols, 1), c_step = ALL - r_step * a.cols;
+    auto step = [&](int& r, int& c) {
+        r += r_step;
+        c += c_step;
+        if (c >= a.cols) {
+            c -= a.cols;
+            r++;
+        }
+    };
+
+    // ---- 1: counters; the first free pages, at most one for each new row
+    for (int64_t i = g; i < a.n_pages; i += ALL) {
         held[i] = 0;
-        a.new_refs[i] = a.refs[i];
+        owner[i] = INT_MAX;
     }
-    __syncthreads();
-    auto used = [&](int len) { return min(a.cols, (len + a.page - 1) / a.page); };
-    for (int64_t e = t; e < static_cast<int64_t>(a.rows) * a.cols; e += 1024) {
-        const int r = static_cast<int>(e / a.cols), c = static_cast<int>(e - static_cast<int64_t>(r) * a.cols);
-        const int pg = a.table[r * a.table_stride + c];
-        if (c < used(a.lens[r]) && pg >= 0 && pg < a.n_pages) {
-            atomicAdd(held + pg, 1);
-            atomicSub(a.new_refs + pg, 1);
+    int found = 0;
+    if (blockIdx.x == 0) {
+        for (int64_t i0 = 0; i0 < a.n_pages && found < a.new_rows; i0 += RT * 8) {
+            const int64_t i = i0 + t * 8;
+            uint32_t free = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (i + e < a.n_pages && __ldg(a.refs + i + e) == 0) free |= 1u << e;
+            uint32_t all;
+            int rank = found + static_cast<int>(block_scan(__popc(free), sm, &all));
+            for (; free && rank < a.new_rows; free &= free - 1, rank++) freelist[rank] = static_cast<int>(i) + __ffs(free) - 1;
+            found += static_cast<int>(all);
         }
     }
-    // a row's tail page: >= 0 part-filled, -1 none (the row ends with a page), -2 no parent
-    for (int r = t; r < a.new_rows; r += 1024) {
+    cluster_sync<RC>();
+
+    // ---- 2: what the old tables hold; the new rows' parents, and their tails' owners
+    constexpr int B = 4;  // entries whose reads are on their way together
+    for (int r = r_first, c = c_first; r < a.rows && a.cols > 0;) {
+        int pg[B], len[B], cc[B];
+#pragma unroll
+        for (int k = 0; k < B; k++, step(r, c)) {
+            const bool in = r < a.rows;
+            pg[k] = in ? __ldg(a.table + r * a.table_stride + c) : -1;
+            len[k] = in ? __ldg(a.lens + r) : 0;
+            cc[k] = c;
+        }
+#pragma unroll
+        for (int k = 0; k < B; k++)
+            if (cc[k] < used(len[k]) && pg[k] >= 0 && pg[k] < a.n_pages) atomicAdd(held + pg[k], 1);
+    }
+    for (int r = g; r < a.new_rows; r += ALL) {
         const int q = a.parents[r];
         if (q >= a.rows) record_error(err, DEVERR_BAD_INDEX);
         const bool live = q >= 0 && q < a.rows;
-        const int len = live ? a.lens[q] : 0, fill = len % a.page, at = len / a.page;
-        int tail = live ? -1 : -2;
-        if (live && fill > 0 && at < a.cols) {
+        const int len = live ? a.lens[q] : 0, at = len >> log2;
+        int tail = -1;  // the page that is part-filled, if one is
+        if (live && (len & (a.page - 1)) && at < a.cols) {
             tail = a.table[q * a.table_stride + at];
             if (tail < 0 || tail >= a.n_pages) {
                 record_error(err, DEVERR_BAD_PAGE);
                 tail = -1;
+            } else {
+                atomicMin(owner + tail, r);
             }
         }
-        tails[r] = tail;
         a.new_lens[r] = len;
+        rows[r] = RowPlan{live ? q : -1, live ? used(len) : 0, at, tail};
     }
-    __syncthreads();
-    int need = 0;
-    for (int r0 = 0; r0 < a.new_rows; r0 += 1024) {
-        const int r = r0 + t;
-        bool fresh = false;
-        if (r < a.new_rows && tails[r] > -2) {
-            bool keeps = tails[r] >= 0 && a.refs[tails[r]] == held[tails[r]];
-            for (int o = 0; keeps && o < r; o++) keeps = tails[o] != tails[r];
-            fresh = !keeps && a.new_lens[r] / a.page < a.cols;
-        }
-        int all;
-        const int rank = need + block_scan(fresh ? 1 : 0, sm, &all);
-        if (r < a.new_rows) copies[r].dst = fresh ? rank : -1;  // its turn in the free list, for now
-        need += all;
-    }
-    __syncthreads();
-    int found = 0;
-    for (int64_t i0 = 0; i0 < a.n_pages && found < need; i0 += 1024) {
-        const int64_t i = i0 + t;
-        const bool is_free = i < a.n_pages && a.refs[i] == 0;
-        int all;
-        const int rank = found + block_scan(is_free ? 1 : 0, sm, &all);
-        if (is_free && rank < need) freelist[rank] = static_cast<int>(i);
-        found += all;
-    }
-    __syncthreads();
-    int short_of = 0;
-    for (int r0 = 0; r0 < a.new_rows; r0 += 1024) {
-        const int r = r0 + t;
-        bool none = false;
-        if (r < a.new_rows) {
-            const int turn = copies[r].dst, len = a.new_lens[r], fill = len % a.page;
-            const bool keeps = fill > 0 && turn < 0 && tails[r] >= 0;
-            const int pg = turn >= 0 && turn < found ? freelist[turn] : -1;
-            none = tails[r] > -2 && !keeps && pg < 0;
-            copies[r] = PageCopy{tails[r], tails[r] >= 0 ? pg : -1, fill};
-            const int q = a.parents[r], n = tails[r] > -2 ? used(len) : 0;
-            for (int c = 0; c < a.cols; c++) {
-                int e = c < n ? a.table[q * a.table_stride + c] : -1;
-                if (c == len / a.page && tails[r] > -2 && !keeps) e = pg;
-                a.new_table[static_cast<int64_t>(r) * a.cols + c] = e;
-                if (e >= 0 && e < a.n_pages) atomicAdd(a.new_refs + e, 1);
+    cluster_sync<RC>();
+
+    // ---- 3: who keeps its tail, who takes which free page (one CTA); the counts without the old tables (the others, if any)
+    if (blockIdx.x == 0) {
+        int taken = 0, short_of = 0, copied = 0;
+        for (int r0 = 0; r0 < a.new_rows; r0 += RT) {
+            const int r = r0 + t;
+            RowPlan p{-1, 0, -1, -1};
+            bool keeps = false, part = false;
+            int fill = 0;
+            if (r < a.new_rows) {
+                const int4 w = __ldcg(reinterpret_cast<const int4*>(rows + r));
+                p = RowPlan{w.x, w.y, w.z, w.w};
+                part = p.page >= 0;
+                fill = __ldcg(a.new_lens + r) & (a.page - 1);
+                keeps = part && __ldcg(owner + p.page) == r && a.refs[p.page] == __ldcg(held + p.page);
             }
+            const bool fresh = p.parent >= 0 && !keeps && p.at < a.cols;
+            uint32_t all;
+            const int turn = taken + static_cast<int>(block_scan(fresh, sm, &all));
+            const bool got = fresh && turn < found;
+            taken += static_cast<int>(all);
+            const uint32_t mine = (got && part) | (p.parent >= 0 && !keeps && !got ? 0x10000u : 0u);
+            const uint32_t before = block_scan(mine, sm, &all);
+            const int page = got ? __ldcg(freelist + turn) : -1;
+            if (got && part) copies[copied + (before & 0xFFFFu)] = PageCopy{p.page, page, fill};
+            copied += static_cast<int>(all & 0xFFFFu);
+            short_of += static_cast<int>(all >> 16);
+            if (r < a.new_rows) rows[r] = RowPlan{p.parent, p.n, fresh ? p.at : -1, page};
         }
-        int all;
-        block_scan(none ? 1 : 0, sm, &all);
-        short_of += all;
+        if (t == 0) {
+            a.status[0] = min(taken, found);
+            a.status[1] = short_of;
+            *n_copies = copied;
+        }
     }
-    if (t == 0) {
-        a.status[0] = min(need, found);
-        a.status[1] = short_of;
+    if (RC == 1 || blockIdx.x > 0)
+        for (int64_t i = RC == 1 ? t : g - RT; i < a.n_pages; i += RC == 1 ? RT : ALL - RT)
+            a.new_refs[i] = a.refs[i] - __ldcg(held + i);
+    cluster_sync<RC>();
+
+    // ---- 4: the new tables, and what they hold
+    for (int r = r_first, c = c_first; r < a.new_rows && a.cols > 0;) {
+        int4 p[B];
+        int rr[B], cc[B], pg[B];
+#pragma unroll
+        for (int k = 0; k < B; k++, step(r, c)) {
+            rr[k] = r;
+            cc[k] = c;
+            p[k] = r < a.new_rows ? __ldcg(reinterpret_cast<const int4*>(rows + r)) : make_int4(-1, 0, -1, -1);
+        }
+#pragma unroll
+        for (int k = 0; k < B; k++)
+            pg[k] = cc[k] == p[k].z ? p[k].w : cc[k] < p[k].y ? __ldg(a.table + p[k].x * a.table_stride + cc[k]) : -1;
+#pragma unroll
+        for (int k = 0; k < B; k++)
+            if (rr[k] < a.new_rows) {
+                a.new_table[static_cast<int64_t>(rr[k]) * a.cols + cc[k]] = pg[k];
+                if (pg[k] >= 0 && pg[k] < a.n_pages) atomicAdd(a.new_refs + pg[k], 1);
+            }
     }
 }
 
 // The filled part of the pages that rows copy, every layer, keys and values.
-__global__ void __launch_bounds__(256) reorder_copy_kernel(const BeamReorderArgs a, const PageCopy* copies) {
+// Bound: memory.  CTAs go over (copy, layer, k or v); a thread has eight
+// 16-byte pieces on their way.
+constexpr int CT = 128, CU = 8;
+__global__ void __launch_bounds__(CT) reorder_copy_kernel(const BeamReorderArgs a, const PageCopy* copies,
+                                                          const int* n_copies) {
     griddep_wait();
-    const PageCopy c = copies[blockIdx.x];
-    if (c.dst < 0) return;
-    const int layer = blockIdx.y >> 1, d8 = a.dim / 8, per = a.kv_heads * d8;
-    const bool v = blockIdx.y & 1;
-    uint16_t* base = static_cast<uint16_t*>(v ? a.v : a.k) + layer * (v ? a.v_layer : a.k_layer);
-    const int64_t page = v ? a.v_page : a.k_page, tok = v ? a.v_tok : a.k_tok, head = v ? a.v_head : a.k_head;
-    for (int i = threadIdx.x; i < c.fill * per; i += 256) {
-        const int t = i / per, h = (i - t * per) / d8, e = i - t * per - h * d8;
-        const int64_t o = t * tok + h * head + e * 8;
-        *reinterpret_cast<uint4*>(base + c.dst * page + o) = *reinterpret_cast<const uint4*>(base + c.src * page + o);
+    const int items = *n_copies * 2 * a.layers, d8 = a.dim / 8, per = a.kv_heads * d8;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int which = item % (2 * a.layers), layer = which >> 1;
+        const PageCopy c = copies[item / (2 * a.layers)];
+        const bool v = which & 1;
+        uint16_t* base = static_cast<uint16_t*>(v ? a.v : a.k) + layer * (v ? a.v_layer : a.k_layer);
+        const int64_t page = v ? a.v_page : a.k_page, tok = v ? a.v_tok : a.k_tok, head = v ? a.v_head : a.k_head;
+        const uint16_t* src = base + c.src * page;
+        uint16_t* dst = base + c.dst * page;
+        const int total = c.fill * per;
+        // pieces in the order of the storage: token, head or head, token
+        const bool by_head = head > tok;
+        const int inner = by_head ? c.fill : a.kv_heads;
+        const int64_t in_step = by_head ? tok : head, out_step = by_head ? head : tok;
+        for (int i0 = threadIdx.x; i0 < total; i0 += CT * CU) {
+            uint4 x[CU];
+            int64_t at[CU];
+#pragma unroll
+            for (int u = 0; u < CU; u++) {
+                const int i = i0 + u * CT;
+                const int j = i / d8, o = j / inner;
+                at[u] = o * out_step + (j - o * inner) * in_step + (i - j * d8) * 8;
+                if (i < total) x[u] = __ldcs(reinterpret_cast<const uint4*>(src + at[u]));
+            }
+#pragma unroll
+            for (int u = 0; u < CU; u++)
+                if (i0 + u * CT < total) *reinterpret_cast<uint4*>(dst + at[u]) = x[u];
+        }
     }
 }
 
@@ -594,7 +690,7 @@ int launch_beam_select(const BeamSelectArgs& a, cudaStream_t st) {
 }
 
 int beam_reorder_workspace(const BeamReorderArgs& a, int64_t* bytes) {
-    *bytes = up256(a.n_pages * 4) + 2 * up256(a.new_rows * 4ll) + up256(a.new_rows * 12ll);
+    *bytes = 256 + 2 * up256(a.n_pages * 4) + up256(a.new_rows * 4ll) + up256(a.new_rows * 16ll) + up256(a.new_rows * 12ll);
     return TVQ_OK;
 }
 
@@ -603,13 +699,24 @@ int launch_beam_reorder(const BeamReorderArgs& a, cudaStream_t st) {
     DeviceState* ds = device_state(&rc);
     if (!ds) return rc;
     uint8_t* w = static_cast<uint8_t*>(a.ws);
-    int* held = reinterpret_cast<int*>(w);
-    int* tails = reinterpret_cast<int*>(w + up256(a.n_pages * 4));
-    int* freelist = reinterpret_cast<int*>(w + up256(a.n_pages * 4) + up256(a.new_rows * 4ll));
-    PageCopy* copies = reinterpret_cast<PageCopy*>(w + up256(a.n_pages * 4) + 2 * up256(a.new_rows * 4ll));
-    rc = launch_pdl(reorder_tables_kernel, dim3(1), dim3(1024), 0, st, a, held, tails, freelist, copies, ds->d_error);
+    auto take = [&](int64_t bytes) {
+        uint8_t* p = w;
+        w += up256(bytes);
+        return p;
+    };
+    int* n_copies = reinterpret_cast<int*>(take(4));
+    int* held = reinterpret_cast<int*>(take(a.n_pages * 4));
+    int* owner = reinterpret_cast<int*>(take(a.n_pages * 4));
+    int* freelist = reinterpret_cast<int*>(take(a.new_rows * 4ll));
+    RowPlan* rows = reinterpret_cast<RowPlan*>(take(a.new_rows * 16ll));
+    PageCopy* copies = reinterpret_cast<PageCopy*>(take(a.new_rows * 12ll));
+    const bool small = static_cast<int64_t>(std::max(a.rows, a.new_rows)) * a.cols <= 2 * RT && a.n_pages <= 16 * RT;
+    rc = launch_pdl(small ? reorder_tables_kernel<1> : reorder_tables_kernel<8>, dim3(small ? 1 : 8), dim3(RT), 0, st, a,
+                    held, owner, freelist, rows, copies, n_copies, ds->d_error);
     if (rc || a.new_rows == 0 || a.layers == 0) return rc;
-    return launch_pdl(reorder_copy_kernel, dim3(a.new_rows, 2 * a.layers), dim3(256), 0, st, a, copies);
+    const int64_t items = 2ll * a.new_rows * a.layers;
+    return launch_pdl(reorder_copy_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(items, ds->sm_count * 12ll))), dim3(CT),
+                      0, st, a, copies, n_copies);
 }
 
 }  // namespace tvq
