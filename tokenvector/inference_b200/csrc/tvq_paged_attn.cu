@@ -9,8 +9,8 @@
 // so the keys are read once and parts are joined at the end.  The query heads
 // that share a kv head are rows of one product: row r = i * group + g.
 //
-// attn_rows_kernel: sequences of at most 16 such rows (single tokens, a few
-// drafted ones).  Every key and value is used for at most 16 rows, so the
+// attn_rows_kernel: calls without a sequence of more than 16 such rows (single
+// tokens, a few drafted ones).  Every key and value is used for at most 16 rows, so the
 // bytes of the cache bound it, and what counts is that enough of them are in
 // flight and that every SM has the same share:
 //  - all tiles (8 KB of keys and values) of all (sequence, kv head) pairs
@@ -40,6 +40,7 @@
 
 #include "tvq_common.cuh"
 #include "tvq_decode.h"
+#include "tvq_exact.cuh"
 #include "tvq_kernels.h"
 
 namespace tvq {
@@ -649,13 +650,15 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 }
 
 // ---------------------------------------------------------------- many rows
-// attn_tile_kernel: sequences of more than 16 rows, on the tcgen05 tensor
-// cores.  A unit is two tiles of up to 128 rows (whole tokens: 128 / group of
-// them, with all heads of the group) of one (sequence, kv head), which share
-// the stream of 128-key tiles of K and V.  All (unit, key tile) stand in one
-// line that is cut into equal pieces, one for each SM, as above, so ragged
-// prompts, causal triangles and few rows over many keys all fill the GPU;
-// units cut by a piece's end are joined by attn_tile_join_kernel.
+// attn_tile_kernel: calls with more than 16 rows in some sequence, on the
+// tcgen05 tensor cores.  A unit is two tiles of up to 128 rows (whole tokens:
+// 128 / group of them, with all heads of the group) of one (sequence, kv head),
+// which share the stream of 128-key tiles of K and V; where a sequence's rows
+// end with the first of the two, both take those rows, one the even key tiles
+// and one the odd.  All (unit, key tile) stand in one line that is cut into
+// equal pieces, one for each SM, as above, so ragged prompts, causal triangles
+// and few rows over many keys all fill the GPU; units cut by a piece's end are
+// joined by attn_tile_join_kernel.
 //
 // Per tile t and key tile j, in tensor memory: S_t = Q_t K_j^T (128 x 128
 // f32), its softmax's weights P_t (16-bit, over S_t's columns), O_t += P_t V_j.
@@ -673,8 +676,12 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 // A commit of S_t(j) covers PV_t(j-1), issued before it, so scaling O needs no
 // barrier of its own; and in-order execution of the products lets S_t(j)
 // overwrite P_t(j-1) right behind the product that reads it.
-// Bound: two products of 128 x 128 x D (2 x 512 cycles at D = 128) and 128 x
-// 128 exponentials (1024 cycles of the special-function units) per tile and j.
+// Bound: the two products of a tile and j (2 x 512 cycles at D = 128) wait for
+// its softmax and the softmax for them, so a softmax has to end within the
+// other tile's products: three of eight exponentials are polynomials on the FMA
+// pipe (128 x 128 of them on the special-function units alone take 1024
+// cycles, and both tiles share the units), and the product with V starts when
+// the weights of the first 64 keys are there.
 constexpr int TM = 128, TKEYS = 128;
 constexpr int TTHR = 384;
 enum : int {
@@ -691,8 +698,9 @@ struct TileCfg {
     static constexpr int STAGES = 163840 / STAGE;        // 5 or 10
     static constexpr int OFF_RING = 2 * QT;
     static constexpr int OFF_BAR = OFF_RING + STAGES * STAGE;
-    static constexpr int OFF_WORK = OFF_BAR + (2 * STAGES + 22) * 8;  // Work[4]
-    static constexpr int OFF_MISC = OFF_WORK + 4 * 96;   // int64 at, int seq, tmem
+    static constexpr int OFF_WORK = OFF_BAR + (2 * STAGES + 26) * 8;  // Work[4]
+    static constexpr int OFF_ML = OFF_WORK + 4 * 96;     // float2 [128]
+    static constexpr int OFF_MISC = OFF_ML + 128 * 8;    // int64 at, int seq, tmem
     static constexpr int SMEM = OFF_MISC + 16;
     static constexpr int64_t SLOT = 2 * TM * (DP * 4 + 8);
     static constexpr uint32_t COL_S = 0, COL_O = 256, COLS = DP == 128 ? 512 : 512;
@@ -735,9 +743,10 @@ struct Work {
     int hk, row0, n, len, a, b, more;
     int whole, begins;  // the piece holds all of the unit's key tiles; the first of them
     int i0[2], cnt[2], lo[2], hi[2];
-    int s, pad[4];
+    int s;
+    int dup;  // both row tiles are the first one: key tiles lo, lo + 2, ... each
 };
-static_assert(sizeof(Work) == 88);
+static_assert(sizeof(Work) <= 96);
 
 // Q_t K_j^T with B transposed as given by idesc; A in tensor memory for P V.
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -775,6 +784,30 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of both, x <= 127: 2^n p(f) with n = round(x), f = x - n in [-1/2, 1/2] and p
+// the polynomial of degree 4 whose relative error to 2^f there is the least
+// (Remez): 2.7 10^-6.  Below 2^-126 it stays there.
+__device__ __forceinline__ uint64_t exp2_pair(float x, float y) {
+    const uint64_t v = f2_pack(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
+    const uint64_t big = f2_pack(12582912.0f, 12582912.0f);  // 1.5 2^23: the sum's last bits are n
+    const uint64_t t = f2_add(v, big);
+    const uint64_t f = f2_sub(v, f2_sub(t, big));
+    uint64_t p = f2_pack(0.009570102207362652f, 0.009570102207362652f);
+    p = f2_fma(p, f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
+    p = f2_fma(p, f, f2_pack(0.240247443318367f, 0.240247443318367f));
+    p = f2_fma(p, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+    p = f2_fma(p, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+    float n0, n1, p0, p1;
+    f2_unpack(t, n0, n1);
+    f2_unpack(p, p0, p1);
+    return f2_pack(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23)),
+                   __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23)));
+}
 // wait_full with a code
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* err, int code) {
     const bool ok = mbar_wait_for(bar, parity, nullptr, code, TVQ_WAIT_LIMIT_NS);
@@ -800,13 +833,16 @@ __global__ void __launch_bounds__(TTHR, 1)
     uint64_t* w_full = drain + 1;  // [4] each
     uint64_t* w_empty = w_full + 4;
     uint64_t* v_last = w_empty + 4;  // the values to be fixed are on their way
+    uint64_t* p_half = v_last + 1;   // [2] the weights of the first 64 keys
+    uint64_t* b_ready = p_half + 2;  // tile B's part of tile A's rows is there
+    uint64_t* b_free = b_ready + 1;  // and has been read
+    float2* ml_b = reinterpret_cast<float2*>(sm + C::OFF_ML);
     Work* works = reinterpret_cast<Work*>(sm + C::OFF_WORK);
     int64_t* s_at = reinterpret_cast<int64_t*>(sm + C::OFF_MISC);
     int* s_seq = reinterpret_cast<int*>(s_at + 1);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(s_seq + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.q_heads / a.c.kv_heads;
-    const int fit = MAX_ROWS / group;  // new rows of a sequence that the rows kernel takes
     if (tid == 0) {
         for (int i = 0; i < C::STAGES; i++) {
             mbar_init(kv_full + i, 1);
@@ -817,10 +853,13 @@ __global__ void __launch_bounds__(TTHR, 1)
             mbar_init(q_empty + t, 1);
             mbar_init(s_full + t, 1);
             mbar_init(p_full + t, 4);
+            mbar_init(p_half + t, 4);
             mbar_init(o_full + t, 1);
         }
         mbar_init(v_fixed, 1);
         mbar_init(v_last, 1);
+        mbar_init(b_ready, 4);
+        mbar_init(b_free, 4);
         mbar_init(drain, 1);
         for (int i = 0; i < 4; i++) {
             mbar_init(w_full + i, 1);
@@ -845,7 +884,7 @@ __global__ void __launch_bounds__(TTHR, 1)
     auto weight = [&](int s) -> int64_t {  // of one kv head
         if (s >= a.c.n_seq) return 0;
         const Seq q = load_seq(a.c, s);
-        if (q.n <= fit) return 0;
+        if (q.n == 0) return 0;
         int64_t sum = 0;
         for (int u = 0; u < seq_units(q, plan.tokens); u++) {
             const Unit w = make_unit(q, u, plan.tokens, a.window);
@@ -956,6 +995,13 @@ __global__ void __launch_bounds__(TTHR, 1)
                             o.lo[t] = max(w.first[t], o.a);
                             o.hi[t] = min(w.end[t], o.b);
                         }
+                        o.dup = w.cnt[1] == 0;
+                        if (o.dup) {
+                            o.i0[1] = w.i0[0];
+                            o.cnt[1] = w.cnt[0];
+                            o.lo[1] = o.a + 1;
+                            o.hi[1] = o.b;
+                        }
                         if (o.begins && !o.whole)
                             begun = make_int4(s, hk, u, static_cast<int>((stop - left + w.e - w.f - 1) / per));
                         left -= o.b - o.a;
@@ -966,7 +1012,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                                 hk = 0;
                                 do {
                                     q = load_seq(a.c, ++s);
-                                } while (q.n <= fit);
+                                } while (q.n == 0);
                                 units = seq_units(q, plan.tokens);
                             }
                         }
@@ -999,7 +1045,7 @@ __global__ void __launch_bounds__(TTHR, 1)
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     int& nq = t ? nq1 : nq0;
-                    if (w.lo[t] >= w.hi[t]) continue;
+                    if (w.lo[t] >= w.hi[t] || (t == 1 && w.dup)) continue;
                     ok = ok && wait_bar(q_empty + t, (nq & 1) ^ 1, err, DEVERR_PTILE_EMPTY);
                     if (ok && lane == 0) {
                         mbar_arrive_expect_tx(q_full + t, C::HALVES * plan.tokens * group * 128);
@@ -1053,50 +1099,78 @@ __global__ void __launch_bounds__(TTHR, 1)
                                          (static_cast<uint32_t>(TM >> 4) << 24);
             constexpr uint32_t idesc_o = (1u << 4) | (ty << 7) | (ty << 10) | (1u << 16) |
                                          (static_cast<uint32_t>(DP >> 3) << 17) | (static_cast<uint32_t>(TM >> 4) << 24);
-            const int ksteps = (a.c.dim + 15) / 16;
             if (lane == 0) {
                 // the ring holds K_a, V_a, K_a+1, ...: step j uses V_{j-1} (stage sv) and K_j (stage sk)
                 int sk = 0, pk = 0, nq = 0, np = 0, nfix = 0;  // nq, np: a bit for each row tile's parity
+                auto scores = [&](int t, int q, uint32_t ka) {  // S_t = Q_q K^T
+                    const uint64_t qd = smem_desc_k_sw128(smem_u32(sm) + q * C::QT), kd = smem_desc_k_sw128(ka);
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++) {  // (values behind the head dim are zeros in both)
+                        const uint64_t off = ((i >> 2) * C::HALF + (i & 3) * 32) >> 4;
+                        umma_f16(tmem + C::COL_S + t * TKEYS, qd + off, kd + off, idesc_s, i > 0);
+                    }
+                    umma_commit(s_full + t);
+                };
+                auto values = [&](int t, uint32_t va, bool first) {  // O_t (+)= P_t V
+                    const uint64_t vd = smem_desc_mn_sw128(va, C::HALF);
+                    for (int h = 0; ok && h < 2; h++) {
+                        ok = wait_bar((h ? p_full : p_half) + t, (np >> t) & 1, err, DEVERR_PTILE_P);
+                        if (!ok) return;
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = 0; i < TKEYS / 32; i++)
+                            umma_ts(tmem + C::COL_O + t * DP, tmem + C::COL_S + t * TKEYS + (h * (TKEYS / 32) + i) * 8,
+                                    vd + (h * (TKEYS / 32) + i) * (2048 >> 4), idesc_o,
+                                    (!first || h > 0 || i > 0) ? 1u : 0u);
+                    }
+                    np ^= 1 << t;
+                };
                 for (int k = 0; take(k); k++) {
                     const Work& w = works[k & 3];
                     const int first = w.a, end = w.b, len = w.len;
                     const int lo[2] = {w.lo[0], w.lo[1]}, hi[2] = {w.hi[0], w.hi[1]};
+                    const bool dup = w.dup;
                     int sv = 0, pv = 0;
                     for (int j = first; ok && j <= end; j++) {
                         const uint32_t ka = smem_u32(sm) + C::OFF_RING + sk * C::STAGE;
                         const uint32_t va = smem_u32(sm) + C::OFF_RING + sv * C::STAGE;
-                        if (j > first) {
+                        if (j < end) ok = wait_bar(kv_full + sk, pk, err, DEVERR_PTILE_KV);
+                        if (ok && dup && j < end) {  // S_t(j) depends on nothing of j - 1, the other tile's
+                            if (j == first) {
+                                ok = wait_bar(q_full, nq & 1, err, DEVERR_PTILE_Q);
+                                nq ^= 1;
+                            }
+                            if (ok) {
+                                scores((j - first) & 1, 0, ka);
+                                if (j == end - 1) umma_commit(q_empty);
+                            }
+                        }
+                        if (ok && j > first) {
                             ok = wait_bar(kv_full + sv, pv, err, DEVERR_PTILE_KV);
                             if (ok && j * TKEYS > len) ok = wait_bar(v_fixed, nfix++ & 1, err, DEVERR_PTILE_FIX);
                         }
-                        if (ok && j < end) ok = wait_bar(kv_full + sk, pk, err, DEVERR_PTILE_KV);
-#pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            if (ok && j - 1 >= lo[t] && j - 1 < hi[t]) {
-                                ok = wait_bar(p_full + t, (np >> t) & 1, err, DEVERR_PTILE_P);
-                                np ^= 1 << t;
-                                if (!ok) break;
-                                tc_fence_after();
-#pragma unroll
-                                for (int i = 0; i < TKEYS / 16; i++)
-                                    umma_ts(tmem + C::COL_O + t * DP, tmem + C::COL_S + t * TKEYS + i * 8,
-                                            smem_desc_mn_sw128(va + i * 2048, C::HALF), idesc_o, (j - 1 > lo[t] || i > 0) ? 1u : 0u);
-                                if (j == hi[t]) umma_commit(o_full + t);
+                        if (dup) {
+                            const int t = (j - first + 1) & 1;  // the tile that has j - 1
+                            if (ok && j > first) {
+                                values(t, va, j - 1 < first + 2);
+                                if (ok && j + 1 >= end) umma_commit(o_full + t);
                             }
-                            if (ok && j >= lo[t] && j < hi[t]) {
-                                if (j == lo[t]) {
-                                    ok = wait_bar(q_full + t, (nq >> t) & 1, err, DEVERR_PTILE_Q);
-                                    nq ^= 1 << t;
-                                    if (!ok) break;
+                        } else {
+#pragma unroll
+                            for (int t = 0; t < 2; t++) {
+                                if (ok && j - 1 >= lo[t] && j - 1 < hi[t]) {
+                                    values(t, va, j - 1 == lo[t]);
+                                    if (ok && j == hi[t]) umma_commit(o_full + t);
                                 }
-                                const uint32_t qa = smem_u32(sm) + t * C::QT;
-                                for (int i = 0; i < ksteps; i++) {
-                                    const uint32_t off = (i >> 2) * C::HALF + (i & 3) * 32;
-                                    umma_f16(tmem + C::COL_S + t * TKEYS, smem_desc_k_sw128(qa + off),
-                                             smem_desc_k_sw128(ka + off), idesc_s, i > 0);
+                                if (ok && j >= lo[t] && j < hi[t]) {
+                                    if (j == lo[t]) {
+                                        ok = wait_bar(q_full + t, (nq >> t) & 1, err, DEVERR_PTILE_Q);
+                                        nq ^= 1 << t;
+                                        if (!ok) break;
+                                    }
+                                    scores(t, t, ka);
+                                    if (j == hi[t] - 1) umma_commit(q_empty + t);
                                 }
-                                umma_commit(s_full + t);
-                                if (j == hi[t] - 1) umma_commit(q_empty + t);
                             }
                         }
                         if (!ok) break;
@@ -1159,7 +1233,7 @@ __global__ void __launch_bounds__(TTHR, 1)
         const uint32_t s_addr = lanes + C::COL_S + t * TKEYS, o_addr = lanes + C::COL_O + t * DP;
         const float scale2 = plan.scale2;
         const int ri = row / group, gi = row - ri * group;  // this row's token of the tile, its head of the group
-        int ns = 0, no = 0;
+        int ns = 0, no = 0, nd = 0;
         for (int k = 0; __all_sync(0xffffffffu, take(k)); k++) {
             const Work& w = works[k & 3];
             const int lo = w.lo[t], hi = w.hi[t];
@@ -1168,35 +1242,45 @@ __global__ void __launch_bounds__(TTHR, 1)
             const int pmin = w.len - w.n + w.i0[t], pmax = pmin + w.cnt[t] - 1;
             const int pos = valid ? pmin + ri : -1;
             float m = -INFINITY, l = 0.0f;  // m of the raw products
-            for (int j = lo; j < hi; j++) {
+            for (int j = lo; j < hi; j += w.dup ? 2 : 1) {
                 if (ok) ok = __all_sync(0xffffffffu, wait_bar(s_full + t, ns & 1, err, DEVERR_PTILE_S));
                 ns++;
                 tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld32(s_addr + c * 32, s[c]);
-                tmem_ld_wait();
-                if (plan.negative) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int e = 0; e < 32; e++) s[c][e] ^= 0x80000000u;
-                }
+                // A row's scores are read twice, 32 at a time, in rolled loops: the code of 128 at once (40 KB) drove
+                // the other warps' out of the instruction cache, and a product's issue took 800 cycles for it.
                 const int k0 = j * TKEYS;
-                if (k0 + TKEYS - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window)) {
-                    const int top = pos - k0, bot = a.window > 0 ? top - a.window : -1;  // columns in (bot, top]
+                const bool edge = k0 + TKEYS - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window);
+                auto load = [&](int c, uint32_t (&s)[32]) {
+                    tmem_ld32(s_addr + c * 32, s);
+                    tmem_ld_wait();
+                    if (plan.negative) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                        for (int e = 0; e < 32; e++) s[e] ^= 0x80000000u;
+                    }
+                    if (edge) {
+                        const int top = pos - k0 - c * 32, bot = a.window > 0 ? top - a.window : -1;  // columns in (bot, top]
 #pragma unroll
                         for (int e = 0; e < 32; e++)
-                            if (c * 32 + e > top || c * 32 + e <= bot) s[c][e] = 0xFF800000u;  // -inf
+                            if (e > top || e <= bot) s[e] = 0xFF800000u;  // -inf
+                    }
+                };
+                // (NaN goes through: the row is then NaN)
+                float tile = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    uint32_t s[32];
+                    load(c, s);
+                    float mx[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        mx[q] = max3(__uint_as_float(s[q * 8]), __uint_as_float(s[q * 8 + 1]), __uint_as_float(s[q * 8 + 2]));
+                        mx[q] = max3(mx[q], __uint_as_float(s[q * 8 + 3]), __uint_as_float(s[q * 8 + 4]));
+                        mx[q] = max3(mx[q], __uint_as_float(s[q * 8 + 5]), __uint_as_float(s[q * 8 + 6]));
+                    }
+                    const float r = max3(max3(mx[0], mx[1], mx[2]), mx[3], __uint_as_float(s[7]));
+                    tile = max3(max3(tile, r, __uint_as_float(s[15])), __uint_as_float(s[23]), __uint_as_float(s[31]));
                 }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int e = 0; e < 32; e++) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
-                const float tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (tile != tile) l = tile;
                 // l == 0 and O == 0 as long as m is -inf: nothing to scale then
                 const bool grow = m != -INFINITY && (tile - m) * scale2 > 8.0f;
                 if (__any_sync(0xffffffffu, grow)) {
@@ -1217,69 +1301,123 @@ __global__ void __launch_bounds__(TTHR, 1)
                 }
                 if (m == -INFINITY) m = tile;
                 const float base = m == -INFINITY ? 0.0f : m * scale2;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t scale22 = f2_pack(scale2, scale2), base2 = f2_pack(-base, -base);
+                uint64_t sum2[2] = {0ull, 0ull};
                 // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
                 // rounding of the result; l sums them unrounded
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 4; c++) {
-                    uint32_t p[16];
+                    uint32_t s[32], p[16];
+                    load(c, s);  // (P's columns of chunk c lie within the scores read so far)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const float x = ex2(fmaf(__uint_as_float(s[c][2 * e]), scale2, -base));
-                        const float y = ex2(fmaf(__uint_as_float(s[c][2 * e + 1]), scale2, -base));
-                        sum[e & 3] += x + y;
-                        p[e] = pack2<T>(x, y);
+                        const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale22, base2);
+                        float y, z;
+                        f2_unpack(x, y, z);
+                        if (e * 3 % 8 < 3) {
+                            const uint64_t q = exp2_pair(y, z);
+                            f2_unpack(q, y, z);
+                            sum2[e & 1] = f2_add(sum2[e & 1], q);
+                        } else {
+                            y = ex2(y);
+                            z = ex2(z);
+                            sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(y, z));
+                        }
+                        p[e] = pack2<T>(y, z);
                     }
                     tmem_st16(s_addr + c * 16, p);
+                    if (c == 1) {  // the first 64 keys' weights
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_half + t);
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float sa, sb, sc, sd;
+                f2_unpack(sum2[0], sa, sb);
+                f2_unpack(sum2[1], sc, sd);
+                l += (sa + sb) + (sc + sd);
+                if (m == -INFINITY) l = 0.0f;  // no key yet (the polynomial's weights of masked ones are 2^-126, not 0)
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + t);
             }
             // ---- the tile's end
-            const bool whole = w.whole;
+            const bool whole = w.whole, dup = w.dup;
             uint8_t* part = plan.parts + (static_cast<int64_t>(blockIdx.x) * 2 + w.begins) * C::SLOT;
             const int64_t at = static_cast<int64_t>(w.row0 + w.i0[t] + ri) * a.q_heads + w.hk * group + gi;
             if (lo < hi) {
                 if (ok) ok = __all_sync(0xffffffffu, wait_bar(o_full + t, no & 1, err, DEVERR_PTILE_O));
                 no++;
                 tc_fence_after();
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-                for (int c = 0; c < DP / 32; c++) {
-                    uint32_t o[32];
+            }
+            float mt = l == 0.0f ? -INFINITY : m * scale2, fa = 1.0f, fb = 0.0f;
+            if (dup) {  // tile A takes up what tile B has of the same rows
+                if (t == 1) {
+                    ml_b[row] = make_float2(mt, l);
+                    tc_fence_before();
                     __syncwarp();
-                    tmem_ld32(o_addr + c * 32, o);
+                    if (lane == 0) mbar_arrive(b_ready);
+                } else {
+                    if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_ready, nd & 1, err, DEVERR_PTILE_O));
+                    tc_fence_after();
+                    const float2 b = ml_b[row];
+                    const float top = fmaxf(mt, b.x), base = top == -INFINITY ? 0.0f : top;
+                    fa = ex2(mt - base);
+                    fb = ex2(b.x - base);
+                    l = l * fa + b.y * fb;
+                    mt = top;
+                }
+            }
+            const bool both = dup && w.lo[1] < w.hi[1];
+            if (lo < hi && !(dup && t == 1)) {
+                const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                const float ga = fa * inv, gb = fb * inv;
+#pragma unroll
+                for (int c = 0; c < DP / 16; c++) {
+                    uint32_t o[16], ob[16];
+                    __syncwarp();
+                    tmem_ld16(o_addr + c * 16, o);
+                    if (both) tmem_ld16(o_addr + DP + c * 16, ob);
                     tmem_ld_wait();
+                    float y[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        y[e] = __uint_as_float(o[e]) * ga;
+                        if (both) y[e] = fmaf(__uint_as_float(ob[e]), gb, y[e]);
+                    }
                     if (!valid) continue;
                     if (whole) {
-                        T* out = static_cast<T*>(a.out) + at * a.c.dim + c * 32;
+                        T* out = static_cast<T*>(a.out) + at * a.c.dim + c * 16;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if (c * 32 + e * 8 >= a.c.dim) continue;
-                            uint4 v;
-                            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                x[i] = pack2<T>(__uint_as_float(o[e * 8 + 2 * i]) * inv, __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
-                            *reinterpret_cast<uint4*>(out + e * 8) = v;
+                        for (int e = 0; e < 2; e++) {
+                            if (c * 16 + e * 8 >= a.c.dim) continue;
+                            *reinterpret_cast<uint4*>(out + e * 8) =
+                                make_uint4(pack2<T>(y[e * 8], y[e * 8 + 1]), pack2<T>(y[e * 8 + 2], y[e * 8 + 3]),
+                                           pack2<T>(y[e * 8 + 4], y[e * 8 + 5]), pack2<T>(y[e * 8 + 6], y[e * 8 + 7]));
                         }
                     } else {
-                        uint4* out = reinterpret_cast<uint4*>(part + ((t * TM + row) * DP + c * 32) * 4);
+                        float4* out = reinterpret_cast<float4*>(part + ((t * TM + row) * DP + c * 16) * 4);
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            out[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        for (int e = 0; e < 4; e++) out[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
                     }
                 }
                 tc_fence_before();
             }
-            if (valid && whole && a.lse)
-                a.lse[at] = l == 0.0f ? -INFINITY : (m * scale2 + log2f(l)) * 0.6931471805599453f;
-            if (valid && !whole)  // (a row tile without keys in the piece: m -inf)
-                *reinterpret_cast<float2*>(part + 2 * TM * DP * 4 + (t * TM + row) * 8) =
-                    make_float2(l == 0.0f ? -INFINITY : m * scale2, l);
+            if (!(dup && t == 1)) {
+                if (valid && whole && a.lse) a.lse[at] = l == 0.0f ? -INFINITY : (mt + log2f(l)) * 0.6931471805599453f;
+                if (valid && !whole)  // (a row tile without keys in the piece: m -inf)
+                    *reinterpret_cast<float2*>(part + 2 * TM * DP * 4 + (t * TM + row) * 8) = make_float2(mt, l);
+            }
+            if (dup && t == 0) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_free);
+            } else if (dup) {  // its output and statistics may be written again
+                if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_free, nd & 1, err, DEVERR_PTILE_O));
+                tc_fence_after();
+            }
+            nd += dup;
             __syncwarp();
             if (lane == 0) done(k);
         }
@@ -1336,6 +1474,10 @@ namespace {
 
 int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
+bool few_rows(const PagedAttnArgs& a) {
+    return static_cast<int64_t>(a.max_q) * (a.q_heads / a.c.kv_heads) <= MAX_ROWS;
+}
+
 // Workspace of the rows kernel: spans of all pairs, then two parts per piece.
 struct RowsSpace {
     int64_t spans = 0, slot = 0, bytes = 0;
@@ -1344,7 +1486,7 @@ struct RowsSpace {
 RowsSpace rows_space(const PagedAttnArgs& a, int sms) {
     RowsSpace w;
     const int group = a.q_heads / a.c.kv_heads;
-    if (group > MAX_ROWS || a.max_q == 0) return w;
+    if (!few_rows(a) || a.max_q == 0) return w;
     const int dp = a.c.dim > 64 ? 128 : 64;
     w.rows_cap = std::min(MAX_ROWS / group, a.max_q) * group;
     w.slot = up256(w.rows_cap * (dp * 4ll + 8));
@@ -1353,13 +1495,13 @@ RowsSpace rows_space(const PagedAttnArgs& a, int sms) {
     return w;
 }
 
-// Workspace of the tile kernel, behind it: the pieces' units, two parts per piece.
+// Workspace of the tile kernel: the pieces' units, two parts per piece.
 struct TileSpace {
     int64_t begun = 0, bytes = 0;
 };
 TileSpace tile_space(const PagedAttnArgs& a, int sms) {
     TileSpace w;
-    if (static_cast<int64_t>(a.max_q) * (a.q_heads / a.c.kv_heads) <= MAX_ROWS) return w;
+    if (few_rows(a)) return w;
     w.begun = up256(16ll * sms);
     w.bytes = w.begun + 2ll * sms * (a.c.dim > 64 ? TileCfg<128>::SLOT : TileCfg<64>::SLOT);
     return w;
@@ -1431,7 +1573,7 @@ int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
         cudaFuncSetAttribute(attn_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     TVQ_CUDA(attr);
     const int group = a.q_heads / a.c.kv_heads;
-    uint8_t* ws = static_cast<uint8_t*>(a.ws) + rows_space(a, ds->sm_count).bytes;
+    uint8_t* ws = static_cast<uint8_t*>(a.ws);
     TilePlan plan;
     plan.begun = reinterpret_cast<int4*>(ws);
     plan.parts = ws + tile_space(a, ds->sm_count).begun;
@@ -1459,14 +1601,12 @@ int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     return launch_pdl(attn_tile_join_kernel<T, DP>, dim3(ds->sm_count, 2 * TM / 8), dim3(256), 0, st, a, plan);
 }
 
-// Each kernel takes the sequences of its side of 16 rows, told apart on the
-// device; max_q rules the tile kernel out for steps of few rows.
+// Steps (no sequence has more than 16 rows): the rows kernel, which waits for
+// nothing but the cache.  Else the tile kernel for all sequences; those of few
+// rows among them take it ~1.5 us a key tile and SM, what their bytes take.
 template <typename T>
 int launch_attention(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
-    const int group = a.q_heads / a.c.kv_heads;
-    int rc = TVQ_OK;
-    if (group <= MAX_ROWS) rc = a.c.dim > 64 ? launch_rows<T, 128>(a, ds, st) : launch_rows<T, 64>(a, ds, st);
-    if (rc || static_cast<int64_t>(a.max_q) * group <= MAX_ROWS) return rc;
+    if (few_rows(a)) return a.c.dim > 64 ? launch_rows<T, 128>(a, ds, st) : launch_rows<T, 64>(a, ds, st);
     return a.c.dim > 64 ? launch_tiles<T, 128>(a, ds, st) : launch_tiles<T, 64>(a, ds, st);
 }
 
