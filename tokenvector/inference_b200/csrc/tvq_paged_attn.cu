@@ -661,7 +661,8 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 // joined by attn_tile_join_kernel.
 //
 // Per tile t and key tile j, in tensor memory: S_t = Q_t K_j^T (128 x 128
-// f32), its softmax's weights P_t (16-bit, over S_t's columns), O_t += P_t V_j.
+// f32), its softmax's weights P_t (16-bit, over S_t's columns: those of keys
+// 0-63 from column 0, of keys 64-127 from column 64), O_t += P_t V_j.
 //   warp 0       TMA: Q of a unit, then K_j, V_j through one ring
 //   warp 1       MMA issuer: for each j, PV_A(j-1), S_A(j), PV_B(j-1), S_B(j),
 //                so one tile's softmax runs under the other's products
@@ -669,7 +670,9 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 //                (they may be anything, and 0 x NaN is NaN)
 //   warp 3       walks the piece and leaves the units for the others in shared
 //                memory, up to four ahead
-//   warps 4-7, 8-11  softmax of tile A, B: a thread has a row, all 128 keys
+//   warps 4-19   softmax, eight for each tile: two threads have a row, 64 keys
+//                each (one thread with 128 keys has too little to do at once:
+//                its instructions waited 1.4 cycles each for one another)
 // O stays relative to the row's first maximum until the running one exceeds it
 // by 2^8 (then O and l are scaled by the softmax warps): weights stay below
 // 2^8, exact enough in either 16-bit type, and nearly no tile is scaled twice.
@@ -683,7 +686,7 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 // cycles, and both tiles share the units), and the product with V starts when
 // the weights of the first 64 keys are there.
 constexpr int TM = 128, TKEYS = 128;
-constexpr int TTHR = 384;
+constexpr int TTHR = 640;
 enum : int {
     DEVERR_PTILE_EMPTY = 73, DEVERR_PTILE_Q = 74, DEVERR_PTILE_KV = 75, DEVERR_PTILE_P = 76, DEVERR_PTILE_S = 77,
     DEVERR_PTILE_O = 78, DEVERR_PTILE_FIX = 79, DEVERR_PTILE_DRAIN = 80, DEVERR_PTILE_WORK = 81
@@ -699,8 +702,8 @@ struct TileCfg {
     static constexpr int OFF_RING = 2 * QT;
     static constexpr int OFF_BAR = OFF_RING + STAGES * STAGE;
     static constexpr int OFF_WORK = OFF_BAR + (2 * STAGES + 26) * 8;  // Work[4]
-    static constexpr int OFF_ML = OFF_WORK + 4 * 96;     // float2 [128]
-    static constexpr int OFF_MISC = OFF_ML + 128 * 8;    // int64 at, int seq, tmem
+    static constexpr int OFF_X = OFF_WORK + 4 * 96;      // float [2][2][128]: what the halves of a row tell each other
+    static constexpr int OFF_MISC = OFF_X + 2 * 2 * 128 * 4;  // int64 at, int seq, tmem
     static constexpr int SMEM = OFF_MISC + 16;
     static constexpr int64_t SLOT = 2 * TM * (DP * 4 + 8);
     static constexpr uint32_t COL_S = 0, COL_O = 256, COLS = DP == 128 ? 512 : 512;
@@ -836,7 +839,6 @@ __global__ void __launch_bounds__(TTHR, 1)
     uint64_t* p_half = v_last + 1;   // [2] the weights of the first 64 keys
     uint64_t* b_ready = p_half + 2;  // tile B's part of tile A's rows is there
     uint64_t* b_free = b_ready + 1;  // and has been read
-    float2* ml_b = reinterpret_cast<float2*>(sm + C::OFF_ML);
     Work* works = reinterpret_cast<Work*>(sm + C::OFF_WORK);
     int64_t* s_at = reinterpret_cast<int64_t*>(sm + C::OFF_MISC);
     int* s_seq = reinterpret_cast<int*>(s_at + 1);
@@ -858,12 +860,12 @@ __global__ void __launch_bounds__(TTHR, 1)
         }
         mbar_init(v_fixed, 1);
         mbar_init(v_last, 1);
-        mbar_init(b_ready, 4);
-        mbar_init(b_free, 4);
+        mbar_init(b_ready, 8);
+        mbar_init(b_free, 8);
         mbar_init(drain, 1);
         for (int i = 0; i < 4; i++) {
             mbar_init(w_full + i, 1);
-            mbar_init(w_empty + i, 11);  // TMA, MMA, fixing and eight softmax warps
+            mbar_init(w_empty + i, 19);  // TMA, MMA, fixing and sixteen softmax warps
         }
         fence_barrier_init();
         tma_prefetch_desc(&tmQ);
@@ -944,9 +946,7 @@ __global__ void __launch_bounds__(TTHR, 1)
     auto done = [&](int k) {  // by one thread of a warp, once the warp needs nothing more of it
         mbar_arrive(w_empty + (k & 3));
     };
-    // a softmax thread holds a row of 128 scores: 256 x 208 + 128 x 88 registers of the 384 x 168 launched with
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 3) {
             // ------------------------------------------------ the walk
             if (lane == 0) {
@@ -1119,7 +1119,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                         tc_fence_after();
 #pragma unroll
                         for (int i = 0; i < TKEYS / 32; i++)
-                            umma_ts(tmem + C::COL_O + t * DP, tmem + C::COL_S + t * TKEYS + (h * (TKEYS / 32) + i) * 8,
+                            umma_ts(tmem + C::COL_O + t * DP, tmem + C::COL_S + t * TKEYS + h * 64 + i * 8,
                                     vd + (h * (TKEYS / 32) + i) * (2048 >> 4), idesc_o,
                                     (!first || h > 0 || i > 0) ? 1u : 0u);
                     }
@@ -1225,16 +1225,22 @@ __global__ void __launch_bounds__(TTHR, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ------------------------------------------------ softmax
-        const int t = (warp >> 2) - 1, wl = warp & 3;
+        const int t = (warp - 4) >> 3, half = (warp >> 2) & 1 ? 0 : 1, wl = warp & 3;  // warps 4-7, 12-15: keys 0-63
         const int row = wl * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(wl * 32) << 16);
-        const uint32_t s_addr = lanes + C::COL_S + t * TKEYS, o_addr = lanes + C::COL_O + t * DP;
+        // this thread's 64 scores; its weights go over the first 32 columns of them
+        const uint32_t s_addr = lanes + C::COL_S + t * TKEYS + half * 64;
+        const uint32_t o_addr = lanes + C::COL_O + t * DP;
+        float* x_mine = reinterpret_cast<float*>(sm + C::OFF_X) + (t * 2 + half) * 128 + row;
+        const float* x_other = reinterpret_cast<float*>(sm + C::OFF_X) + (t * 2 + (half ^ 1)) * 128 + row;
+        const float* x_b = reinterpret_cast<float*>(sm + C::OFF_X) + 2 * 128 + row;  // tile B's, at a unit's end
+        const uint32_t pair_bar = 1 + t * 4 + wl;  // of the two warps that share 32 rows
         const float scale2 = plan.scale2;
         const int ri = row / group, gi = row - ri * group;  // this row's token of the tile, its head of the group
         int ns = 0, no = 0, nd = 0;
-        for (int k = 0; __all_sync(0xffffffffu, take(k)); k++) {
+        // (both warps of a pair go on, or neither: they meet at barriers)
+        for (int k = 0; named_bar_and(pair_bar, 64, take(k)); k++) {
             const Work& w = works[k & 3];
             const int lo = w.lo[t], hi = w.hi[t];
             const bool valid = ri < w.cnt[t];
@@ -1246,10 +1252,10 @@ __global__ void __launch_bounds__(TTHR, 1)
                 if (ok) ok = __all_sync(0xffffffffu, wait_bar(s_full + t, ns & 1, err, DEVERR_PTILE_S));
                 ns++;
                 tc_fence_after();
-                // A row's scores are read twice, 32 at a time, in rolled loops: the code of 128 at once (40 KB) drove
-                // the other warps' out of the instruction cache, and a product's issue took 800 cycles for it.
-                const int k0 = j * TKEYS;
-                const bool edge = k0 + TKEYS - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window);
+                // The scores are read twice, 32 at a time, in rolled loops: unrolled code (40 KB) drove the other
+                // warps' out of the instruction cache, and a product's issue took 800 cycles for it.
+                const int k0 = j * TKEYS + half * 64;
+                const bool edge = k0 + 63 > pmin || (a.window > 0 && k0 <= pmax - a.window);
                 auto load = [&](int c, uint32_t (&s)[32]) {
                     tmem_ld32(s_addr + c * 32, s);
                     tmem_ld_wait();
@@ -1267,7 +1273,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                 // (NaN goes through: the row is then NaN)
                 float tile = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
                     uint32_t s[32];
                     load(c, s);
                     float mx[4];
@@ -1280,13 +1286,16 @@ __global__ void __launch_bounds__(TTHR, 1)
                     const float r = max3(max3(mx[0], mx[1], mx[2]), mx[3], __uint_as_float(s[7]));
                     tile = max3(max3(tile, r, __uint_as_float(s[15])), __uint_as_float(s[23]), __uint_as_float(s[31]));
                 }
+                *x_mine = tile;
+                ok = named_bar_and(pair_bar, 64, ok);
+                tile = max3(tile, *x_other, tile);
                 if (tile != tile) l = tile;
                 // l == 0 and O == 0 as long as m is -inf: nothing to scale then
                 const bool grow = m != -INFINITY && (tile - m) * scale2 > 8.0f;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float f = grow ? ex2((m - tile) * scale2) : 1.0f;
-                    if (j > lo) {
-#pragma unroll
+                    if (j > lo && half == 0) {
+#pragma unroll 1
                         for (int c = 0; c < DP / 16; c++) {
                             uint32_t o[16];
                             tmem_ld16(o_addr + c * 16, o);
@@ -1306,15 +1315,15 @@ __global__ void __launch_bounds__(TTHR, 1)
                 // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
                 // rounding of the result; l sums them unrounded
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
                     uint32_t s[32], p[16];
-                    load(c, s);  // (P's columns of chunk c lie within the scores read so far)
+                    load(c, s);  // (the weights' columns lie within the scores read so far)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale22, base2);
                         float y, z;
                         f2_unpack(x, y, z);
-                        if (e * 3 % 8 < 3) {
+                        if (e % 4 == 3) {
                             const uint64_t q = exp2_pair(y, z);
                             f2_unpack(q, y, z);
                             sum2[e & 1] = f2_add(sum2[e & 1], q);
@@ -1326,12 +1335,6 @@ __global__ void __launch_bounds__(TTHR, 1)
                         p[e] = pack2<T>(y, z);
                     }
                     tmem_st16(s_addr + c * 16, p);
-                    if (c == 1) {  // the first 64 keys' weights
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(p_half + t);
-                    }
                 }
                 float sa, sb, sc, sd;
                 f2_unpack(sum2[0], sa, sb);
@@ -1341,12 +1344,16 @@ __global__ void __launch_bounds__(TTHR, 1)
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + t);
+                if (lane == 0) mbar_arrive((half ? p_full : p_half) + t);
             }
             // ---- the tile's end
             const bool whole = w.whole, dup = w.dup;
             uint8_t* part = plan.parts + (static_cast<int64_t>(blockIdx.x) * 2 + w.begins) * C::SLOT;
             const int64_t at = static_cast<int64_t>(w.row0 + w.i0[t] + ri) * a.q_heads + w.hk * group + gi;
+            named_bar_sync(pair_bar, 64);  // (the last maxima have been read)
+            *x_mine = l;
+            ok = named_bar_and(pair_bar, 64, ok);
+            l += *x_other;
             if (lo < hi) {
                 if (ok) ok = __all_sync(0xffffffffu, wait_bar(o_full + t, no & 1, err, DEVERR_PTILE_O));
                 no++;
@@ -1355,14 +1362,15 @@ __global__ void __launch_bounds__(TTHR, 1)
             float mt = l == 0.0f ? -INFINITY : m * scale2, fa = 1.0f, fb = 0.0f;
             if (dup) {  // tile A takes up what tile B has of the same rows
                 if (t == 1) {
-                    ml_b[row] = make_float2(mt, l);
+                    named_bar_sync(pair_bar, 64);  // (the sums have been read)
+                    *x_mine = half ? l : mt;
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(b_ready);
                 } else {
                     if (ok) ok = __all_sync(0xffffffffu, wait_bar(b_ready, nd & 1, err, DEVERR_PTILE_O));
                     tc_fence_after();
-                    const float2 b = ml_b[row];
+                    const float2 b = make_float2(x_b[0], x_b[128]);
                     const float top = fmaxf(mt, b.x), base = top == -INFINITY ? 0.0f : top;
                     fa = ex2(mt - base);
                     fb = ex2(b.x - base);
@@ -1374,8 +1382,8 @@ __global__ void __launch_bounds__(TTHR, 1)
             if (lo < hi && !(dup && t == 1)) {
                 const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
                 const float ga = fa * inv, gb = fb * inv;
-#pragma unroll
-                for (int c = 0; c < DP / 16; c++) {
+#pragma unroll 1
+                for (int c = half * (DP / 32); c < (half + 1) * (DP / 32); c++) {
                     uint32_t o[16], ob[16];
                     __syncwarp();
                     tmem_ld16(o_addr + c * 16, o);
@@ -1405,7 +1413,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                 }
                 tc_fence_before();
             }
-            if (!(dup && t == 1)) {
+            if (half == 0 && !(dup && t == 1)) {
                 if (valid && whole && a.lse) a.lse[at] = l == 0.0f ? -INFINITY : (mt + log2f(l)) * 0.6931471805599453f;
                 if (valid && !whole)  // (a row tile without keys in the piece: m -inf)
                     *reinterpret_cast<float2*>(part + 2 * TM * DP * 4 + (t * TM + row) * 8) = make_float2(mt, l);
