@@ -701,7 +701,7 @@ struct TileCfg {
     static constexpr int STAGES = 163840 / STAGE;        // 5 or 10
     static constexpr int OFF_RING = 2 * QT;
     static constexpr int OFF_BAR = OFF_RING + STAGES * STAGE;
-    static constexpr int OFF_WORK = OFF_BAR + (2 * STAGES + 26) * 8;  // Work[4]
+    static constexpr int OFF_WORK = OFF_BAR + (3 * STAGES + 24) * 8;  // Work[4]
     static constexpr int OFF_X = OFF_WORK + 4 * 96;      // float [2][2][128]: what the halves of a row tell each other
     static constexpr int OFF_MISC = OFF_X + 2 * 2 * 128 * 4;  // int64 at, int seq, tmem
     static constexpr int SMEM = OFF_MISC + 16;
@@ -831,14 +831,13 @@ __global__ void __launch_bounds__(TTHR, 1)
     uint64_t* s_full = q_empty + 2;
     uint64_t* p_full = s_full + 2;
     uint64_t* o_full = p_full + 2;
-    uint64_t* v_fixed = o_full + 2;
-    uint64_t* drain = v_fixed + 1;
+    uint64_t* drain = o_full + 2;
     uint64_t* w_full = drain + 1;  // [4] each
     uint64_t* w_empty = w_full + 4;
-    uint64_t* v_last = w_empty + 4;  // the values to be fixed are on their way
-    uint64_t* p_half = v_last + 1;   // [2] the weights of the first 64 keys
+    uint64_t* p_half = w_empty + 4;  // [2] the weights of the first 64 keys
     uint64_t* b_ready = p_half + 2;  // tile B's part of tile A's rows is there
     uint64_t* b_free = b_ready + 1;  // and has been read
+    uint64_t* v_fixed = b_free + 1;  // [STAGES] the values there end with the sequence
     Work* works = reinterpret_cast<Work*>(sm + C::OFF_WORK);
     int64_t* s_at = reinterpret_cast<int64_t*>(sm + C::OFF_MISC);
     int* s_seq = reinterpret_cast<int*>(s_at + 1);
@@ -848,7 +847,8 @@ __global__ void __launch_bounds__(TTHR, 1)
     if (tid == 0) {
         for (int i = 0; i < C::STAGES; i++) {
             mbar_init(kv_full + i, 1);
-            mbar_init(kv_empty + i, 1);
+            mbar_init(kv_empty + i, 2);  // the issuer and the fixing warp
+            mbar_init(v_fixed + i, 1);
         }
         for (int t = 0; t < 2; t++) {
             mbar_init(q_full + t, 1);
@@ -858,8 +858,6 @@ __global__ void __launch_bounds__(TTHR, 1)
             mbar_init(p_half + t, 4);
             mbar_init(o_full + t, 1);
         }
-        mbar_init(v_fixed, 1);
-        mbar_init(v_last, 1);
         mbar_init(b_ready, 8);
         mbar_init(b_free, 8);
         mbar_init(drain, 1);
@@ -1079,7 +1077,6 @@ __global__ void __launch_bounds__(TTHR, 1)
                             phase ^= 1;
                         }
                     }
-                    if (ok && (j + 1) * TKEYS > len && lane == 0) mbar_arrive(v_last);
                 }
                 __syncwarp();
                 if (lane == 0) done(k);
@@ -1101,7 +1098,8 @@ __global__ void __launch_bounds__(TTHR, 1)
                                          (static_cast<uint32_t>(DP >> 3) << 17) | (static_cast<uint32_t>(TM >> 4) << 24);
             if (lane == 0) {
                 // the ring holds K_a, V_a, K_a+1, ...: step j uses V_{j-1} (stage sv) and K_j (stage sk)
-                int sk = 0, pk = 0, nq = 0, np = 0, nfix = 0;  // nq, np: a bit for each row tile's parity
+                int sk = 0, pk = 0, nq = 0, np = 0;  // nq, np: a bit for each row tile's parity
+                uint32_t fixes = 0;                  // and one for each stage
                 auto scores = [&](int t, int q, uint32_t ka) {  // S_t = Q_q K^T
                     const uint64_t qd = smem_desc_k_sw128(smem_u32(sm) + q * C::QT), kd = smem_desc_k_sw128(ka);
 #pragma unroll
@@ -1147,7 +1145,10 @@ __global__ void __launch_bounds__(TTHR, 1)
                         }
                         if (ok && j > first) {
                             ok = wait_bar(kv_full + sv, pv, err, DEVERR_PTILE_KV);
-                            if (ok && j * TKEYS > len) ok = wait_bar(v_fixed, nfix++ & 1, err, DEVERR_PTILE_FIX);
+                            if (ok && j * TKEYS > len) {
+                                ok = wait_bar(v_fixed + sv, fixes >> sv & 1, err, DEVERR_PTILE_FIX);
+                                fixes ^= 1u << sv;
+                            }
                         }
                         if (dup) {
                             const int t = (j - first + 1) & 1;  // the tile that has j - 1
@@ -1200,26 +1201,32 @@ __global__ void __launch_bounds__(TTHR, 1)
             __syncwarp();
         } else if (warp == 2) {
             // ------------------------------------------------ values behind a sequence's end
-            int n = 0, fixes = 0;  // ring entries before this unit's
+            // This warp uses every ring entry (and frees it with the issuer), so that it neither falls behind the
+            // ring nor meets a barrier whose parity is a phase before last's; the issuer waits for the fix of a
+            // stage before it frees it, so a stage's fixes do not overtake it either.
+            int stage = 0, phase = 0;
             for (int k = 0; __all_sync(0xffffffffu, take(k)); k++) {
                 const int first = works[k & 3].a, end = works[k & 3].b, len = works[k & 3].len;
-                if (end * TKEYS > len) {  // the last key tile has some
-                    const int ev = n + 2 * (end - 1 - first) + 1, sv = ev % C::STAGES;
-                    // (issued: the stage's barrier is in this phase, or past it; before, its parity would say nothing)
-                    ok = wait_bar(v_last, fixes++ & 1, err, DEVERR_PTILE_FIX);
-                    ok = __all_sync(0xffffffffu, ok && wait_bar(kv_full + sv, (ev / C::STAGES) & 1, err, DEVERR_PTILE_FIX));
-                    const int from = max(0, len - (end - 1) * TKEYS);
-                    uint8_t* v = sm + C::OFF_RING + sv * C::STAGE;
-                    if (ok)
-                        for (int i = from * 8 + lane; i < TKEYS * 8; i += 32)
+                for (int i = 2 * first; ok && i < 2 * end; i++) {  // K_a, V_a, K_a+1, ...
+                    ok = __all_sync(0xffffffffu, wait_bar(kv_full + stage, phase, err, DEVERR_PTILE_FIX));
+                    if (!ok) break;
+                    if ((i & 1) && (i + 1) / 2 * TKEYS > len) {
+                        const int from = max(0, len - i / 2 * TKEYS);
+                        uint8_t* v = sm + C::OFF_RING + stage * C::STAGE;
+                        for (int e = from * 8 + lane; e < TKEYS * 8; e += 32)
 #pragma unroll
                             for (int h = 0; h < C::HALVES; h++)
-                                *reinterpret_cast<uint4*>(v + h * C::HALF + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(v_fixed);
+                                *reinterpret_cast<uint4*>(v + h * C::HALF + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(v_fixed + stage);
+                    }
+                    if (lane == 0) mbar_arrive(kv_empty + stage);
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
-                n += 2 * (end - first);
                 __syncwarp();
                 if (lane == 0) done(k);
             }
