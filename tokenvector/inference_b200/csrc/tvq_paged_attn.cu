@@ -680,11 +680,11 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 // barrier of its own; and in-order execution of the products lets S_t(j)
 // overwrite P_t(j-1) right behind the product that reads it.
 // Bound: the two products of a tile and j (2 x 512 cycles at D = 128) wait for
-// its softmax and the softmax for them, so a softmax has to end within the
-// other tile's products: three of eight exponentials are polynomials on the FMA
-// pipe (128 x 128 of them on the special-function units alone take 1024
-// cycles, and both tiles share the units), and the product with V starts when
-// the weights of the first 64 keys are there.
+// its softmax and the softmax for them.  Its 128 x 128 exponentials take the
+// special-function units 1024 cycles, with reading, maximum, exchange and
+// writing ~1900, so the tensor cores rest in between: 45 % of their rate.
+// (Polynomials on the FMA pipe for a part of the exponentials did not help:
+// the chain through a softmax is as long, with more to issue.)
 constexpr int TM = 128, TKEYS = 128;
 constexpr int TTHR = 640;
 enum : int {
@@ -791,25 +791,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if on
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-// 2^x of both, x <= 127: 2^n p(f) with n = round(x), f = x - n in [-1/2, 1/2] and p
-// the polynomial of degree 4 whose relative error to 2^f there is the least
-// (Remez): 2.7 10^-6.  Below 2^-126 it stays there.
-__device__ __forceinline__ uint64_t exp2_pair(float x, float y) {
-    const uint64_t v = f2_pack(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
-    const uint64_t big = f2_pack(12582912.0f, 12582912.0f);  // 1.5 2^23: the sum's last bits are n
-    const uint64_t t = f2_add(v, big);
-    const uint64_t f = f2_sub(v, f2_sub(t, big));
-    uint64_t p = f2_pack(0.009570102207362652f, 0.009570102207362652f);
-    p = f2_fma(p, f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
-    p = f2_fma(p, f, f2_pack(0.240247443318367f, 0.240247443318367f));
-    p = f2_fma(p, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
-    p = f2_fma(p, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
-    float n0, n1, p0, p1;
-    f2_unpack(t, n0, n1);
-    f2_unpack(p, p0, p1);
-    return f2_pack(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23)),
-                   __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23)));
 }
 // wait_full with a code
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* err, int code) {
@@ -1092,8 +1073,9 @@ __global__ void __launch_bounds__(TTHR, 1)
         } else if (warp == 1) {
             // ------------------------------------------------ MMA issuer
             constexpr uint32_t ty = std::is_same<T, __half>::value ? 0u : 1u;
-            constexpr uint32_t idesc_s = (1u << 4) | (ty << 7) | (ty << 10) | (static_cast<uint32_t>(TKEYS >> 3) << 17) |
-                                         (static_cast<uint32_t>(TM >> 4) << 24);
+            // (bit 13 negates Q: with a negative scale the largest score is still the largest product)
+            const uint32_t idesc_s = (1u << 4) | (ty << 7) | (ty << 10) | (static_cast<uint32_t>(TKEYS >> 3) << 17) |
+                                     (static_cast<uint32_t>(TM >> 4) << 24) | (plan.negative ? 1u << 13 : 0u);
             constexpr uint32_t idesc_o = (1u << 4) | (ty << 7) | (ty << 10) | (1u << 16) |
                                          (static_cast<uint32_t>(DP >> 3) << 17) | (static_cast<uint32_t>(TM >> 4) << 24);
             if (lane == 0) {
@@ -1259,30 +1241,16 @@ __global__ void __launch_bounds__(TTHR, 1)
                 if (ok) ok = __all_sync(0xffffffffu, wait_bar(s_full + t, ns & 1, err, DEVERR_PTILE_S));
                 ns++;
                 tc_fence_after();
-                // The scores are read twice, 32 at a time, in rolled loops: unrolled code (40 KB) drove the other
-                // warps' out of the instruction cache, and a product's issue took 800 cycles for it.
+                // 64 scores do not fit a thread's registers next to what is made of them: the second 32 are read twice.
                 const int k0 = j * TKEYS + half * 64;
                 const bool edge = k0 + 63 > pmin || (a.window > 0 && k0 <= pmax - a.window);
-                auto load = [&](int c, uint32_t (&s)[32]) {
-                    tmem_ld32(s_addr + c * 32, s);
-                    tmem_ld_wait();
-                    if (plan.negative) {
+                auto hide = [&](int c, uint32_t (&s)[32]) {
+                    const int top = pos - k0 - c * 32, bot = a.window > 0 ? top - a.window : -1;  // columns in (bot, top]
 #pragma unroll
-                        for (int e = 0; e < 32; e++) s[e] ^= 0x80000000u;
-                    }
-                    if (edge) {
-                        const int top = pos - k0 - c * 32, bot = a.window > 0 ? top - a.window : -1;  // columns in (bot, top]
-#pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (e > top || e <= bot) s[e] = 0xFF800000u;  // -inf
-                    }
+                    for (int e = 0; e < 32; e++)
+                        if (e > top || e <= bot) s[e] = 0xFF800000u;  // -inf
                 };
-                // (NaN goes through: the row is then NaN)
-                float tile = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 2; c++) {
-                    uint32_t s[32];
-                    load(c, s);
+                auto most = [](const uint32_t (&s)[32]) {  // (NaN goes through: the row is then NaN)
                     float mx[4];
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
@@ -1290,9 +1258,20 @@ __global__ void __launch_bounds__(TTHR, 1)
                         mx[q] = max3(mx[q], __uint_as_float(s[q * 8 + 3]), __uint_as_float(s[q * 8 + 4]));
                         mx[q] = max3(mx[q], __uint_as_float(s[q * 8 + 5]), __uint_as_float(s[q * 8 + 6]));
                     }
-                    const float r = max3(max3(mx[0], mx[1], mx[2]), mx[3], __uint_as_float(s[7]));
-                    tile = max3(max3(tile, r, __uint_as_float(s[15])), __uint_as_float(s[23]), __uint_as_float(s[31]));
+                    mx[0] = max3(mx[0], mx[1], __uint_as_float(s[7]));
+                    mx[2] = max3(mx[2], mx[3], __uint_as_float(s[15]));
+                    return max3(max3(mx[0], mx[2], __uint_as_float(s[23])), __uint_as_float(s[31]), __uint_as_float(s[31]));
+                };
+                uint32_t s0[32], s1[32];
+                tmem_ld32(s_addr, s0);
+                tmem_ld32(s_addr + 32, s1);
+                tmem_ld_wait();
+                if (edge) {
+                    hide(0, s0);
+                    hide(1, s1);
                 }
+                const float mine = most(s0);
+                float tile = max3(mine, most(s1), mine);
                 *x_mine = tile;
                 ok = named_bar_and(pair_bar, 64, ok);
                 tile = max3(tile, *x_other, tile);
@@ -1321,33 +1300,28 @@ __global__ void __launch_bounds__(TTHR, 1)
                 uint64_t sum2[2] = {0ull, 0ull};
                 // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
                 // rounding of the result; l sums them unrounded
-#pragma unroll 1
-                for (int c = 0; c < 2; c++) {
-                    uint32_t s[32], p[16];
-                    load(c, s);  // (the weights' columns lie within the scores read so far)
+                auto weigh = [&](int c, const uint32_t (&s)[32]) {  // (their columns lie within the scores read so far)
+                    uint32_t p[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale22, base2);
                         float y, z;
-                        f2_unpack(x, y, z);
-                        if (e % 4 == 3) {
-                            const uint64_t q = exp2_pair(y, z);
-                            f2_unpack(q, y, z);
-                            sum2[e & 1] = f2_add(sum2[e & 1], q);
-                        } else {
-                            y = ex2(y);
-                            z = ex2(z);
-                            sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(y, z));
-                        }
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale22, base2), y, z);
+                        y = ex2(y);
+                        z = ex2(z);
+                        sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(y, z));
                         p[e] = pack2<T>(y, z);
                     }
                     tmem_st16(s_addr + c * 16, p);
-                }
+                };
+                tmem_ld32(s_addr + 32, s1);
+                weigh(0, s0);
+                tmem_ld_wait();
+                if (edge) hide(1, s1);
+                weigh(1, s1);
                 float sa, sb, sc, sd;
                 f2_unpack(sum2[0], sa, sb);
                 f2_unpack(sum2[1], sc, sd);
                 l += (sa + sb) + (sc + sd);
-                if (m == -INFINITY) l = 0.0f;  // no key yet (the polynomial's weights of masked ones are 2^-126, not 0)
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
