@@ -1,6 +1,7 @@
-"""Build libtvq.so in-tree with nvcc for sm_100a (B200).
+"""Build libtvq.so in-tree with nvcc for sm_100a (B200), and beside it
+_tvq_torch.so, the decoding operators on torch tensors (csrc/tvq_torch.cpp).
 
-The shared library lands next to this file so that it travels with the
+The shared libraries land next to this file so that they travel with the
 repository snapshot; nothing is installed into site-packages.  Objects are
 compiled in parallel and rebuilt only when a source or header is newer.
 """
@@ -18,6 +19,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OBJDIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libtvq.so")
+TORCH_SRC = os.path.join(CSRC, "tvq_torch.cpp")
+TORCH_LIB = os.path.join(HERE, "_tvq_torch.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -51,6 +54,31 @@ def _compile(nvcc, src, obj, verbose):
     return r.stderr
 
 
+def _build_torch(force: bool) -> None:
+    """_tvq_torch.so: g++ against torch's headers, linked to libtvq.so beside it."""
+    newest = max(os.path.getmtime(TORCH_SRC), os.path.getmtime(os.path.join(INCLUDE, "tvq.h")))
+    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= newest:
+        return
+    import sysconfig
+
+    import torch
+    tmp = TORCH_LIB + ".tmp"
+    torch_dir = os.path.dirname(torch.__file__)
+    lib_dir = os.path.join(torch_dir, "lib")
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_tvq_torch",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I", INCLUDE,
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include")]
+    for d in ("include", "include/torch/csrc/api/include"):
+        cmd += ["-isystem", os.path.join(torch_dir, d)]
+    cmd += [TORCH_SRC, "-o", tmp, "-L", HERE, "-l:libtvq.so", "-Wl,-rpath,$ORIGIN", "-L", lib_dir, "-lc10", "-lc10_cuda",
+            "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("building _tvq_torch.so failed:\n%s%s" % (r.stdout, r.stderr))
+    os.replace(tmp, TORCH_LIB)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     nvcc = _nvcc()
     os.makedirs(OBJDIR, exist_ok=True)
@@ -77,6 +105,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError("link failed:\n%s%s" % (r.stdout, r.stderr))
         os.replace(tmp, LIB)
+    _build_torch(force)
     return LIB
 
 
