@@ -706,12 +706,16 @@ struct TileCfg {
     static constexpr int OFF_MISC = OFF_X + 2 * 2 * 128 * 4;  // int64 at, int seq, tmem
     static constexpr int SMEM = OFF_MISC + 16;
     static constexpr int64_t SLOT = 2 * TM * (DP * 4 + 8);
-    static constexpr uint32_t COL_S = 0, COL_O = 256, COLS = DP == 128 ? 512 : 512;
+    static constexpr uint32_t COL_S = 0, COL_O = 256, COLS = 512;
 };
 
+struct Begun {
+    int rows, row0, n, hk;  // rows of the unit (0: none); the sequence's; the kv head
+    int unit, last, pad[2];  // which unit of the sequence; the last piece that has a part of it
+};
 struct TilePlan {
     uint8_t* parts;  // [grid][2] slots: f32 [256][DP], then float2 (m, l) [256]
-    int4* begun;     // [grid]: {s, hk, unit, last piece} of the unit that a piece begins and does not end (s -1: none)
+    struct Begun* begun;  // [grid]: the unit that a piece begins and does not end
     int tokens;      // of a tile: 128 / group
     int box, box_halves, by_value;  // as RowsPlan's, KT = 128
     float scale2;    // log2(e) |scale|, not 0
@@ -860,6 +864,7 @@ __global__ void __launch_bounds__(TTHR, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
     griddep_wait();
+    griddep_launch();  // the join's CTAs take the place of this kernel's as these end
 
     // ---- the piece of the line of key tiles
     auto weight = [&](int s) -> int64_t {  // of one kv head
@@ -929,7 +934,7 @@ __global__ void __launch_bounds__(TTHR, 1)
         if (warp == 3) {
             // ------------------------------------------------ the walk
             if (lane == 0) {
-                int4 begun = make_int4(-1, 0, 0, 0);
+                Begun begun{};
                 int s = 0, hk = 0, u = 0, skip = 0, units = 0;
                 int64_t left = stop - begin;
                 Seq q{0, 0, 0};
@@ -982,7 +987,8 @@ __global__ void __launch_bounds__(TTHR, 1)
                             o.hi[1] = o.b;
                         }
                         if (o.begins && !o.whole)
-                            begun = make_int4(s, hk, u, static_cast<int>((stop - left + w.e - w.f - 1) / per));
+                            begun = Begun{w.cnt[0] + w.cnt[1], q.row0, q.n, hk, u,
+                                          static_cast<int>((stop - left + w.e - w.f - 1) / per)};
                         left -= o.b - o.a;
                         skip = 0;
                         if (left > 0 && ++u == units) {
@@ -1246,9 +1252,12 @@ __global__ void __launch_bounds__(TTHR, 1)
                 const bool edge = k0 + 63 > pmin || (a.window > 0 && k0 <= pmax - a.window);
                 auto hide = [&](int c, uint32_t (&s)[32]) {
                     const int top = pos - k0 - c * 32, bot = a.window > 0 ? top - a.window : -1;  // columns in (bot, top]
+                    uint32_t seen = top >= 31 ? 0xFFFFFFFFu : top < 0 ? 0u : (2u << top) - 1;
+                    if (bot >= 0) seen &= bot >= 31 ? 0u : ~((2u << bot) - 1);
+                    if (__all_sync(0xffffffffu, seen == 0xFFFFFFFFu)) return;
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        if (e > top || e <= bot) s[e] = 0xFF800000u;  // -inf
+                        if (!(seen >> e & 1)) s[e] = 0xFF800000u;  // -inf
                 };
                 auto most = [](const uint32_t (&s)[32]) {  // (NaN goes through: the row is then NaN)
                     float mx[4];
@@ -1417,44 +1426,62 @@ __global__ void __launch_bounds__(TTHR, 1)
     if (warp == 2) tmem_dealloc(tmem, C::COLS);
 }
 
-// The rows of units that lie in several pieces, a warp each: as attn_join_kernel.
+// The rows of units that lie in several pieces: as attn_join_kernel.  DP / 4
+// lanes have a row, 16 bytes each, and four rows of D = 64 (two of 128) go at once,
+// so that all rows of 148 cut units are under way together.
+constexpr int TJ_ROWS = 32;  // rows of a CTA
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) attn_tile_join_kernel(const PagedAttnArgs a, const TilePlan plan) {
     using C = TileCfg<DP>;
-    constexpr int E = DP / 32;
+    constexpr int LANES = DP / 4, SIDE = 256 / LANES, R = TJ_ROWS / SIDE;
     griddep_wait();
-    const int4 b = plan.begun[blockIdx.x];
-    if (b.x < 0) return;
-    const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int group = a.q_heads / a.c.kv_heads;
-    const Seq q = load_seq(a.c, b.x);
-    const int t = row >> 7, r = row & 127, i = r / group, gi = r - i * group;
-    const int tok = (2 * b.z + t) * plan.tokens + i;
-    if (i >= plan.tokens || tok >= q.n) return;
-    float m = -INFINITY, sum = 0.0f, o[E];
+    const int4 b0 = *reinterpret_cast<const int4*>(plan.begun + blockIdx.x);
+    const int2 b1 = *reinterpret_cast<const int2*>(&plan.begun[blockIdx.x].unit);
+    const int group = a.q_heads / a.c.kv_heads, hk = b0.w, unit = b1.x, last = b1.y;
+    const int x = threadIdx.x % LANES, row0 = blockIdx.y * TJ_ROWS + threadIdx.x / LANES;
+    if (b0.x == 0) return;
+    float m[R], sum[R], o[R][4];
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.0f;
-#pragma unroll 4
-    for (int c = blockIdx.x; c <= b.w; c++) {
-        const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == static_cast<int>(blockIdx.x) ? 1 : 0)) * C::SLOT;
-        const float2 ml = *reinterpret_cast<const float2*>(part + 2 * TM * DP * 4 + row * 8);
-        float x[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) x[e] = reinterpret_cast<const float*>(part)[row * DP + e * 32 + lane];
-        const float m2 = fmaxf(m, ml.x), base = m2 == -INFINITY ? 0.0f : m2;
-        const float f = ex2(m - base), w = ex2(ml.x - base);
-        m = m2;
-        sum = sum * f + ml.y * w;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = ml.x == -INFINITY ? o[e] : o[e] * f + x[e] * w;  // (x is not written then)
+    for (int i = 0; i < R; i++) {
+        m[i] = -INFINITY;
+        sum[i] = 0.0f;
+        for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
     }
-    const int64_t at = static_cast<int64_t>(q.row0 + tok) * a.q_heads + b.y * group + gi;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* out = static_cast<T*>(a.out) + at * a.c.dim;
+    for (int c = blockIdx.x; c <= last; c++) {
+        const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == static_cast<int>(blockIdx.x) ? 1 : 0)) * C::SLOT;
+        float2 ml[R];
+        float4 y[R];
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        if (e * 32 + lane < a.c.dim) out[e * 32 + lane] = from_f32<T>(o[e] * inv);
-    if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+        for (int i = 0; i < R; i++) {
+            const int row = row0 + i * SIDE;
+            ml[i] = *reinterpret_cast<const float2*>(part + 2 * TM * DP * 4 + row * 8);
+            y[i] = *reinterpret_cast<const float4*>(part + (row * DP + x * 4) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const float m2 = fmaxf(m[i], ml[i].x), base = m2 == -INFINITY ? 0.0f : m2;
+            const float f = ex2(m[i] - base), w = ex2(ml[i].x - base);
+            m[i] = m2;
+            if (ml[i].x == -INFINITY) continue;  // (y is not written then)
+            sum[i] = sum[i] * f + ml[i].y * w;
+            o[i][0] = o[i][0] * f + y[i].x * w;
+            o[i][1] = o[i][1] * f + y[i].y * w;
+            o[i][2] = o[i][2] * f + y[i].z * w;
+            o[i][3] = o[i][3] * f + y[i].w * w;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int row = row0 + i * SIDE, r = row & (TM - 1), ri = r / group;
+        const int tok = (2 * unit + (row >> 7)) * plan.tokens + ri;
+        if (ri >= plan.tokens || tok >= b0.z) continue;
+        const int64_t at = static_cast<int64_t>(b0.y + tok) * a.q_heads + hk * group + (r - ri * group);
+        const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
+        if (x * 4 < a.c.dim)
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.c.dim + x * 4) =
+                make_uint2(pack2<T>(o[i][0] * inv, o[i][1] * inv), pack2<T>(o[i][2] * inv, o[i][3] * inv));
+        if (x == 0 && a.lse) a.lse[at] = sum[i] == 0.0f ? -INFINITY : (m[i] + log2f(sum[i])) * 0.6931471805599453f;
+    }
 }
 
 }  // namespace
@@ -1491,7 +1518,7 @@ struct TileSpace {
 TileSpace tile_space(const PagedAttnArgs& a, int sms) {
     TileSpace w;
     if (few_rows(a)) return w;
-    w.begun = up256(16ll * sms);
+    w.begun = up256(sizeof(Begun) * sms);
     w.bytes = w.begun + 2ll * sms * (a.c.dim > 64 ? TileCfg<128>::SLOT : TileCfg<64>::SLOT);
     return w;
 }
@@ -1564,7 +1591,7 @@ int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     const int group = a.q_heads / a.c.kv_heads;
     uint8_t* ws = static_cast<uint8_t*>(a.ws);
     TilePlan plan;
-    plan.begun = reinterpret_cast<int4*>(ws);
+    plan.begun = reinterpret_cast<Begun*>(ws);
     plan.parts = ws + tile_space(a, ds->sm_count).begun;
     plan.tokens = TM / group;
     plan.box = std::min(a.c.page, TKEYS);
@@ -1587,7 +1614,7 @@ int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     rc = launch_pdl(attn_tile_kernel<T, DP>, dim3(ds->sm_count), dim3(TTHR), C::SMEM, st, tmQ, tmK, tmV, a, plan,
                     ds->d_error);
     if (rc) return rc;
-    return launch_pdl(attn_tile_join_kernel<T, DP>, dim3(ds->sm_count, 2 * TM / 8), dim3(256), 0, st, a, plan);
+    return launch_pdl(attn_tile_join_kernel<T, DP>, dim3(ds->sm_count, 2 * TM / TJ_ROWS), dim3(256), 0, st, a, plan);
 }
 
 // Steps (no sequence has more than 16 rows): the rows kernel, which waits for
