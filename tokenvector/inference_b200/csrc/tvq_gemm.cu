@@ -1531,9 +1531,11 @@ int make_tma_16bit(CUtensorMap* map, const void* ptr, int rank, const uint64_t* 
         b[i] = box[i];
         if (i > 0) st[i - 1] = dims[i] > 1 ? strides[i - 1] : 16;
     }
+    // (128-byte lines: the line beside one is another head's where a token's heads lie side by side, and with
+    // 256 a batch's tokens read 20 % more than they use: 128 us instead of 101 for 128 x 25 heads of 64)
     const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
                                 const_cast<void*>(ptr), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     TVQ_CHECK(r == CUDA_SUCCESS, TVQ_ERR_UNSUPPORTED,
               "strides that a tensor map cannot hold (cuTensorMapEncodeTiled code " +
