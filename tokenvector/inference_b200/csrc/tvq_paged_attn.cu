@@ -138,6 +138,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// a / b for a >= 0, b > 0; short for what fits 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 // One sequence as both kernels see it.
 struct Seq {
     int row0;  // first packed row
@@ -218,9 +224,11 @@ __global__ void __launch_bounds__(NTHR, 1)
     uint8_t* ring = sm + mine * (C::STAGES * C::STAGE);
     const int group = a.q_heads / a.c.kv_heads;
     const int fit = MAX_ROWS / group;  // new rows of a sequence that this kernel takes
-    if (tid == 0) {
-        for (int i = 0; i < 2 * NW * C::STAGES; i++) mbar_init(reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + i, 1);
+    static_assert(2 * NW * C::STAGES <= NTHR - 32);
+    if (tid < 2 * NW * C::STAGES) {
+        mbar_init(reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + tid, 1);
         fence_barrier_init();
+    } else if (tid == NTHR - 1) {
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
@@ -261,7 +269,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     }
     total *= a.c.kv_heads;
     const int64_t pieces = static_cast<int64_t>(gridDim.x) * NW;
-    const int64_t per = max(static_cast<int64_t>(1), (total + pieces - 1) / pieces);
+    const int64_t per = max(static_cast<int64_t>(1), quotient(total + pieces - 1, pieces));
     int64_t before = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += NTHR) {
         int all = 0;
@@ -310,7 +318,7 @@ __global__ void __launch_bounds__(NTHR, 1)
         cur.q = load_seq(a.c, cur.s);
         const int64_t in_seq = begin - s_at[mine];
         const int2 t = seq_tiles<KT>(cur.q, a.window);
-        cur.hk = static_cast<int>(in_seq / (t.y - t.x));
+        cur.hk = static_cast<int>(quotient(in_seq, t.y - t.x));
         enter(cur, static_cast<int>(in_seq - static_cast<int64_t>(cur.hk) * (t.y - t.x)));
     }
 
@@ -537,7 +545,7 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (begins && lane == 0) {
             const int64_t at0 = stop - cur.left;  // the pair's first tile in the line
             plan.spans[static_cast<int64_t>(cur.s) * a.c.kv_heads + cur.hk] =
-                make_int2(piece, static_cast<int>((at0 + cur.all.y - cur.all.x - 1) / per));
+                make_int2(piece, static_cast<int>(quotient(at0 + cur.all.y - cur.all.x - 1, per)));
         }
         uint8_t* part = plan.parts + (static_cast<int64_t>(piece) * 2 + (begins ? 1 : 0)) * plan.slot;
 #pragma unroll
@@ -576,8 +584,8 @@ __global__ void __launch_bounds__(NTHR, 1)
 // are in L2), so a row's parts are spread over as many warps as there are.
 constexpr int JW = 8;
 template <typename T, int DP, int SHARE>
-__global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs a, const RowsPlan plan) {
-    constexpr int E = DP / 32, ROWS = JW / SHARE;
+__global__ void __launch_bounds__(JW * 32, 6) attn_join_kernel(const PagedAttnArgs a, const RowsPlan plan) {
+    constexpr int E = DP / 32, ROWS = JW / SHARE, AHEAD = DP == 128 ? 2 : 4;
     __shared__ float s_o[JW][DP];
     __shared__ float2 s_ml[JW];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -599,19 +607,36 @@ __global__ void __launch_bounds__(JW * 32) attn_join_kernel(const PagedAttnArgs 
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] = 0.0f;
         if (act)
-#pragma unroll 4
-            for (int c = span.x + warp % SHARE; c <= span.y; c += SHARE) {
-                const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == span.x ? 1 : 0)) * plan.slot;
-                const float2 ml = *reinterpret_cast<const float2*>(part + (static_cast<int64_t>(plan.rows_cap) * DP * 4 + r * 8));
-                float x[E];
+            for (int c0 = span.x + warp % SHARE; c0 <= span.y; c0 += SHARE * AHEAD) {
+                float2 ml[AHEAD];
+                float x[AHEAD][E];
 #pragma unroll
-                for (int e = 0; e < E; e++) x[e] = reinterpret_cast<const float*>(part)[r * DP + e * 32 + lane];
-                const float t2 = fmaxf(t, ml.x), base = t2 == -INFINITY ? 0.0f : t2;
-                const float f = ex2(t - base), w = ex2(ml.x - base);
+                for (int i = 0; i < AHEAD; i++) {  // (asked for together: one after the other, each took ~800 cycles)
+                    const int c = c0 + i * SHARE;
+                    ml[i] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[i][e] = 0.0f;
+                    if (c > span.y) continue;
+                    const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == span.x ? 1 : 0)) * plan.slot;
+                    ml[i] = *reinterpret_cast<const float2*>(part + (static_cast<int64_t>(plan.rows_cap) * DP * 4 + r * 8));
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[i][e] = reinterpret_cast<const float*>(part)[r * DP + e * 32 + lane];
+                }
+                float t2 = t;
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) t2 = fmaxf(t2, ml[i].x);
+                const float base = t2 == -INFINITY ? 0.0f : t2, f = ex2(t - base);
                 t = t2;
-                sum = sum * f + ml.y * w;
+                sum *= f;
 #pragma unroll
-                for (int e = 0; e < E; e++) o[e] = o[e] * f + x[e] * w;
+                for (int e = 0; e < E; e++) o[e] *= f;
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) {
+                    const float w = ex2(ml[i].x - base);
+                    sum += ml[i].y * w;
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] += x[i][e] * w;
+                }
             }
         if constexpr (SHARE > 1) {
             if (lane == 0) s_ml[warp] = make_float2(t, sum);
@@ -701,7 +726,8 @@ struct TileCfg {
     static constexpr int STAGES = 163840 / STAGE;        // 5 or 10
     static constexpr int OFF_RING = 2 * QT;
     static constexpr int OFF_BAR = OFF_RING + STAGES * STAGE;
-    static constexpr int OFF_WORK = OFF_BAR + (3 * STAGES + 24) * 8;  // Work[4]
+    static constexpr int BARS = 3 * STAGES + 23;
+    static constexpr int OFF_WORK = OFF_BAR + (BARS + 1) * 8;  // Work[4]
     static constexpr int OFF_X = OFF_WORK + 4 * 96;      // float [2][2][128]: what the halves of a row tell each other
     static constexpr int OFF_MISC = OFF_X + 2 * 2 * 128 * 4;  // int64 at, int seq, tmem
     static constexpr int SMEM = OFF_MISC + 16;
@@ -829,28 +855,16 @@ __global__ void __launch_bounds__(TTHR, 1)
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(s_seq + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.q_heads / a.c.kv_heads;
-    if (tid == 0) {
-        for (int i = 0; i < C::STAGES; i++) {
-            mbar_init(kv_full + i, 1);
-            mbar_init(kv_empty + i, 2);  // the issuer and the fixing warp
-            mbar_init(v_fixed + i, 1);
-        }
-        for (int t = 0; t < 2; t++) {
-            mbar_init(q_full + t, 1);
-            mbar_init(q_empty + t, 1);
-            mbar_init(s_full + t, 1);
-            mbar_init(p_full + t, 4);
-            mbar_init(p_half + t, 4);
-            mbar_init(o_full + t, 1);
-        }
-        mbar_init(b_ready, 8);
-        mbar_init(b_free, 8);
-        mbar_init(drain, 1);
-        for (int i = 0; i < 4; i++) {
-            mbar_init(w_full + i, 1);
-            mbar_init(w_empty + i, 19);  // TMA, MMA, fixing and sixteen softmax warps
-        }
+    if (tid < C::BARS) {
+        uint64_t* bar = kv_full + tid;
+        int users = 1;
+        if (bar >= kv_empty && bar < q_full) users = 2;                                          // the issuer and the fixing warp
+        if ((bar >= p_full && bar < o_full) || (bar >= p_half && bar < b_ready)) users = 4;      // a tile's warps with half the keys
+        if (bar == b_ready || bar == b_free) users = 8;                                          // a tile's warps
+        if (bar >= w_empty && bar < p_half) users = 19;  // TMA, MMA, fixing and sixteen softmax warps
+        mbar_init(bar, users);
         fence_barrier_init();
+    } else if (tid == TTHR - 1) {
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
@@ -903,7 +917,7 @@ __global__ void __launch_bounds__(TTHR, 1)
         total += all;
     }
     total *= a.c.kv_heads;
-    const int64_t per = max(static_cast<int64_t>(1), (total + gridDim.x - 1) / gridDim.x);
+    const int64_t per = max(static_cast<int64_t>(1), quotient(total + gridDim.x - 1, gridDim.x));
     const int64_t begin = per * blockIdx.x, stop = min(total, begin + per);
     int64_t before = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += TTHR) {
@@ -947,7 +961,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                         const Unit w = make_unit(q, i, plan.tokens, a.window);
                         one += w.e - w.f;
                     }
-                    hk = static_cast<int>(in / one);
+                    hk = static_cast<int>(quotient(in, one));
                     in -= hk * one;
                     for (u = 0; u < units; u++) {
                         const Unit w = make_unit(q, u, plan.tokens, a.window);
@@ -988,7 +1002,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                         }
                         if (o.begins && !o.whole)
                             begun = Begun{w.cnt[0] + w.cnt[1], q.row0, q.n, hk, u,
-                                          static_cast<int>((stop - left + w.e - w.f - 1) / per)};
+                                          static_cast<int>(quotient(stop - left + w.e - w.f - 1, per))};
                         left -= o.b - o.a;
                         skip = 0;
                         if (left > 0 && ++u == units) {
@@ -1427,42 +1441,52 @@ __global__ void __launch_bounds__(TTHR, 1)
 }
 
 // The rows of units that lie in several pieces: as attn_join_kernel.  DP / 4
-// lanes have a row, 16 bytes each, and four rows of D = 64 (two of 128) go at once,
-// so that all rows of 148 cut units are under way together.
-constexpr int TJ_ROWS = 32;  // rows of a CTA
+// lanes have a row, 16 bytes each, and two rows go at once, so that hardly more
+// CTAs come than are under way together (a warp a row: 7.5 us for 148 units
+// cut in two, D = 64, of which this leaves ~3).
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) attn_tile_join_kernel(const PagedAttnArgs a, const TilePlan plan) {
     using C = TileCfg<DP>;
-    constexpr int LANES = DP / 4, SIDE = 256 / LANES, R = TJ_ROWS / SIDE;
+    constexpr int LANES = DP / 4, SIDE = 256 / LANES, R = 2;
     griddep_wait();
     const int4 b0 = *reinterpret_cast<const int4*>(plan.begun + blockIdx.x);
     const int2 b1 = *reinterpret_cast<const int2*>(&plan.begun[blockIdx.x].unit);
     const int group = a.q_heads / a.c.kv_heads, hk = b0.w, unit = b1.x, last = b1.y;
-    const int x = threadIdx.x % LANES, row0 = blockIdx.y * TJ_ROWS + threadIdx.x / LANES;
+    const int x = threadIdx.x % LANES, row0 = blockIdx.y * SIDE * R + threadIdx.x / LANES;
     if (b0.x == 0) return;
+    int64_t at[R];  // the rows' places in out (below 0: none)
     float m[R], sum[R], o[R][4];
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < R; i++) {
+        const int row = row0 + i * SIDE, r = row & (TM - 1), ri = r / group;
+        const int tok = (2 * unit + (row >> 7)) * plan.tokens + ri;
+        at[i] = ri < plan.tokens && tok < b0.z ? static_cast<int64_t>(b0.y + tok) * a.q_heads + hk * group + (r - ri * group) : -1;
+        any |= at[i] >= 0;
         m[i] = -INFINITY;
         sum[i] = 0.0f;
         for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
     }
+    if (!any) return;
+#pragma unroll 2
     for (int c = blockIdx.x; c <= last; c++) {
         const uint8_t* part = plan.parts + (static_cast<int64_t>(c) * 2 + (c == static_cast<int>(blockIdx.x) ? 1 : 0)) * C::SLOT;
         float2 ml[R];
         float4 y[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            if (at[i] < 0) continue;
             const int row = row0 + i * SIDE;
             ml[i] = *reinterpret_cast<const float2*>(part + 2 * TM * DP * 4 + row * 8);
             y[i] = *reinterpret_cast<const float4*>(part + (row * DP + x * 4) * 4);
         }
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            const float m2 = fmaxf(m[i], ml[i].x), base = m2 == -INFINITY ? 0.0f : m2;
-            const float f = ex2(m[i] - base), w = ex2(ml[i].x - base);
-            m[i] = m2;
             if (ml[i].x == -INFINITY) continue;  // (y is not written then)
+            const float m2 = fmaxf(m[i], ml[i].x);
+            const float f = ex2(m[i] - m2), w = ex2(ml[i].x - m2);
+            m[i] = m2;
             sum[i] = sum[i] * f + ml[i].y * w;
             o[i][0] = o[i][0] * f + y[i].x * w;
             o[i][1] = o[i][1] * f + y[i].y * w;
@@ -1472,15 +1496,12 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const PagedAttnArgs
     }
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        const int row = row0 + i * SIDE, r = row & (TM - 1), ri = r / group;
-        const int tok = (2 * unit + (row >> 7)) * plan.tokens + ri;
-        if (ri >= plan.tokens || tok >= b0.z) continue;
-        const int64_t at = static_cast<int64_t>(b0.y + tok) * a.q_heads + hk * group + (r - ri * group);
+        if (at[i] < 0) continue;
         const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
         if (x * 4 < a.c.dim)
-            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.c.dim + x * 4) =
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at[i] * a.c.dim + x * 4) =
                 make_uint2(pack2<T>(o[i][0] * inv, o[i][1] * inv), pack2<T>(o[i][2] * inv, o[i][3] * inv));
-        if (x == 0 && a.lse) a.lse[at] = sum[i] == 0.0f ? -INFINITY : (m[i] + log2f(sum[i])) * 0.6931471805599453f;
+        if (x == 0 && a.lse) a.lse[at[i]] = sum[i] == 0.0f ? -INFINITY : (m[i] + log2f(sum[i])) * 0.6931471805599453f;
     }
 }
 
@@ -1614,7 +1635,7 @@ int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     rc = launch_pdl(attn_tile_kernel<T, DP>, dim3(ds->sm_count), dim3(TTHR), C::SMEM, st, tmQ, tmK, tmV, a, plan,
                     ds->d_error);
     if (rc) return rc;
-    return launch_pdl(attn_tile_join_kernel<T, DP>, dim3(ds->sm_count, 2 * TM / TJ_ROWS), dim3(256), 0, st, a, plan);
+    return launch_pdl(attn_tile_join_kernel<T, DP>, dim3(ds->sm_count, DP / 8), dim3(256), 0, st, a, plan);
 }
 
 // Steps (no sequence has more than 16 rows): the rows kernel, which waits for
