@@ -740,7 +740,7 @@ struct Begun {
     int unit, last, pad[2];  // which unit of the sequence; the last piece that has a part of it
 };
 struct TilePlan {
-    uint8_t* parts;  // [grid][2] slots: f32 [256][DP], then float2 (m, l) [256]
+    uint8_t* parts;  // [grid][2] slots: float4 [DP / 4][256 rows] (a warp's rows side by side), then float2 (m, l) [256]
     struct Begun* begun;  // [grid]: the unit that a piece begins and does not end
     int tokens;      // of a tile: 128 / group
     int box, box_halves, by_value;  // as RowsPlan's, KT = 128
@@ -1410,9 +1410,9 @@ __global__ void __launch_bounds__(TTHR, 1)
                                            pack2<T>(y[e * 8 + 4], y[e * 8 + 5]), pack2<T>(y[e * 8 + 6], y[e * 8 + 7]));
                         }
                     } else {
-                        float4* out = reinterpret_cast<float4*>(part + ((t * TM + row) * DP + c * 16) * 4);
+                        float4* out = reinterpret_cast<float4*>(part) + c * 4 * (2 * TM) + t * TM + row;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) out[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+                        for (int e = 0; e < 4; e++) out[e * 2 * TM] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
                     }
                 }
                 tc_fence_before();
@@ -1452,7 +1452,9 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const PagedAttnArgs
     const int4 b0 = *reinterpret_cast<const int4*>(plan.begun + blockIdx.x);
     const int2 b1 = *reinterpret_cast<const int2*>(&plan.begun[blockIdx.x].unit);
     const int group = a.q_heads / a.c.kv_heads, hk = b0.w, unit = b1.x, last = b1.y;
-    const int x = threadIdx.x % LANES, row0 = blockIdx.y * SIDE * R + threadIdx.x / LANES;
+    // a warp: eight rows, four float4 of each
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int x = warp % (LANES / 4) * 4 + (lane >> 3), row0 = blockIdx.y * SIDE * R + warp / (LANES / 4) * 8 + (lane & 7);
     if (b0.x == 0) return;
     int64_t at[R];  // the rows' places in out (below 0: none)
     float m[R], sum[R], o[R][4];
@@ -1479,7 +1481,7 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const PagedAttnArgs
             if (at[i] < 0) continue;
             const int row = row0 + i * SIDE;
             ml[i] = *reinterpret_cast<const float2*>(part + 2 * TM * DP * 4 + row * 8);
-            y[i] = *reinterpret_cast<const float4*>(part + (row * DP + x * 4) * 4);
+            y[i] = reinterpret_cast<const float4*>(part)[x * 2 * TM + row];
         }
 #pragma unroll
         for (int i = 0; i < R; i++) {
