@@ -1386,6 +1386,9 @@ __global__ void __launch_bounds__(TTHR, 1)
             if (lo < hi && !(dup && t == 1)) {
                 const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
                 const float ga = fa * inv, gb = fb * inv;
+                const int odd = lane & 1;
+                const int64_t own = valid ? at : -1, other = __shfl_xor_sync(0xffffffffu, own, 1);
+                const int64_t at_even = odd ? other : own, at_odd = odd ? own : other;
 #pragma unroll 1
                 for (int c = half * (DP / 32); c < (half + 1) * (DP / 32); c++) {
                     uint32_t o[16], ob[16];
@@ -1399,17 +1402,23 @@ __global__ void __launch_bounds__(TTHR, 1)
                         y[e] = __uint_as_float(o[e]) * ga;
                         if (both) y[e] = fmaf(__uint_as_float(ob[e]), gb, y[e]);
                     }
-                    if (!valid) continue;
                     if (whole) {
-                        T* out = static_cast<T*>(a.out) + at * a.c.dim + c * 16;
+                        // two lanes write the 32 bytes of a row, then those of the other's (16 bytes a row and store
+                        // cost the same as 32)
+                        uint32_t u[8];
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            if (c * 16 + e * 8 >= a.c.dim) continue;
-                            *reinterpret_cast<uint4*>(out + e * 8) =
-                                make_uint4(pack2<T>(y[e * 8], y[e * 8 + 1]), pack2<T>(y[e * 8 + 2], y[e * 8 + 3]),
-                                           pack2<T>(y[e * 8 + 4], y[e * 8 + 5]), pack2<T>(y[e * 8 + 6], y[e * 8 + 7]));
+                        for (int e = 0; e < 8; e++) u[e] = pack2<T>(y[2 * e], y[2 * e + 1]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? u[e] : u[4 + e], 1);
+                            if (odd) u[e] = got;  // row of the even lane, then the own one
+                            else u[4 + e] = got;  // the own row, then the odd lane's
                         }
-                    } else {
+                        if (c * 16 + odd * 8 >= a.c.dim) continue;
+                        T* out = static_cast<T*>(a.out) + c * 16 + odd * 8;
+                        if (at_even >= 0) *reinterpret_cast<uint4*>(out + at_even * a.c.dim) = make_uint4(u[0], u[1], u[2], u[3]);
+                        if (at_odd >= 0) *reinterpret_cast<uint4*>(out + at_odd * a.c.dim) = make_uint4(u[4], u[5], u[6], u[7]);
+                    } else if (valid) {
                         float4* out = reinterpret_cast<float4*>(part) + c * 4 * (2 * TM) + t * TM + row;
 #pragma unroll
                         for (int e = 0; e < 4; e++) out[e * 2 * TM] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
