@@ -289,7 +289,9 @@ __global__ void __launch_bounds__(SLT) select_slice_kernel(const BeamSelectArgs 
 // its place in the beam's list.
 struct Place {
     uint64_t hi, lo;
-    __device__ bool above(const Place& o) const { return hi > o.hi || (hi == o.hi && lo > o.lo); }
+    __device__ int above(const Place& o) const {  // (without branches: with them a comparison took ~190 cycles)
+        return static_cast<int>(hi > o.hi) | (static_cast<int>(hi == o.hi) & static_cast<int>(lo > o.lo));
+    }
 };
 
 // One request: the `keep` best of its beams' slices' lists.  (A candidate that
@@ -335,17 +337,20 @@ __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a
         }
     }
     __syncthreads();
+    // (quotients of numbers below 2^22 by way of the reciprocal: right, and a tenth of the division's code)
+    const float by_slices = 1.0f / slices, by_keep = 1.0f / a.keep;
     auto place = [&](uint64_t key, int list) {
-        const int w = list / slices;
+        const int w = static_cast<int>((list + 0.5f) * by_slices);
         float total = s_score[w] + ((key_value(key) - s_max[w]) - s_z[w]);
         if (total != total) total = -INFINITY;
         return Place{order_key(total, w), key};
     };
-    auto rank_of = [](const Place* set, int n, const Place& p) {
+    // a warp's lanes compare p with all
+    auto rank_of = [&](const Place* set, int n, const Place& p) {
         int rank = 0;
-#pragma unroll 4
-        for (int i = 0; i < n; i++) rank += set[i].above(p);
-        return rank;
+#pragma unroll 1
+        for (int i = lane; i < n; i += 32) rank += set[i].above(p);
+        return __reduce_add_sync(0xffffffffu, rank);
     };
     Place top{0, 0};
     if (tid < lists) top = place(head, tid);
@@ -356,7 +361,11 @@ __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a
     best[tid] = top;
     __syncthreads();
     const int threads = min(lists, ST);
-    if (tid < threads && rank_of(best, threads, top) == a.keep - 1) s_bar = top;
+#pragma unroll 1
+    for (int i = warp; i < threads; i += ST / 32) {
+        const Place p = best[i];
+        if (rank_of(best, threads, p) == a.keep - 1 && lane == 0) s_bar = p;
+    }
     __syncthreads();
     if (lists > ST) {  // the bar among all heads that reach the one among the threads'
         const Place first = s_bar;
@@ -366,13 +375,16 @@ __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a
         }
         __syncthreads();
         const int n = s_n[1];
-        for (int i = tid; i < n; i += ST)
-            if (rank_of(heads, n, heads[i]) == a.keep - 1) s_bar = heads[i];
+#pragma unroll 1
+        for (int i = warp; i < n; i += ST / 32) {
+            const Place p = heads[i];
+            if (rank_of(heads, n, p) == a.keep - 1 && lane == 0) s_bar = p;
+        }
         __syncthreads();
     }
     const Place bar = s_bar;
     auto collect = [&](uint64_t key, int c) {
-        const Place p = place(key, c / a.keep);
+        const Place p = place(key, static_cast<int>((c + 0.5f) * by_keep));
         if (!bar.above(p)) found[atomicAdd(&s_n[0], 1)] = p;
     };
 #pragma unroll
@@ -381,10 +393,11 @@ __global__ void __launch_bounds__(ST) select_merge_kernel(const BeamSelectArgs a
     for (int c = tid + AHEAD * ST; c < all; c += ST) collect(mine[c], c);
     __syncthreads();
     const int n = s_n[0];
-    for (int i = tid; i < n; i += ST) {
+#pragma unroll 1
+    for (int i = warp; i < n; i += ST / 32) {
         const Place p = found[i];
         const int rank = rank_of(found, n, p);
-        if (rank >= a.keep) continue;
+        if (lane != 0 || rank >= a.keep) continue;
         const int o = b * a.keep + rank;
         a.out_scores[o] = key_value(p.hi);
         a.out_tokens[o] = key_token(p.lo);
