@@ -442,10 +442,16 @@ TVQ_API int tvq_dev_paged_append(int type, int src_type, const void* k, const vo
  * {token, head}, out contiguous.  lse (or NULL) f32 [n_rows, q_heads] = ln
  * sum_j exp(scale q . k_j).  A row without keys (at a negative position): out
  * 0, lse -inf.  max_q: no sequence has more new rows (a host bound; the rows
- * of a longer one are left as they are from there on).
- * What lies in a page behind a sequence's end has no influence.  Products
- * are formed in f32; the softmax's weights are rounded to `type` before
- * they meet V (relative 2^-11 / 2^-8 each), its statistics stay f32.
+ * of a longer one are left as they are from there on).  At most 128 query
+ * heads share a kv head.
+ * What lies in a page behind a sequence's end has no influence, and pages
+ * that lie before the window of the sequence's first new row are not read
+ * (their table entries may be anything).  A NaN or
+ * infinity in a value of the sequence itself may also reach rows that do not
+ * see it (positions up to 127 before it: a tile's masked weights are zeros,
+ * and 0 x inf is NaN).  Products are summed in f32; the softmax's
+ * weights are rounded to `type` before they meet V (relative 2^-11 / 2^-8
+ * each), its statistics stay f32.  The same call gives the same bits.
  * ws: at least tvq_paged_attention_workspace bytes, 256-byte aligned, used by
  * one call at a time; nothing in it has to last from call to call. */
 TVQ_API int tvq_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t n_seq,
@@ -464,7 +470,7 @@ TVQ_API int tvq_dev_paged_attention(int type, const void* q, const int64_t* q_st
  * the lower beam, then to the place in its list.  finished (or NULL) [batch *
  * beams] bytes: a finished beam has the one continuation eos at no cost (its
  * row counts as 0 at eos, -inf elsewhere).  keep <= 64, keep <= vocab <= 2^20,
- * beams <= 64, batch * beams <= 65535.  parents: the row batch * beams is numbered within its request (0 ..
+ * beams <= 64, batch * beams <= 65535.  parents: beams of the request (0 ..
  * beams - 1).  ws as for attention, tvq_beam_select_workspace bytes. */
 TVQ_API int tvq_beam_select_workspace(int64_t batch, int64_t beams, int64_t keep, int64_t vocab, int64_t* bytes);
 TVQ_API int tvq_dev_beam_select(int type, const void* logits, int64_t stride, const float* scores,

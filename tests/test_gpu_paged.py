@@ -246,6 +246,27 @@ def test_attention_reads_no_page_outside_the_cache(new):
     hold(zero, got, lse, definition(zero))
 
 
+@pytest.mark.parametrize("page", [8, 64, 256])
+@pytest.mark.parametrize("new,ctx", [([1, 1], [1000, 77]), ([9, 2], [700, 130]), ([300, 40], [1300, 900])])
+def test_attention_reads_no_page_before_the_window(new, ctx, page):
+    """Pages that lie before every window are free for others: any entry, any values."""
+    torch = _torch()
+    clean()
+    window = 50
+    s = make(new, ctx, 4, 2, 64, page, "float16", seed=page)
+    want = definition(s, window=window)
+    table = s["table"].clone()
+    for i, (n, c) in enumerate(zip(new, ctx)):
+        for col in range(max(0, c - n - window + 1) // page):
+            old = table[i, col].long()
+            s["k"][old] = float("nan")
+            s["v"][old] = float("inf")
+            if col % 2:
+                table[i, col] = -1
+    hold(s, *attend(dict(s, table=table), max_q=max(new), window=window), want)
+    clean()
+
+
 def test_attention_without_cu_and_without_rows():
     torch = _torch()
     from tokenvector.inference_b200.generation import paged_attention

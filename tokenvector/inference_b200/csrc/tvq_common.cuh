@@ -65,9 +65,11 @@ enum : int {
 // kernel of its stream is still running: its CTAs start as the
 // predecessor's CTAs exit.  Every thread calls griddep_wait() before it reads
 // anything the predecessor writes or writes anything the predecessor reads,
-// and before it exits.  griddep_launch() (an earlier explicit trigger) is not
-// used: triggering at kernel start measured slower, since chains of waiting
-// CTAs then hold SMs.  Without the launch attribute both are no-ops.
+// and before it exits.  griddep_launch() (an earlier explicit trigger) is used
+// by the decoding operators' first kernels alone, for the short kernel that
+// joins their parts; elsewhere triggering at kernel start measured slower,
+// since chains of waiting CTAs then hold SMs.  Without the launch attribute
+// both are no-ops.
 __device__ __forceinline__ void griddep_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }

@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(NTHR, 1)
         const int x = plan.by_value ? h * 64 : 0, y = plan.by_value ? 0 : h;
         struct Window {
             int t, end, hk, page;
+            bool read;  // (a box behind the sequence's end or before all windows is zeros)
         };
         int next_t = cur.left > 0 ? cur.first : 0;
         bool more = cur.left > 0;
@@ -343,11 +344,14 @@ __global__ void __launch_bounds__(NTHR, 1)
             Window w;
             w.t = w.end = next_t;
             w.hk = cur.hk;
-            w.page = 0;
+            w.page = -1;  // outside the tensor map: zeros
+            w.read = false;
             if (!more) return w;
             w.end = min(cur.end, next_t + 8 / boxes);
             const int j = w.t * KT + sub * plan.box;
-            if (j < w.end * KT && j < cur.q.len) {
+            const int low = a.window > 0 ? cur.q.len - cur.q.n - a.window + 1 : 0;  // the first key that a row sees
+            if (j < w.end * KT && j < cur.q.len && j + plan.box > low) {
+                w.read = true;
                 const int col = j >> a.c.page_log2;
                 w.page = col < a.c.n_cols ? __ldg(a.c.table + cur.s * a.c.table_stride + col) : -1;
             }
@@ -359,9 +363,9 @@ __global__ void __launch_bounds__(NTHR, 1)
             return w;
         };
         auto checked = [&](Window w) {
-            if (static_cast<unsigned>(w.page) >= static_cast<unsigned>(a.c.n_pages)) {
+            if (w.read && static_cast<unsigned>(w.page) >= static_cast<unsigned>(a.c.n_pages)) {
                 record_error(err, DEVERR_BAD_PAGE);
-                w.page = -1;  // outside the tensor map: zeros
+                w.page = -1;
             }
             return w;
         };
@@ -1033,10 +1037,11 @@ __global__ void __launch_bounds__(TTHR, 1)
             for (int k = 0; __all_sync(0xffffffffu, take(k)); k++) {
                 const Work& w = works[k & 3];
                 const int hk = w.hk, len = w.len, end = w.b;
+                const int low = a.window > 0 ? len - w.n + w.i0[0] - a.window + 1 : 0;  // the first key that a row sees
                 const int32_t* row = a.c.table + w.s * a.c.table_stride;
                 auto look = [&](int j) {
                     const int key = j * TKEYS + b * plan.box;
-                    if (!issues || j >= end || key >= len) return 0;
+                    if (!issues || j >= end || key >= len || key + plan.box <= low) return 0;
                     const int col = key >> a.c.page_log2;
                     return col < a.c.n_cols ? __ldg(row + col) : -1;
                 };
@@ -1062,9 +1067,10 @@ __global__ void __launch_bounds__(TTHR, 1)
                         record_error(err, DEVERR_BAD_PAGE);
                         now = -1;  // outside the tensor map: zeros
                     }
-                    // (a box behind the sequence's end, of a page that is not its own, is not read either)
-                    if (j * TKEYS + b * plan.box >= len) now = -1;
-                    const int slot = (j * TKEYS + b * plan.box) & (a.c.page - 1);
+                    // (a box behind the sequence's end or before all windows is not read either)
+                    const int key = j * TKEYS + b * plan.box;
+                    if (key >= len || key + plan.box <= low) now = -1;
+                    const int slot = key & (a.c.page - 1);
                     for (int v = 0; v < 2; v++) {
                         ok = __all_sync(0xffffffffu, wait_bar(kv_empty + stage, phase, err, DEVERR_PTILE_EMPTY));
                         if (!ok) break;
