@@ -1,3 +1,4 @@
 """Decoding: a paged key/value cache, attention of new tokens over it, and beam search on the device."""
 from .beam import beam_reorder, beam_select  # noqa: F401
+from .gpt2 import GPT2Generator  # noqa: F401
 from .paged import paged_append, paged_attention  # noqa: F401
