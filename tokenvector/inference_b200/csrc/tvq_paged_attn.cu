@@ -1143,40 +1143,59 @@ __global__ void __launch_bounds__(TTHR, 1)
                     }
                     np ^= 1 << t;
                 };
+                auto fixed = [&](int sv) {  // the values of stage sv end with the sequence
+                    ok = ok && wait_bar(v_fixed + sv, fixes >> sv & 1, err, DEVERR_PTILE_FIX);
+                    fixes ^= 1u << sv;
+                };
+                auto next = [&](int& sv, int& pv) {  // behind V_{sv}: the stages of V and K
+                    umma_commit(kv_empty + sk);
+                    sv = sk + 1;
+                    pv = pk;
+                    if (sv == C::STAGES) {
+                        sv = 0;
+                        pv ^= 1;
+                    }
+                    sk = sv + 1;
+                    pk = pv;
+                    if (sk == C::STAGES) {
+                        sk = 0;
+                        pk ^= 1;
+                    }
+                };
                 for (int k = 0; take(k); k++) {
                     const Work& w = works[k & 3];
                     const int first = w.a, end = w.b, len = w.len;
                     const int lo[2] = {w.lo[0], w.lo[1]}, hi[2] = {w.hi[0], w.hi[1]};
-                    const bool dup = w.dup;
                     int sv = 0, pv = 0;
-                    for (int j = first; ok && j <= end; j++) {
-                        const uint32_t ka = smem_u32(sm) + C::OFF_RING + sk * C::STAGE;
-                        const uint32_t va = smem_u32(sm) + C::OFF_RING + sv * C::STAGE;
-                        if (j < end) ok = wait_bar(kv_full + sk, pk, err, DEVERR_PTILE_KV);
-                        if (ok && dup && j < end) {  // S_t(j) depends on nothing of j - 1, the other tile's
-                            if (j == first) {
-                                ok = wait_bar(q_full, nq & 1, err, DEVERR_PTILE_Q);
-                                nq ^= 1;
+                    if (!w.dup) {
+                        // the key tiles in the midst of both row tiles' (their last S and first PV excepted) have a loop
+                        // without questions, if they are many: the code between the products is time (441 -> 422 us for
+                        // the long chunk), but code that runs a few times costs more to fetch than it saves
+                        const int mid = max(lo[0], lo[1]) + 2, mid_end = min(hi[0], hi[1]) - 1;
+                        for (int j = first; ok && j <= end; j++) {
+                            if (j == mid && mid_end - mid >= 8) {
+                                for (; ok && j < mid_end; j++) {
+                                    const uint32_t ka = smem_u32(sm) + C::OFF_RING + sk * C::STAGE;
+                                    const uint32_t va = smem_u32(sm) + C::OFF_RING + sv * C::STAGE;
+                                    ok = wait_bar(kv_full + sk, pk, err, DEVERR_PTILE_KV) &&
+                                         wait_bar(kv_full + sv, pv, err, DEVERR_PTILE_KV);
+#pragma unroll
+                                    for (int t = 0; t < 2; t++) {
+                                        if (ok) values(t, va, false);
+                                        if (ok) scores(t, t, ka);
+                                    }
+                                    if (!ok) break;
+                                    umma_commit(kv_empty + sv);
+                                    next(sv, pv);
+                                }
+                                if (!ok) break;
                             }
-                            if (ok) {
-                                scores((j - first) & 1, 0, ka);
-                                if (j == end - 1) umma_commit(q_empty);
-                            }
-                        }
-                        if (ok && j > first) {
-                            ok = wait_bar(kv_full + sv, pv, err, DEVERR_PTILE_KV);
-                            if (ok && j * TKEYS > len) {
-                                ok = wait_bar(v_fixed + sv, fixes >> sv & 1, err, DEVERR_PTILE_FIX);
-                                fixes ^= 1u << sv;
-                            }
-                        }
-                        if (dup) {
-                            const int t = (j - first + 1) & 1;  // the tile that has j - 1
-                            if (ok && j > first) {
-                                values(t, va, j - 1 < first + 2);
-                                if (ok && j + 1 >= end) umma_commit(o_full + t);
-                            }
-                        } else {
+                            const uint32_t ka = smem_u32(sm) + C::OFF_RING + sk * C::STAGE;
+                            const uint32_t va = smem_u32(sm) + C::OFF_RING + sv * C::STAGE;
+                            if (j < end) ok = wait_bar(kv_full + sk, pk, err, DEVERR_PTILE_KV);
+                            if (ok && j > first) ok = wait_bar(kv_full + sv, pv, err, DEVERR_PTILE_KV);
+                            // (V of the last key tile, the only one that may end with the sequence)
+                            if (j == end && end * TKEYS > len) fixed(sv);
 #pragma unroll
                             for (int t = 0; t < 2; t++) {
                                 if (ok && j - 1 >= lo[t] && j - 1 < hi[t]) {
@@ -1193,23 +1212,36 @@ __global__ void __launch_bounds__(TTHR, 1)
                                     if (j == hi[t] - 1) umma_commit(q_empty + t);
                                 }
                             }
+                            if (!ok) break;
+                            if (j > first) umma_commit(kv_empty + sv);
+                            if (j < end) next(sv, pv);
                         }
-                        if (!ok) break;
-                        if (j > first) umma_commit(kv_empty + sv);
-                        if (j < end) {
-                            umma_commit(kv_empty + sk);
-                            sv = sk + 1;
-                            pv = pk;
-                            if (sv == C::STAGES) {
-                                sv = 0;
-                                pv ^= 1;
+                    } else {
+                        // key tiles a, a + 2, ... are tile A's, the others B's; S(j) depends on nothing of j - 1, the other's
+                        for (int j = first; ok && j <= end; j++) {
+                            const uint32_t va = smem_u32(sm) + C::OFF_RING + sv * C::STAGE;
+                            if (j < end) {
+                                ok = wait_bar(kv_full + sk, pk, err, DEVERR_PTILE_KV);
+                                if (ok) {
+                                    if (j == first) {
+                                        ok = wait_bar(q_full, nq & 1, err, DEVERR_PTILE_Q);
+                                        nq ^= 1;
+                                    }
+                                    if (ok) {
+                                        scores((j - first) & 1, 0, smem_u32(sm) + C::OFF_RING + sk * C::STAGE);
+                                        if (j == end - 1) umma_commit(q_empty);
+                                    }
+                                }
                             }
-                            sk = sv + 1;
-                            pk = pv;
-                            if (sk == C::STAGES) {
-                                sk = 0;
-                                pk ^= 1;
+                            if (ok && j > first) {
+                                const int t = (j - first + 1) & 1;  // the tile that has j - 1
+                                ok = wait_bar(kv_full + sv, pv, err, DEVERR_PTILE_KV);
+                                if (j * TKEYS > len) fixed(sv);
+                                if (ok) values(t, va, j - 1 < first + 2);
+                                if (ok && j + 1 >= end) umma_commit(o_full + t);
+                                if (ok) umma_commit(kv_empty + sv);
                             }
+                            if (ok && j < end) next(sv, pv);
                         }
                     }
                     done(k);
