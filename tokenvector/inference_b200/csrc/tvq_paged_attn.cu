@@ -722,8 +722,8 @@ __global__ void __launch_bounds__(JW * 32, 6) attn_join_kernel(const PagedAttnAr
 // issuer that takes whichever tile is ready, or one that starts a unit's first
 // S before the last PV of the unit before: their code comes between the
 // products, which cost the long chunk 25 % and 4 %.)
-// Measured: a chunk of 4096 tokens behind 16384, 16 heads on 4 of 128: 442 us,
-// 1088 TFLOP/s, 66 % of a large product's rate.  Nine prompts of up to 1023,
+// Measured: a chunk of 4096 tokens behind 16384, 16 heads on 4 of 128: 422 us,
+// 1139 TFLOP/s, 69 % of a large product's rate.  Nine prompts of up to 1023,
 // 12 heads of 64: 50 us, where a unit's end and the next one's first tile take
 // ~4 us beside its few tiles, and the start ~6.
 constexpr int TM = 128, TKEYS = 128;
