@@ -1308,7 +1308,8 @@ __global__ void __launch_bounds__(TTHR, 1)
             const int pos = valid ? pmin + ri : -1;
             float m = -INFINITY, l = 0.0f;  // m of the raw products
             for (int j = lo; j < hi; j += w.dup ? 2 : 1) {
-                if (ok) ok = __all_sync(0xffffffffu, wait_bar(s_full + t, ns & 1, err, DEVERR_PTILE_S));
+                if (ok) ok = wait_bar(s_full + t, ns & 1, err, DEVERR_PTILE_S);
+                __syncwarp();
                 ns++;
                 tc_fence_after();
                 // 64 scores do not fit a thread's registers next to what is made of them: the second 32 are read twice.
@@ -1346,7 +1347,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                 const float mine = most(s0);
                 float tile = max3(mine, most(s1), mine);
                 *x_mine = tile;
-                ok = named_bar_and(pair_bar, 64, ok);
+                named_bar_sync(pair_bar, 64);
                 tile = max3(tile, *x_other, tile);
                 if (tile != tile) l = tile;
                 // l == 0 and O == 0 as long as m is -inf: nothing to scale then
@@ -1406,7 +1407,7 @@ __global__ void __launch_bounds__(TTHR, 1)
             const int64_t at = static_cast<int64_t>(w.row0 + w.i0[t] + ri) * a.q_heads + w.hk * group + gi;
             named_bar_sync(pair_bar, 64);  // (the last maxima have been read)
             *x_mine = l;
-            ok = named_bar_and(pair_bar, 64, ok);
+            named_bar_sync(pair_bar, 64);
             l += *x_other;
             if (lo < hi) {
                 if (ok) ok = __all_sync(0xffffffffu, wait_bar(o_full + t, no & 1, err, DEVERR_PTILE_O));
