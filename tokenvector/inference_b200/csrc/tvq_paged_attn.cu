@@ -710,6 +710,8 @@ __global__ void __launch_bounds__(JW * 32, 6) attn_join_kernel(const PagedAttnAr
 // O stays relative to the row's first maximum until the running one exceeds it
 // by 2^8 (then O and l are scaled by the softmax warps): weights stay below
 // 2^8, exact enough in either 16-bit type, and nearly no tile is scaled twice.
+// The weights of the first 32 keys of each thread are handed over by themselves,
+// so that half of PV runs while the other weights are made (414 -> 403 us below).
 // A commit of S_t(j) covers PV_t(j-1), issued before it, so scaling O needs no
 // barrier of its own; and in-order execution of the products lets S_t(j)
 // overwrite P_t(j-1) right behind the product that reads it.
@@ -722,8 +724,8 @@ __global__ void __launch_bounds__(JW * 32, 6) attn_join_kernel(const PagedAttnAr
 // issuer that takes whichever tile is ready, or one that starts a unit's first
 // S before the last PV of the unit before: their code comes between the
 // products, which cost the long chunk 25 % and 4 %.)
-// Measured: a chunk of 4096 tokens behind 16384, 16 heads on 4 of 128: 422 us,
-// 1139 TFLOP/s, 69 % of a large product's rate.  Nine prompts of up to 1023,
+// Measured: a chunk of 4096 tokens behind 16384, 16 heads on 4 of 128: 403 us,
+// 1194 TFLOP/s, 73 % of a large product's rate.  Nine prompts of up to 1023,
 // 12 heads of 64: 50 us, where a unit's end and the next one's first tile take
 // ~4 us beside its few tiles, and the start ~6.
 constexpr int TM = 128, TKEYS = 128;
@@ -861,7 +863,7 @@ __global__ void __launch_bounds__(TTHR, 1)
     uint64_t* drain = o_full + 2;
     uint64_t* w_full = drain + 1;  // [4] each
     uint64_t* w_empty = w_full + 4;
-    uint64_t* p_half = w_empty + 4;  // [2] the weights of the first 64 keys
+    uint64_t* p_half = w_empty + 4;  // [2] the weights of keys 0-31 and 64-95
     uint64_t* b_ready = p_half + 2;  // tile B's part of tile A's rows is there
     uint64_t* b_free = b_ready + 1;  // and has been read
     uint64_t* v_fixed = b_free + 1;  // [STAGES] the values there end with the sequence
@@ -875,8 +877,7 @@ __global__ void __launch_bounds__(TTHR, 1)
         uint64_t* bar = kv_full + tid;
         int users = 1;
         if (bar >= kv_empty && bar < q_full) users = 2;                                          // the issuer and the fixing warp
-        if ((bar >= p_full && bar < o_full) || (bar >= p_half && bar < b_ready)) users = 4;      // a tile's warps with half the keys
-        if (bar == b_ready || bar == b_free) users = 8;                                          // a tile's warps
+        if ((bar >= p_full && bar < o_full) || (bar >= p_half && bar < v_fixed)) users = 8;     // a tile's warps
         if (bar >= w_empty && bar < p_half) users = 19;  // TMA, MMA, fixing and sixteen softmax warps
         mbar_init(bar, users);
         fence_barrier_init();
@@ -1131,15 +1132,16 @@ __global__ void __launch_bounds__(TTHR, 1)
                 };
                 auto values = [&](int t, uint32_t va, bool first) {  // O_t (+)= P_t V
                     const uint64_t vd = smem_desc_mn_sw128(va, C::HALF);
-                    for (int h = 0; ok && h < 2; h++) {
-                        ok = wait_bar((h ? p_full : p_half) + t, (np >> t) & 1, err, DEVERR_PTILE_P);
+                    for (int c = 0; ok && c < 2; c++) {  // keys 0-31 and 64-95, while the others' weights are made
+                        ok = wait_bar((c ? p_full : p_half) + t, (np >> t) & 1, err, DEVERR_PTILE_P);
                         if (!ok) return;
                         tc_fence_after();
 #pragma unroll
-                        for (int i = 0; i < TKEYS / 32; i++)
-                            umma_ts(tmem + C::COL_O + t * DP, tmem + C::COL_S + t * TKEYS + h * 64 + i * 8,
-                                    vd + (h * (TKEYS / 32) + i) * (2048 >> 4), idesc_o,
-                                    (!first || h > 0 || i > 0) ? 1u : 0u);
+                        for (int i = 0; i < 4; i++) {
+                            const int at = (i >> 1) * 4 + c * 2 + (i & 1);  // of the eight times 16 keys
+                            umma_ts(tmem + C::COL_O + t * DP, tmem + C::COL_S + t * TKEYS + (at >> 2) * 64 + (at & 3) * 8,
+                                    vd + at * (2048 >> 4), idesc_o, (!first || c > 0 || i > 0) ? 1u : 0u);
+                        }
                     }
                     np ^= 1 << t;
                 };
@@ -1389,6 +1391,10 @@ __global__ void __launch_bounds__(TTHR, 1)
                 };
                 tmem_ld32(s_addr + 32, s1);
                 weigh(0, s0);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_half + t);
                 tmem_ld_wait();
                 if (edge) hide(1, s1);
                 weigh(1, s1);
@@ -1399,7 +1405,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive((half ? p_full : p_half) + t);
+                if (lane == 0) mbar_arrive(p_full + t);
             }
             // ---- the tile's end
             const bool whole = w.whole, dup = w.dup;
