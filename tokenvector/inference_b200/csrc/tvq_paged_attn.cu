@@ -32,8 +32,8 @@
 //    bytes take ~330, so the wider tcgen05 tile (128 rows) would buy nothing.
 //  - a pair that lies in one piece is written at once; the parts of the others
 //    go to the workspace in f32, and attn_join_kernel joins them in order.
-// Measured: 24 sequences of up to 24000 tokens, 32 heads on 8 of 128: 222 us,
-// 6.2 TB/s, 95 % of a copy's rate.  48 sequences of up to 1024, 25 heads of 64,
+// Measured: 24 sequences of up to 24000 tokens, 32 heads on 8 of 128: 224 us,
+// 6.2 TB/s, 94 % of a copy's rate.  48 sequences of up to 1024, 25 heads of 64,
 // whose tokens have their heads side by side: 46 us, of which ~10 are the start
 // and the join, and 128-byte pieces get 5.0 TB/s (2 KB ones 5.8).  One token
 // of one sequence of 700: 9.6 us, all latency.
