@@ -419,7 +419,8 @@ TVQ_API int tvq_matmul_int4_grouped(const float* A, const uint8_t* packed_w, con
  * of 8 (a token's head is contiguous; bases 16-byte aligned), so pages may be
  * [page, heads, dim] or [heads, page, dim] inside, with gaps.  Sequence s holds
  * ctx_len[s] tokens, token j in page table[s * table_stride + j / page], slot
- * j % page; cols = columns of the table.  Its new rows are the packed rows
+ * j % page; cols = columns of the table (table_stride 0: all sequences share
+ * one row of it; else at least cols).  Its new rows are the packed rows
  * cu[s] .. cu[s + 1] (cu NULL: one row each, n_rows = n_seq); row i of n sits
  * at position ctx_len[s] - n + i.  Page numbers outside [0, pages) within a
  * sequence's length record a device error (tvq_device_error: TVQ_ERR_INVALID)
@@ -463,7 +464,8 @@ TVQ_API int tvq_dev_paged_attention(int type, const void* q, const int64_t* q_st
                                     int64_t max_q, float scale, int64_t window, void* out, float* lse, void* ws,
                                     int64_t ws_bytes, void* stream);
 /* One step of beam search.  logits [batch * beams, vocab] of `type`, rows
- * `stride` elements apart; scores f32 [batch * beams].  Each beam lists its
+ * `stride` elements apart (0: all rows are the first; else at least vocab);
+ * scores f32 [batch * beams].  Each beam lists its
  * `keep` largest logits (ties: lowest token; NaN counts as -inf), each with
  * total = score + ((x - max) - ln sum exp(x - max)) in f32 (NaN counts as
  * -inf); out: the `keep` best totals of a request's lists, descending, ties to
@@ -478,7 +480,7 @@ TVQ_API int tvq_dev_beam_select(int type, const void* logits, int64_t stride, co
                                 int64_t eos, float* out_scores, int64_t* out_tokens, int32_t* out_parents, void* ws,
                                 int64_t ws_bytes, void* stream);
 /* Row r of the new tables continues row parents[r] of the old ones (-1: an
- * empty row).  Full pages are shared; refs[pages] counts how often the tables
+ * empty row), which stand table_stride apart (0: all of them are the first).  Full pages are shared; refs[pages] counts how often the tables
  * (and whoever else keeps pages) hold each page.  Every row gets room for
  * one more token: behind a full page a free page; a part-filled last page
  * stays with the lowest new row that has it (if nobody but the old tables

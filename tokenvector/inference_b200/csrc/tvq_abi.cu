@@ -1512,7 +1512,7 @@ int paged_view(tvq::PagedView& c, int type, void* k, void* v, const int64_t* sha
                   cols * shape[1] < (1ll << 31),
               TVQ_ERR_UNSUPPORTED, "too many sequences, rows, pages or table columns");
     TVQ_CHECK(cu || n_rows == n_seq, TVQ_ERR_SIZE, "without cu every sequence has one row");
-    TVQ_CHECK(table_stride >= cols, TVQ_ERR_SIZE, "table_stride smaller than the table's columns");
+    TVQ_CHECK(table_stride == 0 || table_stride >= cols, TVQ_ERR_SIZE, "table_stride smaller than the table's columns");
     if (n_rows > 0) {
         TVQ_CHECK(n_seq > 0 && table && ctx && (shape[0] == 0 || (k && v)), TVQ_ERR_INVALID, "null buffer");
         TVQ_CHECK(aligned16(k) && aligned16(v), TVQ_ERR_UNSUPPORTED, "pages must be 16-byte aligned");
@@ -1679,7 +1679,7 @@ int tvq_dev_beam_select(int type, const void* logits, int64_t stride, const floa
     TVQ_CHECK(type == TVQ_TYPE_F32 || type == TVQ_TYPE_F16 || type == TVQ_TYPE_BF16, TVQ_ERR_INVALID,
               "unknown logits type");
     STEP(select_args(a, batch, beams, keep, vocab));
-    TVQ_CHECK(stride >= vocab, TVQ_ERR_SIZE, "logits rows overlap (stride smaller than the vocabulary)");
+    TVQ_CHECK(stride == 0 || stride >= vocab, TVQ_ERR_SIZE, "logits rows overlap (stride smaller than the vocabulary)");
     TVQ_CHECK(!finished || (eos >= 0 && eos < vocab), TVQ_ERR_INVALID, "finished beams need eos within the vocabulary");
     if (batch == 0) return TVQ_OK;
     TVQ_CHECK(logits && scores && out_scores && out_tokens && out_parents, TVQ_ERR_INVALID, "null buffer");
@@ -1734,7 +1734,7 @@ int tvq_dev_beam_reorder(const int32_t* table, int64_t table_stride, const int32
     TVQ_CHECK(shape[2] >= 1 && shape[2] <= 65535, TVQ_ERR_INVALID, "kv heads out of range");
     TVQ_CHECK(shape[3] >= 8 && shape[3] <= 128 && shape[3] % 8 == 0, TVQ_ERR_UNSUPPORTED,
               "head dim must be a multiple of 8 up to 128");
-    TVQ_CHECK(table_stride >= cols, TVQ_ERR_SIZE, "table_stride smaller than the table's columns");
+    TVQ_CHECK(table_stride == 0 || table_stride >= cols, TVQ_ERR_SIZE, "table_stride smaller than the table's columns");
     TVQ_CHECK((rows * cols == 0 || table) && (rows == 0 || lens) && (new_rows == 0 || (parents && new_lens)) &&
                   (new_rows * cols == 0 || new_table) && (shape[0] == 0 || (refs && new_refs)) && status,
               TVQ_ERR_INVALID, "null buffer");

@@ -57,6 +57,9 @@ const int32_t* i32_of(const Tensor& t, int ndim, const char* name) {
     return static_cast<const int32_t*>(t.data_ptr());
 }
 
+// Elements from row to row (a row alone may have any stride; 0: an expanded tensor, all rows are the first).
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 
@@ -101,7 +104,7 @@ Cache cache_of(const Tensor& k, const Tensor& v, const Tensor& table, const Tens
         c.strides[i] = k.stride(i);
         c.strides[3 + i] = v.stride(i);
     }
-    c.table_stride = c.seqs > 1 ? table.stride(0) : std::max(table.stride(0), table.size(1));
+    c.table_stride = row_stride(table);
     c.cols = table.size(1);
     return c;
 }
@@ -205,7 +208,7 @@ std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits, const Tenso
     int64_t bytes = 0;
     check(tvq_beam_select_workspace(batch, beams, keep, vocab, &bytes));
     const Tensor ws = workspace(dev, bytes);
-    check(tvq_dev_beam_select(type_of(logits), ptr(logits), std::max(logits.stride(0), vocab), static_cast<const float*>(ptr(scores)),
+    check(tvq_dev_beam_select(type_of(logits), ptr(logits), row_stride(logits), static_cast<const float*>(ptr(scores)),
                               static_cast<const uint8_t*>(ptr(finished)), batch, beams, keep, vocab, eos ? *eos : -1,
                               static_cast<float*>(ptr(out)), static_cast<int64_t*>(ptr(tokens)),
                               static_cast<int32_t*>(ptr(parents)), ptr(ws), bytes, st));
@@ -247,7 +250,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> beam_reorder(const Tensor& table, con
     check(tvq_beam_reorder_workspace(pages, rows, new_rows, &bytes));
     const Tensor ws = workspace(dev, bytes);
     auto i32 = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
-    check(tvq_dev_beam_reorder(table_p, std::max(table.stride(0), cols), lens_p, rows, cols, parents_p, new_rows, refs_p, ptr(k),
+    check(tvq_dev_beam_reorder(table_p, row_stride(table), lens_p, rows, cols, parents_p, new_rows, refs_p, ptr(k),
                                ptr(v), shape, strides, i32(new_table), i32(new_lens), i32(new_refs), i32(status), ptr(ws), bytes,
                                st));
     return {new_table, new_lens, new_refs, status};

@@ -9,9 +9,10 @@ __all__ = ["beam_select", "beam_reorder"]
 
 def beam_select(logits, scores, beams, keep, *, finished=None, eos=None):
     """One step's choice.  logits [batch * beams, vocab] (float32, float16 or
-    bfloat16), scores float32 [batch * beams] (log-probabilities so far; -inf
-    for a beam that does not take part) -> (scores float32, tokens int64,
-    parents int32), each [batch, keep], best first.
+    bfloat16; one row expanded over all beams will do), scores float32 [batch *
+    beams] (log-probabilities so far; -inf for a beam that does not take part)
+    -> (scores float32, tokens int64, parents int32), each [batch, keep], best
+    first.
 
     Each beam lists its `keep` largest logits (ties: the lowest token; NaN
     counts as -inf) with total = score + log softmax; the `keep` best of a
@@ -25,7 +26,7 @@ def beam_reorder(table, lens, parents, refs, k_pages, v_pages):
     """The beams' caches after a choice: row r of the new table continues row
     parents[r] of the old one (-1: an empty row), with room for one more token.
 
-    table int32 [rows, cols], lens int32 [rows], parents int32 [new_rows],
+    table int32 [rows, cols] (or one row expanded), lens int32 [rows], parents int32 [new_rows],
     refs int32 [pages] (how often the tables, and whoever else keeps pages,
     hold each page), k_pages and v_pages the cache of every layer [layers,
     pages, page, kv_heads, head_dim].  Full pages are shared.  A part-filled
