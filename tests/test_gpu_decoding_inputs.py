@@ -68,3 +68,43 @@ def test_attention_and_append_read_an_expanded_table(new):
         paged_append(rows, rows, k, v, table, ctx)
         paged_append(rows, rows, k2, v2, table.contiguous(), ctx)
         assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
+# ---------------------------------------------------------------- a bound on the new rows that a call exceeds
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("new,most,heads,kv_heads,dim", [
+    ([1, 5, 1, 16, 2, 9], 1, 2, 2, 64), ([5, 1, 16, 3, 7, 1], 3, 4, 2, 128), ([16] * 6, 2, 8, 1, 64),
+    ([90, 20, 300, 1, 65, 64], 64, 2, 2, 64), ([140, 3, 33, 500, 20, 1], 130, 4, 1, 128)])
+def test_attention_takes_max_q_rows_of_a_sequence(new, most, heads, kv_heads, dim, window):
+    """The first max_q rows of each sequence follow the definition; the others' outputs, and what lies behind the
+    workspace, stay as they are."""
+    import ctypes as C
+    from test_gpu_paged import clean, definition, hold, make
+    from tokenvector.inference_b200 import _native as N
+    torch = _torch()
+    ctx = [4000, 2500, 16, 900, 3100, 1700]
+    s = make(new, ctx, heads, kv_heads, dim, 32, "float16", seed=most)
+    rows, group = sum(new), heads // kv_heads
+    i64 = lambda *v: (C.c_int64 * len(v))(*v)  # noqa: E731
+    need = C.c_int64()
+    N.call("tvq_paged_attention_workspace", heads, kv_heads, dim, len(new), rows, most, C.byref(need))
+    ws = torch.full((need.value + 65536,), 0xA5, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(s["q"], 77.0)
+    lse = torch.full((rows, heads), 77.0, device="cuda")
+    k, v, q, table = s["k"], s["v"], s["q"], s["table"]
+    N.call("tvq_dev_paged_attention", N.TYPE_F16, q.data_ptr(), i64(*q.stride()[:2]), heads, k.data_ptr(), v.data_ptr(),
+           i64(*k.shape), i64(*(k.stride()[:3] + v.stride()[:3])), table.data_ptr(), table.stride(0), table.shape[1],
+           s["ctx"].data_ptr(), s["cu"].data_ptr(), len(new), rows, most, dim ** -0.5, window, out.data_ptr(),
+           lse.data_ptr(), ws.data_ptr(), need.value, torch.cuda.current_stream().cuda_stream)
+    clean()
+    assert group * most <= 16 or most > 16
+    assert (ws[need.value:] == 0xA5).all()
+    taken = torch.cat([torch.arange(n) < most for n in new]).cuda()
+    assert (out[~taken] == 77.0).all() and (lse[~taken] == 77.0).all()
+    want = definition(s, window=window)
+    for t in want:  # a row that is not taken: nothing to compare
+        t[~taken] = 0.0
+    got, got_lse = out.clone(), lse.clone()
+    got[~taken] = 0.0
+    got_lse[~taken] = 0.0
+    hold(s, got, got_lse, want)

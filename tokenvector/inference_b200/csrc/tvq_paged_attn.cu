@@ -149,21 +149,24 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return a / b;
 }
 
-// One sequence as both kernels see it.
+// One sequence as the kernels see it.
 struct Seq {
     int row0;  // first packed row
     int n;     // new rows
+    int m;     // those that the call takes: the first max_q, as the workspace is sized for
     int len;   // tokens in the cache
 };
-__device__ __forceinline__ Seq load_seq(const PagedView& c, int s) {
+__device__ __forceinline__ Seq load_seq(const PagedAttnArgs& a, int s) {
+    const PagedView& c = a.c;
     Seq q;
     q.len = __ldg(c.ctx + s);
     if (c.cu) {
-        q.row0 = max(0, __ldg(c.cu + s));
-        q.n = max(0, min(__ldg(c.cu + s + 1), c.n_rows) - q.row0);
+        q.row0 = __ldg(c.cu + s);
+        q.n = __ldg(c.cu + s + 1) - q.row0;
+        q.m = q.row0 < 0 ? 0 : max(0, min(min(q.n, a.max_q), c.n_rows - q.row0));
     } else {
         q.row0 = s;
-        q.n = 1;
+        q.n = q.m = 1;
     }
     return q;
 }
@@ -174,7 +177,7 @@ template <int KT>
 __device__ __forceinline__ int2 seq_tiles(const Seq& q, int window) {
     const int p0 = q.len - q.n;
     const int first = window > 0 ? max(0, p0 - window + 1) / KT : 0;
-    return make_int2(first, max(first + 1, (max(q.len, 0) + KT - 1) / KT));
+    return make_int2(first, max(first + 1, (max(p0 + q.m, 0) + KT - 1) / KT));
 }
 
 // ---------------------------------------------------------------- few rows
@@ -227,8 +230,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + mine * C::STAGES;
     uint64_t* empty = full + NW * C::STAGES;
     uint8_t* ring = sm + mine * (C::STAGES * C::STAGE);
-    const int group = a.q_heads / a.c.kv_heads;
-    const int fit = MAX_ROWS / group;  // new rows of a sequence that this kernel takes
+    const int group = a.q_heads / a.c.kv_heads;  // (max_q * group <= MAX_ROWS: few_rows)
     static_assert(2 * NW * C::STAGES <= NTHR - 32);
     if (tid < 2 * NW * C::STAGES) {
         mbar_init(reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + tid, 1);
@@ -243,8 +245,8 @@ __global__ void __launch_bounds__(NTHR, 1)
     // ---- the pieces of the line of tiles
     auto weight = [&](int s) -> int {
         if (s >= a.c.n_seq) return 0;
-        const Seq q = load_seq(a.c, s);
-        if (q.n == 0 || q.n > fit) return 0;
+        const Seq q = load_seq(a, s);
+        if (q.m == 0) return 0;
         const int2 t = seq_tiles<KT>(q, a.window);
         return t.y - t.x;
     };
@@ -311,8 +313,8 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (++c.hk == a.c.kv_heads) {
             c.hk = 0;
             do {
-                c.q = load_seq(a.c, ++c.s);
-            } while (c.q.n == 0 || c.q.n > fit);
+                c.q = load_seq(a, ++c.s);
+            } while (c.q.m == 0);
         }
         enter(c, 0);
         return true;
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     cur.left = stop - begin;
     if (cur.left > 0) {
         cur.s = s_seq[mine];
-        cur.q = load_seq(a.c, cur.s);
+        cur.q = load_seq(a, cur.s);
         const int64_t in_seq = begin - s_at[mine];
         const int2 t = seq_tiles<KT>(cur.q, a.window);
         cur.hk = static_cast<int>(quotient(in_seq, t.y - t.x));
@@ -433,7 +435,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     bool ok = true;
     for (bool go = true; go; go = next_pair(cur)) {
         // ---- the pair's rows as A fragments
-        const int rows = cur.q.n * group;
+        const int rows = cur.q.m * group;
         uint32_t qf[DP / 16][4];
         int pos[2];     // of this thread's two rows (below 0: sees nothing)
         int64_t at[2];  // their place in out (below 0: none)
@@ -605,12 +607,12 @@ __global__ void __launch_bounds__(JW * 32, 6) attn_join_kernel(const PagedAttnAr
         const int64_t u = u0 + warp / SHARE, pair = u / plan.rows_cap;
         const int r = static_cast<int>(u - pair * plan.rows_cap);
         const int s = static_cast<int>(pair / a.c.kv_heads), hk = static_cast<int>(pair - static_cast<int64_t>(s) * a.c.kv_heads);
-        Seq q{0, 0, 0};
-        if (u < all) q = load_seq(a.c, s);  // (the rows kernel started this one after its own wait: they are there)
+        Seq q{};
+        if (u < all) q = load_seq(a, s);  // (the rows kernel started this one after its own wait: they are there)
         if (!waited) griddep_wait();
         waited = true;
         int2 span = make_int2(0, 0);
-        if (q.n > 0 && q.n <= MAX_ROWS / group && r < q.n * group) span = plan.spans[pair];
+        if (r < q.m * group) span = plan.spans[pair];
         const bool act = span.x != span.y;
         float t = -INFINITY, sum = 0.0f, o[E];
 #pragma unroll
@@ -754,7 +756,7 @@ struct TileCfg {
 };
 
 struct Begun {
-    int rows, row0, n, hk;  // rows of the unit (0: none); the sequence's; the kv head
+    int rows, row0, m, hk;  // rows of the unit (0: none); the sequence's; the kv head
     int unit, last, pad[2];  // which unit of the sequence; the last piece that has a part of it
 };
 struct TilePlan {
@@ -776,7 +778,7 @@ __device__ __forceinline__ Unit make_unit(const Seq& q, int u, int tokens, int w
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         w.i0[t] = (2 * u + t) * tokens;
-        w.cnt[t] = max(0, min(tokens, q.n - w.i0[t]));
+        w.cnt[t] = max(0, min(tokens, q.m - w.i0[t]));
         const int pa = q.len - q.n + w.i0[t], pb = pa + w.cnt[t] - 1;
         w.first[t] = window > 0 ? max(0, pa - window + 1) / TKEYS : 0;
         w.end[t] = max(w.first[t] + 1, (max(pb + 1, 0) + TKEYS - 1) / TKEYS);
@@ -786,7 +788,7 @@ __device__ __forceinline__ Unit make_unit(const Seq& q, int u, int tokens, int w
     w.e = max(w.end[0], w.end[1]);
     return w;
 }
-__device__ __forceinline__ int seq_units(const Seq& q, int tokens) { return (q.n + 2 * tokens - 1) / (2 * tokens); }
+__device__ __forceinline__ int seq_units(const Seq& q, int tokens) { return (q.m + 2 * tokens - 1) / (2 * tokens); }
 
 // A unit's share of a CTA's piece: key tiles [a, b), of them [lo, hi) for each
 // row tile (lo >= hi: none).
@@ -900,8 +902,8 @@ __global__ void __launch_bounds__(TTHR, 1)
     // ---- the piece of the line of key tiles
     auto weight = [&](int s) -> int64_t {  // of one kv head
         if (s >= a.c.n_seq) return 0;
-        const Seq q = load_seq(a.c, s);
-        if (q.n == 0) return 0;
+        const Seq q = load_seq(a, s);
+        if (q.m == 0) return 0;
         int64_t sum = 0;
         for (int u = 0; u < seq_units(q, plan.tokens); u++) {
             const Unit w = make_unit(q, u, plan.tokens, a.window);
@@ -968,10 +970,10 @@ __global__ void __launch_bounds__(TTHR, 1)
                 Begun begun{};
                 int s = 0, hk = 0, u = 0, skip = 0, units = 0;
                 int64_t left = stop - begin;
-                Seq q{0, 0, 0};
+                Seq q{};
                 if (left > 0) {
                     s = *s_seq;
-                    q = load_seq(a.c, s);
+                    q = load_seq(a, s);
                     int64_t in = begin - *s_at, one = 0;  // one: tiles of one kv head
                     units = seq_units(q, plan.tokens);
                     for (int i = 0; i < units; i++) {
@@ -1018,7 +1020,7 @@ __global__ void __launch_bounds__(TTHR, 1)
                             o.hi[1] = o.b;
                         }
                         if (o.begins && !o.whole)
-                            begun = Begun{w.cnt[0] + w.cnt[1], q.row0, q.n, hk, u,
+                            begun = Begun{w.cnt[0] + w.cnt[1], q.row0, q.m, hk, u,
                                           static_cast<int>(quotient(stop - left + w.e - w.f - 1, per))};
                         left -= o.b - o.a;
                         skip = 0;
@@ -1027,8 +1029,8 @@ __global__ void __launch_bounds__(TTHR, 1)
                             if (++hk == a.c.kv_heads) {
                                 hk = 0;
                                 do {
-                                    q = load_seq(a.c, ++s);
-                                } while (q.n == 0);
+                                    q = load_seq(a, ++s);
+                                } while (q.m == 0);
                                 units = seq_units(q, plan.tokens);
                             }
                         }
