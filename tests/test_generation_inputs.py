@@ -25,3 +25,31 @@ def test_rows_may_coincide_but_not_overlap():
                                             i64(0, 2048, 128, 64, 0, 2048, 128, 64), apart, apart, apart, FAKE, None, 0,
                                             None) == N.TVQ_ERR_SIZE
         assert why in N.last_error()
+
+
+# ---------------------------------------------------------------- the generator
+@pytest.fixture
+def generator():
+    """A generator without a session: what is refused is refused before the device is touched."""
+    torch = pytest.importorskip("torch")
+    from tokenvector.inference_b200.generation import GPT2Generator
+    from tokenvector.inference_b200.gpt2 import GPT2Config
+    g = GPT2Generator.__new__(GPT2Generator)
+    g.cfg = GPT2Config(vocab=320, d_model=128, n_heads=2, n_layers=2, d_ffn=512, max_pos=64)
+    g.page, g.dtype, g.dev = 16, torch.float16, torch.device("cuda", 0)
+    return g
+
+
+@pytest.mark.parametrize("ids", [[320], [3, -1], [2 ** 40], [1, 2, 2 ** 70], [1.5, 2.0], [True, False], [], [[1, 2]], "12"])
+def test_generator_refuses_ids_outside_the_vocabulary(generator, ids):
+    with pytest.raises(ValueError):
+        generator.log_probs(ids)
+    with pytest.raises(ValueError):
+        generator.generate([[1, 2, 3], ids], 2, 4)
+
+
+def test_generator_refuses_sequences_longer_than_its_positions(generator):
+    with pytest.raises(ValueError, match="positions"):
+        generator.log_probs([1] * 65)
+    with pytest.raises(ValueError, match="positions"):
+        generator.generate([[1], [2] * 62], 2, 3)

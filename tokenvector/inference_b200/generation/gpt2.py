@@ -100,13 +100,23 @@ class GPT2Generator:
         return y
 
     # ---- prompts
+    def _ids(self, prompt):
+        """A prompt's token ids as int64, checked on the host: the embeddings are indexed on the device."""
+        ids = np.asarray(prompt)
+        if ids.ndim != 1 or ids.size == 0:
+            raise ValueError("every prompt needs a token")
+        if ids.dtype.kind not in "iu" or ids.min() < 0 or ids.max() >= self.cfg.vocab:
+            raise ValueError("token ids must be integers within the vocabulary")
+        if ids.size > self.cfg.max_pos:
+            raise ValueError("sequence longer than the model's positions")
+        return ids.astype(np.int64)
+
     def _prefill(self, prompts, spare_pages, cols=0):
         """The prompts' cache and last hidden states, with `spare_pages` free
         pages and `cols` table columns at least."""
         page, cfg = self.page, self.cfg
+        prompts = [self._ids(p) for p in prompts]
         lens = [len(p) for p in prompts]
-        if min(lens) < 1:
-            raise ValueError("every prompt needs a token")
         held = [-(-n // page) for n in lens]
         pool = sum(held) + spare_pages
         shape = (cfg.n_layers, pool, page, cfg.n_heads, cfg.d_model // cfg.n_heads)
@@ -120,7 +130,7 @@ class GPT2Generator:
         table = put(table, torch.int32)
         refs = put((np.arange(pool) < first).astype(np.int32), torch.int32)
         cu = np.concatenate([[0], np.cumsum(lens)])
-        ids = put(np.concatenate([np.asarray(p, np.int64) for p in prompts]), torch.int64)
+        ids = put(np.concatenate(prompts), torch.int64)
         pos = put(np.concatenate([np.arange(n) for n in lens]), torch.int64)
         ctx = put(lens, torch.int32)
         x = self._rows(ids, pos, cache, table, ctx, put(cu, torch.int32), max(lens))
@@ -128,9 +138,10 @@ class GPT2Generator:
 
     def log_probs(self, ids):
         """log p(ids[t] | ids[:t]) for t >= 1, one sequence at once: float32 [len - 1]."""
+        ids = self._ids(ids)
         x = self._prefill([ids], 0)[4]
         lp = torch.log_softmax(self._logits(x[:-1]), 1)
-        return lp.gather(1, torch.as_tensor(np.asarray(ids[1:], np.int64), device=self.dev)[:, None])[:, 0]
+        return lp.gather(1, torch.as_tensor(ids[1:], device=self.dev)[:, None])[:, 0]
 
     def generate(self, prompts, beams: int, max_new: int, eos: int | None = None):
         """Beam search over several prompts (lists of token ids) at once.
