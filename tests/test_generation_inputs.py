@@ -53,3 +53,9 @@ def test_generator_refuses_sequences_longer_than_its_positions(generator):
         generator.log_probs([1] * 65)
     with pytest.raises(ValueError, match="positions"):
         generator.generate([[1], [2] * 62], 2, 3)
+
+
+@pytest.mark.parametrize("max_new", [0, -1])
+def test_generator_refuses_to_make_no_token(generator, max_new):
+    with pytest.raises(ValueError, match="max_new"):
+        generator.generate([[1, 2]], 2, max_new)

@@ -150,6 +150,8 @@ class GPT2Generator:
         (tokens, score) with score the sum of the tokens' log-probabilities;
         a continuation ends with `eos` or after max_new tokens."""
         cfg, page = self.cfg, self.page
+        if max_new < 1:
+            raise ValueError("max_new must be at least 1")
         longest = max(len(p) for p in prompts)
         if longest + max_new > cfg.max_pos:
             raise ValueError("prompt and continuation exceed the model's positions")
