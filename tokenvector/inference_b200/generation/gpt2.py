@@ -139,6 +139,8 @@ class GPT2Generator:
     def log_probs(self, ids):
         """log p(ids[t] | ids[:t]) for t >= 1, one sequence at once: float32 [len - 1]."""
         ids = self._ids(ids)
+        if ids.size == 1:  # its logits predict nothing
+            return torch.empty(0, dtype=torch.float32, device=self.dev)
         x = self._prefill([ids], 0)[4]
         lp = torch.log_softmax(self._logits(x[:-1]), 1)
         return lp.gather(1, torch.as_tensor(ids[1:], device=self.dev)[:, None])[:, 0]
