@@ -12,3 +12,21 @@ def test_log_probs_of_the_shortest_and_the_longest_sequence(model):  # noqa: F81
     assert g.log_probs([5]).shape == (0,)
     longest = g.log_probs(np.arange(cfg.max_pos) % cfg.vocab)
     assert longest.shape == (cfg.max_pos - 1,) and bool((longest < 0).all())
+
+
+@pytest.mark.parametrize("call", ["log_probs", "generate"])
+def test_an_error_of_the_device_is_raised(model, call):  # noqa: F811
+    """An error that a kernel of the stream recorded (a page number out of range) ends the call, once."""
+    import torch
+
+    from tokenvector.inference_b200 import _native as N
+    from tokenvector.inference_b200.generation import paged_append
+    cfg, w, s, g = model
+    run = {"log_probs": lambda: g.log_probs([1, 2, 3]), "generate": lambda: g.generate([[1, 2]], 2, 3)}[call]
+    k = torch.zeros((2, 16, 2, 64), dtype=torch.float16, device="cuda")
+    row = torch.ones((1, 2, 64), device="cuda")
+    one = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    paged_append(row, row, k, k.clone(), one([[7]]), one([1]))
+    with pytest.raises(N.TvqError, match="page"):
+        run()
+    run()

@@ -48,6 +48,10 @@ class GPT2Generator:
     def _call(self, name, *args):
         D.call(name, self.dev, *args, D.stream(self.dev))
 
+    def _check(self):
+        """Waits for the stream; raises what its kernels recorded (a wait that ran out, a page out of range)."""
+        self._call("tvq_device_error")
+
     def _split(self, x):
         hi, lo = (torch.empty(x.shape, dtype=torch.float16, device=self.dev) for _ in range(2))
         scale = torch.empty(x.shape[0], dtype=torch.float32, device=self.dev)
@@ -143,7 +147,9 @@ class GPT2Generator:
             return torch.empty(0, dtype=torch.float32, device=self.dev)
         x = self._prefill([ids], 0)[4]
         lp = torch.log_softmax(self._logits(x[:-1]), 1)
-        return lp.gather(1, torch.as_tensor(ids[1:], device=self.dev)[:, None])[:, 0]
+        lp = lp.gather(1, torch.as_tensor(ids[1:], device=self.dev)[:, None])[:, 0]
+        self._check()
+        return lp
 
     def generate(self, prompts, beams: int, max_new: int, eos: int | None = None):
         """Beam search over several prompts (lists of token ids) at once.
@@ -186,7 +192,7 @@ class GPT2Generator:
                 break
         if int(short) > 0:
             raise RuntimeError("the page pool ran out")
-        D.call("tvq_device_error", self.dev, D.stream(self.dev))
+        self._check()
         out = []
         for s in range(len(prompts)):
             mine = []
