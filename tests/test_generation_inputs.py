@@ -59,3 +59,23 @@ def test_generator_refuses_sequences_longer_than_its_positions(generator):
 def test_generator_refuses_to_make_no_token(generator, max_new):
     with pytest.raises(ValueError, match="max_new"):
         generator.generate([[1, 2]], 2, max_new)
+
+
+# ---------------------------------------------------------------- several devices
+def test_kernel_limits_are_set_on_every_device(tmp_path):
+    """The flag that the launchers keep for a kernel's attribute (the two-GPU test of it is in test_gpu_decoding_inputs)."""
+    import os
+    import shutil
+    import subprocess
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe = str(tmp_path / "once")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-o", exe, os.path.join(here, "native", "once_per_device.cpp")])
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
+    csrc = os.path.join(here, "..", "tokenvector", "inference_b200", "csrc")
+    for name in ("tvq_paged_attn.cu", "tvq_beam.cu"):  # no flag of the process beside it
+        with open(os.path.join(csrc, name)) as f:
+            text = f.read()
+        assert "cudaFuncSetAttribute" not in text and "allow_smem<" in text

@@ -108,3 +108,27 @@ def test_attention_takes_max_q_rows_of_a_sequence(new, most, heads, kv_heads, di
     got[~taken] = 0.0
     got_lse[~taken] = 0.0
     hold(s, got, got_lse, want)
+
+
+# ---------------------------------------------------------------- several devices in a process
+def test_operators_work_on_every_device():
+    """Kernels with more than 48 KB of shared memory, on one GPU and then on another one of the process."""
+    torch = _torch()
+    from tokenvector.inference_b200.generation import beam_select, paged_attention
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    gen = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((9, 16, 2, 64), generator=gen).half() for _ in range(2))
+    q = torch.randn((40, 4, 64), generator=gen).half()
+    x, scores = torch.randn((64, 9000), generator=gen), torch.zeros(64)
+    table = torch.tensor([[3, 0, 8, 5]], dtype=torch.int32)
+    results = []
+    for dev in ("cuda:0", "cuda:1"):
+        on = lambda t: t.to(dev)  # noqa: E731,B023
+        ctx = torch.tensor([60], dtype=torch.int32, device=dev)
+        cu = torch.tensor([0, 40], dtype=torch.int32, device=dev)
+        results.append([paged_attention(on(q[:1]), on(k), on(v), on(table), ctx),
+                        paged_attention(on(q), on(k), on(v), on(table), ctx, cu),
+                        *beam_select(on(x), on(scores), 64, 64)])
+    for a, b in zip(*results):
+        assert torch.equal(a.cpu(), b.cpu())

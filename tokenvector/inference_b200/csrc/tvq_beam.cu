@@ -669,9 +669,8 @@ int launch_select(const BeamSelectArgs& a, const Slices& s, cudaStream_t st) {
     if (!ds) return rc;
     uint64_t* keys = static_cast<uint64_t*>(a.ws);
     float2* stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.ws) + s.keys);
-    static const cudaError_t attr2 =
-        cudaFuncSetAttribute(select_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    TVQ_CUDA(attr2);
+    rc = allow_smem<select_merge_kernel>(200 * 1024);
+    if (rc) return rc;
     const int64_t items = static_cast<int64_t>(a.batch) * a.beams * s.n;
     rc = launch_pdl(select_slice_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(items, kSliceCtas))), dim3(SLT),
                     static_cast<size_t>(SBUF + SCAP * 8), st, a, keys, stats, s.n, s.width, ds->d_error);

@@ -14,6 +14,7 @@
 #include <string>
 
 #include "tvq.h"
+#include "tvq_once.h"
 
 namespace tvq {
 
@@ -94,6 +95,19 @@ int launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cu
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
     TVQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
     return TVQ_OK;
+}
+
+// A kernel's limit of dynamic shared memory, raised on the current device (the
+// attribute belongs to a device, not to the process).
+template <auto KERNEL>
+int allow_smem(size_t bytes) {
+    static OncePerDevice once;
+    int dev = 0;
+    TVQ_CUDA(cudaGetDevice(&dev));
+    return once(dev, [&]() -> int {
+        TVQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+        return TVQ_OK;
+    });
 }
 
 // Wall-clock bound on one wait (ns).  A healthy wait lasts microseconds.

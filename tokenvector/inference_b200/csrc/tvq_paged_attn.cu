@@ -1644,9 +1644,8 @@ int cache_map(CUtensorMap* map, const PagedView& c, const void* ptr, int64_t tok
 template <typename T, int DP>
 int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     using C = RowsCfg<DP>;
-    static const cudaError_t attr =
-        cudaFuncSetAttribute(attn_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    TVQ_CUDA(attr);
+    int rc = allow_smem<attn_rows_kernel<T, DP>>(C::SMEM);
+    if (rc) return rc;
     const RowsSpace w = rows_space(a, ds->sm_count);
     RowsPlan plan;
     plan.spans = static_cast<int2*>(a.ws);
@@ -1657,7 +1656,7 @@ int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     plan.by_value = a.c.dim % 64 != 0;
     plan.box_halves = a.c.dim == 128 && plan.box == C::KT ? 2 : 1;
     CUtensorMap tmK, tmV;
-    int rc = cache_map(&tmK, a.c, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
+    rc = cache_map(&tmK, a.c, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
     if (rc) return rc;
     rc = cache_map(&tmV, a.c, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
     if (rc) return rc;
@@ -1676,9 +1675,8 @@ int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
 template <typename T, int DP>
 int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     using C = TileCfg<DP>;
-    static const cudaError_t attr =
-        cudaFuncSetAttribute(attn_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    TVQ_CUDA(attr);
+    int rc = allow_smem<attn_tile_kernel<T, DP>>(C::SMEM);
+    if (rc) return rc;
     const int group = a.q_heads / a.c.kv_heads;
     uint8_t* ws = static_cast<uint8_t*>(a.ws);
     TilePlan plan;
@@ -1696,7 +1694,7 @@ int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
                               static_cast<uint64_t>(a.q_heads), static_cast<uint64_t>(a.c.n_rows)};
     const uint64_t strides[3] = {128, static_cast<uint64_t>(a.q_head) * 2, static_cast<uint64_t>(a.q_tok) * 2};
     const uint32_t box[4] = {64, 1, static_cast<uint32_t>(group), static_cast<uint32_t>(plan.tokens)};
-    int rc = make_tma_16bit(&tmQ, a.q, 4, dims, strides, box);
+    rc = make_tma_16bit(&tmQ, a.q, 4, dims, strides, box);
     if (rc) return rc;
     rc = cache_map(&tmK, a.c, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
     if (rc) return rc;
