@@ -79,3 +79,18 @@ def test_kernel_limits_are_set_on_every_device(tmp_path):
         with open(os.path.join(csrc, name)) as f:
             text = f.read()
         assert "cudaFuncSetAttribute" not in text and "allow_smem<" in text
+
+
+@pytest.mark.parametrize("change", [dict(vocab=319), dict(vocab=321), dict(d_model=64), dict(max_pos=63), dict(n_layers=1),
+                                    dict(n_layers=3)])
+def test_generator_refuses_weights_of_another_shape(change):
+    """Before the session is asked for anything: it is a stand-in."""
+    pytest.importorskip("torch")
+    from types import SimpleNamespace
+
+    from tokenvector.inference_b200.generation import GPT2Generator
+    from tokenvector.inference_b200.gpt2 import GPT2Config, GPT2Weights
+    cfg = dict(vocab=320, d_model=128, n_heads=2, n_layers=2, d_ffn=256, max_pos=64)
+    session = SimpleNamespace(cfg=GPT2Config(**cfg), device=0)
+    with pytest.raises(ValueError, match="shape"):
+        GPT2Generator(session, GPT2Weights.random(GPT2Config(**{**cfg, **change})))

@@ -30,3 +30,19 @@ def test_an_error_of_the_device_is_raised(model, call):  # noqa: F811
     with pytest.raises(N.TvqError, match="page"):
         run()
     run()
+
+
+def test_weights_of_another_float_type_are_the_same_model(model):  # noqa: F811
+    """The session takes embeddings and norms in any float type; so does the generator."""
+    from dataclasses import replace
+
+    import torch
+
+    from tokenvector.inference_b200.generation import GPT2Generator
+    cfg, w, s, g = model
+    names = ("ln1_g", "ln1_b", "ln2_g", "ln2_b")
+    wide = replace(w, wte=w.wte.astype(np.float64), wpe=w.wpe.astype(np.float64), lnf_g=w.lnf_g.astype(np.float64),
+                   lnf_b=w.lnf_b.astype(np.float64),
+                   layers=[{k: a.astype(np.float64) if k in names else a for k, a in L.items()} for L in w.layers])
+    ids = [3, 1, 4, 1, 5, 9, 2, 6]
+    assert torch.equal(GPT2Generator(s, wide).log_probs(ids), g.log_probs(ids))

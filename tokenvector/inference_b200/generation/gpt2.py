@@ -31,17 +31,29 @@ class GPT2Generator:
 
     def __init__(self, session, weights, *, page: int = 16, dtype=torch.float16):
         cfg = session.cfg
+        d = cfg.d_model
+
+        def same(a, *shape):
+            if np.shape(a) != shape:
+                raise ValueError("weights of another shape than the session's")
+            return np.asarray(a, np.float32)
+
+        if len(weights.layers) != cfg.n_layers:
+            raise ValueError("weights of another shape than the session's")
+        norms = [[same(w[name], d) for name in ("ln1_g", "ln1_b", "ln2_g", "ln2_b")] for w in weights.layers]
+        final = same(weights.lnf_g, d), same(weights.lnf_b, d)
+        wte, wpe = same(weights.wte, cfg.vocab, d), same(weights.wpe, cfg.max_pos, d)
         self.cfg, self.page, self.dtype = cfg, page, dtype
         self.dev = torch.device("cuda", session.device)
         put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self.dev)  # noqa: E731
         self.scales = put(session.act_scales())  # [layers, 4]: ln_1, attention, ln_2, GELU outputs
         self.layers = []
-        for li, w in enumerate(weights.layers):
+        for li, norm in enumerate(norms):
             lin = [tuple(put(x) for x in session.linear_i8(li, which)) + (put(session._bias[li][which]),)
                    for which in range(4)]
-            self.layers.append((lin, put(w["ln1_g"]), put(w["ln1_b"]), put(w["ln2_g"]), put(w["ln2_b"])))
-        self.lnf = put(weights.lnf_g), put(weights.lnf_b)
-        self.wte, self.wpe = put(weights.wte), put(weights.wpe)
+            self.layers.append((lin, *(put(a) for a in norm)))
+        self.lnf = put(final[0]), put(final[1])
+        self.wte, self.wpe = put(wte), put(wpe)
         self.head = self._split(self.wte)
 
     # ---- the stack on T rows
