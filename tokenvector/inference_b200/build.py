@@ -3,11 +3,15 @@ _tvq_torch.so, the decoding operators on torch tensors (csrc/tvq_torch.cpp).
 
 The shared libraries land next to this file so that they travel with the
 repository snapshot; nothing is installed into site-packages.  Objects are
-compiled in parallel and rebuilt only when a source or header is newer.
+compiled in parallel and rebuilt only when a source or header is newer,
+_tvq_torch.so also when Python or torch is another one.  Without torch it is
+left out: libtvq.so does not need it.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -54,11 +58,22 @@ def _compile(nvcc, src, obj, verbose):
     return r.stderr
 
 
+def _torch_stamp() -> str:
+    """What _tvq_torch.so depends on beside its sources."""
+    return "python %s, torch %s" % (sys.version, importlib.metadata.version("torch"))
+
+
 def _build_torch(force: bool) -> None:
     """_tvq_torch.so: g++ against torch's headers, linked to libtvq.so beside it."""
-    newest = max(os.path.getmtime(TORCH_SRC), os.path.getmtime(os.path.join(INCLUDE, "tvq.h")))
-    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= newest:
+    if importlib.util.find_spec("torch") is None:
+        sys.stderr.write("torch is not installed: _tvq_torch.so (the generation package) is not built\n")
         return
+    newest = max(os.path.getmtime(TORCH_SRC), os.path.getmtime(os.path.join(INCLUDE, "tvq.h")))
+    stamp, built_for = os.path.join(OBJDIR, "tvq_torch.stamp"), _torch_stamp()
+    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == built_for:
+                return
     import sysconfig
 
     import torch
@@ -77,6 +92,8 @@ def _build_torch(force: bool) -> None:
     if r.returncode != 0:
         raise RuntimeError("building _tvq_torch.so failed:\n%s%s" % (r.stdout, r.stderr))
     os.replace(tmp, TORCH_LIB)
+    with open(stamp, "w") as f:
+        f.write(built_for)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
