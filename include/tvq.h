@@ -480,7 +480,8 @@ TVQ_API int tvq_dev_beam_select(int type, const void* logits, int64_t stride, co
                                 int64_t eos, float* out_scores, int64_t* out_tokens, int32_t* out_parents, void* ws,
                                 int64_t ws_bytes, void* stream);
 /* Row r of the new tables continues row parents[r] of the old ones (-1: an
- * empty row), which stand table_stride apart (0: all of them are the first).  Full pages are shared; refs[pages] counts how often the tables
+ * empty row), which stand table_stride apart (0: all of them are the first).
+ * A length below 0 counts as 0.  Full pages are shared; refs[pages] counts how often the tables
  * (and whoever else keeps pages) hold each page.  Every row gets room for
  * one more token: behind a full page a free page; a part-filled last page
  * stays with the lowest new row that has it (if nobody but the old tables

@@ -132,3 +132,28 @@ def test_operators_work_on_every_device():
                         *beam_select(on(x), on(scores), 64, 64)])
     for a, b in zip(*results):
         assert torch.equal(a.cpu(), b.cpu())
+
+
+# ---------------------------------------------------------------- lengths out of range
+@pytest.mark.parametrize("lens,same", [
+    ([-3, 20, -16, -(1 << 31)], [0, 20, 0, 0]), ([(1 << 31) - 1, 37, (1 << 31) - 16, 1 << 30], [3 * 16 + 5, 37, 48, 48])])
+def test_reorder_of_lengths_out_of_range(lens, same):
+    """Below 0 is 0; behind the table's columns there is no room, whatever the length."""
+    torch = _torch()
+    from tokenvector.inference_b200.generation import beam_reorder
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    store = i32([[1 << 29] * 3] * 3 + [[0, 3, 6], [1, 4, 7], [2, 5, 8], [9, 10, 11]] + [[1 << 29] * 3] * 3)
+    table = store[3:7]  # page numbers out of range in front and behind
+    k = torch.randn((2, 16, 16, 2, 64), device="cuda", generator=gen).half()
+    v, k2 = torch.randn_like(k), k.clone()
+    v2 = v.clone()
+    refs = [0] * 16
+    for row, n in zip(table.tolist(), same):
+        for p in row[:-(-n // 16)]:
+            refs[p] += 1
+    parents = i32([0, 1, 3, 2, 0])
+    got = beam_reorder(table, i32(lens), parents, i32(refs), k, v)
+    want = beam_reorder(table, i32(same), parents, i32(refs), k2, v2)
+    assert got[1].tolist() == [max(0, lens[p]) for p in parents.tolist()]
+    for a, b in zip((got[0], got[2], got[3], k, v), (want[0], want[2], want[3], k2, v2)):
+        assert torch.equal(a, b)

@@ -468,7 +468,7 @@ __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
     constexpr int ALL = RC * RT;
     const int t = threadIdx.x, g = blockIdx.x * RT + t;  // the cluster is the grid
     const int log2 = __ffs(a.page) - 1;
-    auto used = [&](int len) { return min(a.cols, (len + a.page - 1) >> log2); };
+    auto used = [&](int len) { return min(a.cols, (len >> log2) + ((len & (a.page - 1)) != 0)); };  // (any int)
     // (row, column) of the entries g, g + ALL, ... of a table: one division, not one each
     const int r_first = g / max(a.cols, 1), c_first = g - r_first * a.cols;
     const int r_step = ALL / max(a.cols, 1), c_step = ALL - r_step * a.cols;
@@ -521,7 +521,7 @@ __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
         const int q = a.parents[r];
         if (q >= a.rows) record_error(err, DEVERR_BAD_INDEX);
         const bool live = q >= 0 && q < a.rows;
-        const int len = live ? a.lens[q] : 0, at = len >> log2;
+        const int len = live ? max(0, a.lens[q]) : 0, at = len >> log2;  // (at indexes the table: never below 0)
         int tail = -1;  // the page that is part-filled, if one is
         if (live && (len & (a.page - 1)) && at < a.cols) {
             tail = a.table[q * a.table_stride + at];

@@ -26,8 +26,8 @@ def beam_reorder(table, lens, parents, refs, k_pages, v_pages):
     """The beams' caches after a choice: row r of the new table continues row
     parents[r] of the old one (-1: an empty row), with room for one more token.
 
-    table int32 [rows, cols] (or one row expanded), lens int32 [rows], parents int32 [new_rows],
-    refs int32 [pages] (how often the tables, and whoever else keeps pages,
+    table int32 [rows, cols] (or one row expanded), lens int32 [rows] (below 0
+    counts as 0), parents int32 [new_rows], refs int32 [pages] (how often the tables, and whoever else keeps pages,
     hold each page), k_pages and v_pages the cache of every layer [layers,
     pages, page, kv_heads, head_dim].  Full pages are shared.  A part-filled
     last page stays with the lowest row that has it, if nobody but the old
