@@ -485,8 +485,9 @@ TVQ_API int tvq_dev_beam_select(int type, const void* logits, int64_t stride, co
  * (and whoever else keeps pages) hold each page.  Every row gets room for
  * one more token: behind a full page a free page; a part-filled last page
  * stays with the lowest new row that has it (if nobody but the old tables
- * holds it), the other rows take a free page each and its filled tokens are
- * copied there, in every layer, keys and values.  Free pages are those with
+ * holds it, and none of their rows as a full page), the other rows take a free
+ * page each and its filled tokens are copied there, in every layer, keys and
+ * values.  Free pages are those with
  * refs 0 before the call, lowest number first, in row order.  Written:
  * new_table [new_rows, cols] (unused entries -1), new_lens, new_refs (all
  * apart from their inputs), status[2] = {pages taken, rows left without room:

@@ -157,3 +157,39 @@ def test_reorder_of_lengths_out_of_range(lens, same):
     assert got[1].tolist() == [max(0, lens[p]) for p in parents.tolist()]
     for a, b in zip((got[0], got[2], got[3], k, v), (want[0], want[2], want[3], k2, v2)):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- a page that is one row's last and another's full one
+def test_reorder_leaves_a_page_alone_that_another_row_holds_in_full():
+    """Rows of different lengths over a shared prefix: the shorter one gets a copy, or its next token would overwrite
+    the longer one's."""
+    torch = _torch()
+    from tokenvector.inference_b200.generation import beam_reorder, paged_append
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn((1, 9, 16, 2, 64), device="cuda", generator=gen).half()
+    v = torch.randn_like(k)
+    #       ends in page 1    page 1 is full    the same tokens as row 0
+    table = i32([[0, 1, -1, -1], [0, 1, 2, -1], [0, 1, -1, -1], [3, 4, -1, -1]])
+    lens, refs = i32([20, 40, 21, 18]), i32([3, 3, 1, 1, 1, 0, 0, 0, 0])
+    old = [k[0, p].clone() for p in range(9)]
+    t, n, c, status = beam_reorder(table, lens, i32([0, 1, 2, 3, 3]), refs, k, v)
+    assert t.tolist() == [[0, 5, -1, -1], [0, 1, 2, -1], [0, 6, -1, -1], [3, 4, -1, -1], [3, 7, -1, -1]]
+    assert c.tolist() == [3, 1, 1, 2, 1, 1, 1, 1, 0] and status.tolist() == [3, 0]
+    for dst, src, fill in ((5, 1, 4), (6, 1, 5), (7, 4, 2)):
+        assert torch.equal(k[0, dst, :fill], old[src][:fill])
+    # the rows' next tokens leave the other rows' as they are
+    rows = torch.ones((5, 2, 64), device="cuda")
+    paged_append(rows, rows, k[0], v[0], t, n + 1)
+    assert torch.equal(k[0, 1], old[1]) and torch.equal(k[0, 0], old[0])
+    assert torch.equal(k[0, 2, :8], old[2][:8]) and bool((k[0, 2, 8] == 1).all())
+
+
+def test_reorder_keeps_a_last_page_of_rows_of_different_lengths():
+    """A last page that only last pages share stays with the lowest row."""
+    torch = _torch()
+    from tokenvector.inference_b200.generation import beam_reorder
+    k = torch.zeros((1, 6, 16, 2, 64), device="cuda").half()
+    t, n, c, status = beam_reorder(i32([[0, 1, -1], [0, 1, -1], [2, -1, -1]]), i32([20, 25, 0]), i32([1, 0, 2]),
+                                   i32([2, 2, 0, 0, 0, 0]), k, k.clone())
+    assert t.tolist() == [[0, 1, -1], [0, 2, -1], [3, -1, -1]] and c.tolist() == [2, 1, 1, 1, 0, 0]
+    assert status.tolist() == [2, 0]

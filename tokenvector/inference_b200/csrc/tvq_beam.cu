@@ -456,12 +456,14 @@ __device__ __forceinline__ void cluster_sync() {
 // the atomics of one SM (one address a cycle), so a cluster of eight CTAs does
 // large ones (256 rows: 13 us, one CTA 25), and one CTA small ones, where a
 // barrier across the cluster costs more (4 rows: 6 us, the cluster 9); both in
-// three phases.  (The new tables themselves are written by the next kernel.)  held[page]: how often
-// the old tables hold it; owner[page]: the lowest new row whose tail it is.
+// three phases.  (The new tables themselves are written by the next kernel.)  full[page], part[page]:
+// how often the old tables hold it as a full page and as a part-filled one; owner[page]: the lowest new
+// row whose tail it is.  A page that some row holds as a full one is nobody's to go on in, also where
+// another row ends in it (rows of different lengths that share a prefix).
 template <int RC>
 __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
-    reorder_tables_kernel(const BeamReorderArgs a, int* held, int* owner, int* freelist, RowPlan* rows, PageCopy* copies,
-                          int* n_copies, int* err) {
+    reorder_tables_kernel(const BeamReorderArgs a, int* full, int* part, int* owner, int* freelist, RowPlan* rows,
+                          PageCopy* copies, int* n_copies, int* err) {
     __shared__ uint32_t sm[32];
     griddep_wait();
     griddep_launch();
@@ -483,7 +485,7 @@ __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
 
     // ---- 1: counters; the first free pages, at most one for each new row
     for (int64_t i = g; i < a.n_pages; i += ALL) {
-        held[i] = 0;
+        full[i] = part[i] = 0;
         owner[i] = INT_MAX;
     }
     int found = 0;
@@ -515,7 +517,8 @@ __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
         }
 #pragma unroll
         for (int k = 0; k < B; k++)
-            if (cc[k] < used(len[k]) && pg[k] >= 0 && pg[k] < a.n_pages) atomicAdd(held + pg[k], 1);
+            if (cc[k] < used(len[k]) && pg[k] >= 0 && pg[k] < a.n_pages)
+                atomicAdd((cc[k] < len[k] >> log2 ? full : part) + pg[k], 1);
     }
     for (int r = g; r < a.new_rows; r += ALL) {
         const int q = a.parents[r];
@@ -543,24 +546,25 @@ __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
         for (int r0 = 0; r0 < a.new_rows; r0 += RT) {
             const int r = r0 + t;
             RowPlan p{-1, 0, -1, -1};
-            bool keeps = false, part = false;
+            bool filled = false, keeps = false;  // it ends in a part-filled page, and stays there
             int fill = 0;
             if (r < a.new_rows) {
                 const int4 w = __ldcg(reinterpret_cast<const int4*>(rows + r));
                 p = RowPlan{w.x, w.y, w.z, w.w};
-                part = p.page >= 0;
+                filled = p.page >= 0;
                 fill = __ldcg(a.new_lens + r) & (a.page - 1);
-                keeps = part && __ldcg(owner + p.page) == r && a.refs[p.page] == __ldcg(held + p.page);
+                keeps = filled && __ldcg(owner + p.page) == r && __ldcg(full + p.page) == 0 &&
+                        a.refs[p.page] == __ldcg(part + p.page);
             }
             const bool fresh = p.parent >= 0 && !keeps && p.at < a.cols;
             uint32_t all;
             const int turn = taken + static_cast<int>(block_scan(fresh, sm, &all));
             const bool got = fresh && turn < found;
             taken += static_cast<int>(all);
-            const uint32_t mine = (got && part) | (p.parent >= 0 && !keeps && !got ? 0x10000u : 0u);
+            const uint32_t mine = (got && filled) | (p.parent >= 0 && !keeps && !got ? 0x10000u : 0u);
             const uint32_t before = block_scan(mine, sm, &all);
             const int page = got ? __ldcg(freelist + turn) : -1;
-            if (got && part) copies[copied + (before & 0xFFFFu)] = PageCopy{p.page, page, fill};
+            if (got && filled) copies[copied + (before & 0xFFFFu)] = PageCopy{p.page, page, fill};
             copied += static_cast<int>(all & 0xFFFFu);
             short_of += static_cast<int>(all >> 16);
             if (r < a.new_rows) rows[r] = RowPlan{p.parent, p.n, fresh ? p.at : -1, page};
@@ -573,7 +577,7 @@ __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
     }
     if (RC == 1 || blockIdx.x > 0)
         for (int64_t i = RC == 1 ? t : g - RT; i < a.n_pages; i += RC == 1 ? RT : ALL - RT)
-            a.new_refs[i] = a.refs[i] - __ldcg(held + i);
+            a.new_refs[i] = a.refs[i] - __ldcg(full + i) - __ldcg(part + i);
 }
 
 // The new tables and what they hold, and the filled part of the pages that
@@ -695,7 +699,7 @@ int launch_beam_select(const BeamSelectArgs& a, cudaStream_t st) {
 }
 
 int beam_reorder_workspace(const BeamReorderArgs& a, int64_t* bytes) {
-    *bytes = 256 + 2 * up256(a.n_pages * 4) + up256(a.new_rows * 4ll) + up256(a.new_rows * 16ll) + up256(a.new_rows * 12ll);
+    *bytes = 256 + 3 * up256(a.n_pages * 4) + up256(a.new_rows * 4ll) + up256(a.new_rows * 16ll) + up256(a.new_rows * 12ll);
     return TVQ_OK;
 }
 
@@ -710,14 +714,15 @@ int launch_beam_reorder(const BeamReorderArgs& a, cudaStream_t st) {
         return p;
     };
     int* n_copies = reinterpret_cast<int*>(take(4));
-    int* held = reinterpret_cast<int*>(take(a.n_pages * 4));
+    int* full = reinterpret_cast<int*>(take(a.n_pages * 4));
+    int* part = reinterpret_cast<int*>(take(a.n_pages * 4));
     int* owner = reinterpret_cast<int*>(take(a.n_pages * 4));
     int* freelist = reinterpret_cast<int*>(take(a.new_rows * 4ll));
     RowPlan* rows = reinterpret_cast<RowPlan*>(take(a.new_rows * 16ll));
     PageCopy* copies = reinterpret_cast<PageCopy*>(take(a.new_rows * 12ll));
     const bool small = static_cast<int64_t>(std::max(a.rows, a.new_rows)) * a.cols <= 2 * RT && a.n_pages <= 16 * RT;
     rc = launch_pdl(small ? reorder_tables_kernel<1> : reorder_tables_kernel<8>, dim3(small ? 1 : 8), dim3(RT), 0, st, a,
-                    held, owner, freelist, rows, copies, n_copies, ds->d_error);
+                    full, part, owner, freelist, rows, copies, n_copies, ds->d_error);
     if (rc || a.new_rows == 0) return rc;
     const int64_t items = std::max<int64_t>(2ll * a.new_rows * a.layers, (static_cast<int64_t>(a.new_rows) * a.cols + CT - 1) / CT);
     if (items == 0) return rc;

@@ -31,8 +31,8 @@ def beam_reorder(table, lens, parents, refs, k_pages, v_pages):
     hold each page), k_pages and v_pages the cache of every layer [layers,
     pages, page, kv_heads, head_dim].  Full pages are shared.  A part-filled
     last page stays with the lowest row that has it, if nobody but the old
-    tables holds it; the other rows take a free page and its filled tokens are
-    copied (in k_pages and v_pages themselves, in every layer).  Behind a full
+    tables holds it, and none of their rows as a full page; the other rows take
+    a free page and its filled tokens are copied (in k_pages and v_pages themselves, in every layer).  Behind a full
     page comes a free page.  Free are the pages with refs 0 before the call,
     the lowest first.  Returns (table, lens, refs, status), all new; status
     int32 [2] = (pages taken, rows left without room: their next entry is -1)."""
