@@ -417,7 +417,8 @@ TVQ_API int tvq_matmul_int4_grouped(const float* A, const uint8_t* packed_w, con
  * multiple of 8 up to 128, values of `type` (F16 or BF16).  strides (host, in
  * elements) = {k page, k token, k head, v page, v token, v head}, multiples
  * of 8 (a token's head is contiguous; bases 16-byte aligned), so pages may be
- * [page, heads, dim] or [heads, page, dim] inside, with gaps.  Sequence s holds
+ * [page, heads, dim] or [heads, page, dim] inside, with gaps; where the cache
+ * is written, no stride of more than one entry is 0.  Sequence s holds
  * ctx_len[s] tokens, token j in page table[s * table_stride + j / page], slot
  * j % page; cols = columns of the table (table_stride 0: all sequences share
  * one row of it; else at least cols).  Its new rows are the packed rows

@@ -94,3 +94,28 @@ def test_generator_refuses_weights_of_another_shape(change):
     session = SimpleNamespace(cfg=GPT2Config(**cfg), device=0)
     with pytest.raises(ValueError, match="shape"):
         GPT2Generator(session, GPT2Weights.random(GPT2Config(**{**cfg, **change})))
+
+
+# ---------------------------------------------------------------- caches that are written
+@pytest.mark.parametrize("place", range(6))
+def test_append_refuses_a_cache_whose_entries_coincide(place):
+    def append(shape, strides):
+        return N.lib().tvq_dev_paged_append(N.TYPE_F16, N.TYPE_F32, FAKE, FAKE, None, i64(128, 64, 128, 64, 0, 0), 0, None,
+                                            FAKE, FAKE, i64(*shape), i64(*strides), FAKE, 4, 4, FAKE, None, 3, 3, None)
+    strides = [2048, 128, 64, 2048, 128, 64]
+    strides[place] = 0
+    assert append((10, 16, 2, 64), strides) == N.TVQ_ERR_INVALID and "strides of 0" in N.last_error()
+
+
+@pytest.mark.parametrize("place", range(8))
+def test_reorder_refuses_a_cache_whose_entries_coincide(place):
+    strides = [20480, 2048, 128, 64] * 2
+    strides[place] = 0
+    apart = C.c_void_p(8192)
+
+    def reorder(layers):
+        return N.lib().tvq_dev_beam_reorder(FAKE, 4, FAKE, 3, 4, FAKE, 3, FAKE, FAKE, FAKE, i64(10, 16, 2, 64, layers),
+                                            i64(*strides), apart, apart, apart, FAKE, None, 0, None)
+    assert reorder(3) == N.TVQ_ERR_INVALID and "strides of 0" in N.last_error()
+    if place % 4 == 0:  # of a single layer any stride will do
+        assert reorder(1) == N.TVQ_ERR_SIZE and "workspace" in N.last_error()

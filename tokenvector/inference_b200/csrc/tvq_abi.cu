@@ -1544,6 +1544,12 @@ int paged_view(tvq::PagedView& c, int type, void* k, void* v, const int64_t* sha
     return TVQ_OK;
 }
 
+// A cache that is written: no two of its entries are one (a stride of 0, as expanded tensors have).
+int check_apart(int64_t size, int64_t stride) {
+    TVQ_CHECK(size <= 1 || stride > 0, TVQ_ERR_INVALID, "a cache that is written must not have strides of 0");
+    return TVQ_OK;
+}
+
 int check_ws(const void* ws, int64_t have, int64_t need) {
     TVQ_CHECK(have >= need, TVQ_ERR_SIZE, "workspace too small");
     TVQ_CHECK(need == 0 || (ws && (reinterpret_cast<uintptr_t>(ws) & 255) == 0), TVQ_ERR_INVALID,
@@ -1581,6 +1587,7 @@ int tvq_dev_paged_append(int type, int src_type, const void* k, const void* v, c
     TVQ_CHECK(q_heads >= 0 && q_heads <= 65535, TVQ_ERR_INVALID, "q heads out of range");
     if (n_rows == 0) return TVQ_OK;
     TVQ_CHECK(k && v && (!q || q_out), TVQ_ERR_INVALID, "null buffer");
+    for (int i = 0; i < 6; i++) STEP(check_apart(shape[i % 3], strides[i]));
     TVQ_CHECK(aligned16(k) && aligned16(v) && aligned16(q) && aligned16(q_out), TVQ_ERR_UNSUPPORTED,
               "rows must be 16-byte aligned");
     const int64_t unit = src_type == TVQ_TYPE_F32 ? 4 : 8;
@@ -1743,9 +1750,11 @@ int tvq_dev_beam_reorder(const int32_t* table, int64_t table_stride, const int32
     if (shape[4] > 0 && shape[0] > 0) {
         TVQ_CHECK(k_pages && v_pages, TVQ_ERR_INVALID, "null buffer");
         TVQ_CHECK(aligned16(k_pages) && aligned16(v_pages), TVQ_ERR_UNSUPPORTED, "pages must be 16-byte aligned");
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 8; i++) {
             TVQ_CHECK(strides[i] >= 0 && strides[i] % 8 == 0, TVQ_ERR_UNSUPPORTED,
                       "cache strides must be non-negative multiples of 8 elements");
+            STEP(check_apart(i % 4 == 0 ? shape[4] : shape[i % 4 - 1], strides[i]));
+        }
     }
     a.table = table;
     a.table_stride = table_stride;
