@@ -119,3 +119,23 @@ def test_reorder_refuses_a_cache_whose_entries_coincide(place):
     assert reorder(3) == N.TVQ_ERR_INVALID and "strides of 0" in N.last_error()
     if place % 4 == 0:  # of a single layer any stride will do
         assert reorder(1) == N.TVQ_ERR_SIZE and "workspace" in N.last_error()
+
+
+# ---------------------------------------------------------------- gradients
+def test_operators_without_a_backward_pass_say_so():
+    torch = pytest.importorskip("torch")
+    from tokenvector.inference_b200 import generation as G
+    k = torch.zeros((4, 16, 2, 64), dtype=torch.float16)
+    t, n = torch.zeros((1, 2), dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    row, x, scores = torch.zeros((1, 2, 64), dtype=torch.float16), torch.zeros((4, 9)), torch.zeros(4)
+    grad = lambda a: a.clone().requires_grad_()  # noqa: E731
+    calls = [lambda: G.paged_attention(grad(row), k, k, t, n), lambda: G.paged_attention(row, grad(k), k, t, n),
+             lambda: G.paged_attention(row, k, grad(k), t, n), lambda: G.paged_append(grad(row), row, k, k, t, n),
+             lambda: G.paged_append(row, grad(row), k, k, t, n), lambda: G.paged_append(row, row, k, grad(k), t, n),
+             lambda: G.paged_append(row, row, k, k, t, n, q=grad(row)), lambda: G.beam_select(grad(x), scores, 4, 4),
+             lambda: G.beam_select(x, grad(scores), 4, 4), lambda: G.beam_reorder(t, n, n, n, grad(k[None]), k[None])]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # (as far as the next check)
+            call()

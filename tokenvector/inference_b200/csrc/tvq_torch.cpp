@@ -63,6 +63,16 @@ int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 
+// The operators have no backward pass: an output that a gradient is expected of would silently have none.
+void no_grad(const Tensor& t, const char* name) {
+    if (t.requires_grad() && at::GradMode::is_enabled())
+        throw py::value_error(std::string(name) + " requires a gradient, which this operator does not have: detach it, or "
+                                                  "call under torch.no_grad()");
+}
+void no_grad(const OptTensor& t, const char* name) {
+    if (t) no_grad(*t, name);
+}
+
 // Scratch of one call (stream-ordered memory of torch's allocator).
 Tensor workspace(at::Device dev, int64_t bytes) {
     return at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
@@ -76,6 +86,8 @@ struct Cache {
     int64_t table_stride, cols, seqs;
 };
 Cache cache_of(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& ctx, const OptTensor& cu, int64_t n_rows) {
+    no_grad(k, "k_pages");
+    no_grad(v, "v_pages");
     need(k.is_cuda(), "the cache must be on a CUDA device");
     Cache c;
     c.type = type_of(k);
@@ -117,6 +129,9 @@ void rows_of(const Tensor& t, int64_t heads, int64_t dim, const char* name) {
 
 OptTensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
                        const Tensor& ctx_len, const OptTensor& cu, const OptTensor& q) {
+    no_grad(k, "k");
+    no_grad(v, "v");
+    no_grad(q, "q");
     need(k.dim() == 3, "k must be [rows, heads, head_dim] like the cache");
     const Cache c = cache_of(k_pages, v_pages, table, ctx_len, cu, k.size(0));
     rows_of(k, c.shape[2], c.shape[3], "k");
@@ -148,6 +163,7 @@ std::tuple<Tensor, OptTensor> paged_attention(const Tensor& q, const Tensor& k_p
                                               const Tensor& ctx_len, const OptTensor& cu, std::optional<int64_t> max_q,
                                               std::optional<double> scale, int64_t window, const OptTensor& given,
                                               bool return_lse) {
+    no_grad(q, "q");
     need(q.dim() == 3, "q must be [rows, heads, head_dim] like the cache");
     const int64_t n_rows = q.size(0), heads = q.size(1);
     const Cache c = cache_of(k_pages, v_pages, table, ctx_len, cu, n_rows);
@@ -183,6 +199,8 @@ std::tuple<Tensor, OptTensor> paged_attention(const Tensor& q, const Tensor& k_p
 
 std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits, const Tensor& scores, int64_t beams, int64_t keep,
                                                const OptTensor& finished, std::optional<int64_t> eos) {
+    no_grad(logits, "logits");
+    no_grad(scores, "scores");
     need(logits.dim() == 2 && type_of(logits) >= 0 && logits.is_cuda(),
          "logits must be a [rows, vocab] tensor of floats on a CUDA device");
     const int64_t rows = logits.size(0), vocab = logits.size(1);
@@ -217,6 +235,8 @@ std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits, const Tenso
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> beam_reorder(const Tensor& table, const Tensor& lens, const Tensor& parents,
                                                         const Tensor& refs, const Tensor& k, const Tensor& v) {
+    no_grad(k, "k_pages");
+    no_grad(v, "v_pages");
     const int32_t* table_p = i32_of(table, 2, "table");
     const int32_t* lens_p = i32_of(lens, 1, "lens");
     const int32_t* parents_p = i32_of(parents, 1, "parents");
