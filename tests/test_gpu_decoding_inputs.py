@@ -193,3 +193,42 @@ def test_reorder_keeps_a_last_page_of_rows_of_different_lengths():
                                    i32([2, 2, 0, 0, 0, 0]), k, k.clone())
     assert t.tolist() == [[0, 1, -1], [0, 2, -1], [3, -1, -1]] and c.tolist() == [2, 1, 1, 1, 0, 0]
     assert status.tolist() == [2, 0]
+
+
+# ---------------------------------------------------------------- caches without pages, tables without columns
+@pytest.mark.parametrize("cols", [0, 2])
+@pytest.mark.parametrize("new,dim,page", [(1, 64, 16), (1, 128, 16), (1, 80, 8), (40, 64, 16), (40, 128, 128)])
+def test_an_empty_cache_holds_empty_sequences(new, dim, page, cols):
+    """Rows in front of the cache's first token: nothing to read or to write; a token that should be there is reported."""
+    import math
+
+    from test_gpu_paged import clean
+    from tokenvector.inference_b200 import _native as N
+    from tokenvector.inference_b200.generation import paged_append, paged_attention
+    torch = _torch()
+    k = torch.empty((0, page, 2, dim), dtype=torch.float16, device="cuda")
+    table = torch.full((2, cols), 3, dtype=torch.int32, device="cuda")
+    q = torch.ones((2 * new, 4, dim), dtype=torch.float16, device="cuda")
+    cu, rows = i32([0, new, 2 * new]), q[:, :2].float()
+    clean()
+    for ctx in ([0, 0], [0, 5]):
+        out, lse = paged_attention(q, k, k, table, i32(ctx), cu, max_q=new, return_lse=True)
+        assert not out.any() and bool((lse[:new] == -math.inf).all())
+        if ctx[1] == 0:
+            assert bool((lse == -math.inf).all())
+            paged_append(rows, rows, k, k.clone(), table, i32(ctx), cu)
+            clean()
+        else:
+            assert N.lib().tvq_device_error(None) == N.TVQ_ERR_INVALID and "page" in N.last_error()
+            assert abs(float(lse[-1, 0]) - math.log(5)) < 1e-5  # five keys of zeros
+            paged_append(rows, rows, k, k.clone(), table, i32(ctx), cu)
+            assert N.lib().tvq_device_error(None) == N.TVQ_ERR_INVALID and "page" in N.last_error()
+    clean()
+
+
+def test_reorder_without_pages():
+    torch = _torch()
+    from tokenvector.inference_b200.generation import beam_reorder
+    k = torch.empty((2, 0, 16, 2, 64), dtype=torch.float16, device="cuda")
+    t, n, c, status = beam_reorder(i32([[-1, -1]] * 2), i32([0, 0]), i32([1, 0, -1]), i32([]), k, k.clone())
+    assert t.tolist() == [[-1, -1]] * 3 and n.tolist() == [0, 0, 0] and c.numel() == 0 and status.tolist() == [0, 2]

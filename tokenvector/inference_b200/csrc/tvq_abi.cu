@@ -1514,7 +1514,8 @@ int paged_view(tvq::PagedView& c, int type, void* k, void* v, const int64_t* sha
     TVQ_CHECK(cu || n_rows == n_seq, TVQ_ERR_SIZE, "without cu every sequence has one row");
     TVQ_CHECK(table_stride == 0 || table_stride >= cols, TVQ_ERR_SIZE, "table_stride smaller than the table's columns");
     if (n_rows > 0) {
-        TVQ_CHECK(n_seq > 0 && table && ctx && (shape[0] == 0 || (k && v)), TVQ_ERR_INVALID, "null buffer");
+        TVQ_CHECK(n_seq > 0 && (cols == 0 || table) && ctx && (shape[0] == 0 || (k && v)), TVQ_ERR_INVALID,
+                  "null buffer");
         TVQ_CHECK(aligned16(k) && aligned16(v), TVQ_ERR_UNSUPPORTED, "pages must be 16-byte aligned");
         for (int i = 0; i < 6; i++)
             TVQ_CHECK(strides[i] >= 0 && strides[i] % 8 == 0, TVQ_ERR_UNSUPPORTED,

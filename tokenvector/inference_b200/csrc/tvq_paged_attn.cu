@@ -1078,13 +1078,13 @@ __global__ void __launch_bounds__(TTHR, 1)
                 for (int j = w.a; ok && j < end; j++) {
                     int now = page;
                     page = look(j + 1);
-                    if (static_cast<unsigned>(now) >= static_cast<unsigned>(a.c.n_pages)) {
-                        record_error(err, DEVERR_BAD_PAGE);
-                        now = -1;  // outside the tensor map: zeros
-                    }
-                    // (a box behind the sequence's end or before all windows is not read either)
                     const int key = j * TKEYS + b * plan.box;
-                    if (key >= len || key + plan.box <= low) now = -1;
+                    if (key >= len || key + plan.box <= low) {
+                        now = -1;  // behind the sequence's end or before all windows: outside the tensor map, zeros
+                    } else if (issues && static_cast<unsigned>(now) >= static_cast<unsigned>(a.c.n_pages)) {
+                        record_error(err, DEVERR_BAD_PAGE);
+                        now = -1;
+                    }
                     const int slot = key & (a.c.page - 1);
                     for (int v = 0; v < 2; v++) {
                         ok = __all_sync(0xffffffffu, wait_bar(kv_empty + stage, phase, err, DEVERR_PTILE_EMPTY));
@@ -1628,13 +1628,17 @@ namespace {
 
 // The cache as a {value, token, half, head, page} tensor map, boxes of 64
 // values x `box` tokens x `halves` (128-byte swizzle).  A head dim that is no
-// multiple of 64 stays one dimension, so that nothing behind it is read.
-int cache_map(CUtensorMap* map, const PagedView& c, const void* ptr, int64_t tok, int64_t head, int64_t page, int box,
+// multiple of 64 stays one dimension, so that nothing behind it is read.  A
+// cache without pages has one in its map, at any address: the kernels check
+// page numbers against n_pages and ask for page -1, zeros, instead.
+int cache_map(CUtensorMap* map, const PagedAttnArgs& a, const void* ptr, int64_t tok, int64_t head, int64_t page, int box,
               int halves) {
+    const PagedView& c = a.c;
+    if (c.n_pages == 0) ptr = a.out;
     const bool whole = c.dim % 64 == 0;
     const uint64_t dims[5] = {static_cast<uint64_t>(whole ? 64 : c.dim), static_cast<uint64_t>(c.page),
                               static_cast<uint64_t>(whole ? c.dim / 64 : 1), static_cast<uint64_t>(c.kv_heads),
-                              static_cast<uint64_t>(c.n_pages)};
+                              static_cast<uint64_t>(std::max<int64_t>(c.n_pages, 1))};
     const uint64_t strides[4] = {static_cast<uint64_t>(tok) * 2, 128, static_cast<uint64_t>(head) * 2,
                                  static_cast<uint64_t>(page) * 2};
     const uint32_t boxes[5] = {64, static_cast<uint32_t>(box), static_cast<uint32_t>(halves), 1, 1};
@@ -1656,9 +1660,9 @@ int launch_rows(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     plan.by_value = a.c.dim % 64 != 0;
     plan.box_halves = a.c.dim == 128 && plan.box == C::KT ? 2 : 1;
     CUtensorMap tmK, tmV;
-    rc = cache_map(&tmK, a.c, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
+    rc = cache_map(&tmK, a, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
     if (rc) return rc;
-    rc = cache_map(&tmV, a.c, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
+    rc = cache_map(&tmV, a, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
     if (rc) return rc;
     rc = launch_pdl(attn_rows_kernel<T, DP>, dim3(ds->sm_count), dim3(NTHR), C::SMEM, st, tmK, tmV, a, plan,
                     ds->d_error);
@@ -1696,9 +1700,9 @@ int launch_tiles(const PagedAttnArgs& a, DeviceState* ds, cudaStream_t st) {
     const uint32_t box[4] = {64, 1, static_cast<uint32_t>(group), static_cast<uint32_t>(plan.tokens)};
     rc = make_tma_16bit(&tmQ, a.q, 4, dims, strides, box);
     if (rc) return rc;
-    rc = cache_map(&tmK, a.c, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
+    rc = cache_map(&tmK, a, a.c.k, a.c.k_tok, a.c.k_head, a.c.k_page, plan.box, plan.box_halves);
     if (rc) return rc;
-    rc = cache_map(&tmV, a.c, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
+    rc = cache_map(&tmV, a, a.c.v, a.c.v_tok, a.c.v_head, a.c.v_page, plan.box, plan.box_halves);
     if (rc) return rc;
     rc = launch_pdl(attn_tile_kernel<T, DP>, dim3(ds->sm_count), dim3(TTHR), C::SMEM, st, tmQ, tmK, tmV, a, plan,
                     ds->d_error);
