@@ -46,3 +46,21 @@ def test_weights_of_another_float_type_are_the_same_model(model):  # noqa: F811
                    layers=[{k: a.astype(np.float64) if k in names else a for k, a in L.items()} for L in w.layers])
     ids = [3, 1, 4, 1, 5, 9, 2, 6]
     assert torch.equal(GPT2Generator(s, wide).log_probs(ids), g.log_probs(ids))
+
+
+def test_continuations_end_with_eos(model):  # noqa: F811
+    """eos is a token of the best continuation without one: with it that continuation ends there, with its own score
+    (the tolerance a token of test_gpu_generation), and the others go on."""
+    from test_gpu_generation import TOL
+    cfg, w, s, g = model
+    prompt = np.random.default_rng(7).integers(0, cfg.vocab, 19).tolist()
+    free = g.generate([prompt], 3, 20)[0]
+    at = 3
+    eos = free[0][0][at]
+    found = g.generate([prompt], 3, 20, eos=eos)[0]
+    ended = [(t, sc) for t, sc in found if t[-1] == eos and len(t) < 20]
+    assert ended
+    for t, sc in found:
+        assert eos not in t[:-1] and (t[-1] == eos or len(t) == 20)
+        own = float(g.log_probs(prompt + t)[len(prompt) - 1:].sum())
+        assert abs(own - sc) <= TOL * len(t), (own, sc)
