@@ -1373,8 +1373,26 @@ __global__ void __launch_bounds__(TTHR, 1)
                     if (grow) m = tile;
                 }
                 if (m == -INFINITY) m = tile;
-                const float base = m == -INFINITY ? 0.0f : m * scale2;
-                const uint64_t scale22 = f2_pack(scale2, scale2), base2 = f2_pack(-base, -base);
+                // One FMA makes the exponent scale2 s - scale2 m.  Where the bits of scale2 m end above 2^-4 its
+                // rounding is off by whole powers of two: there m is subtracted from the scores first, where they are.
+                float base = m == -INFINITY ? 0.0f : -m * scale2;
+                if (__any_sync(0xffffffffu, fabsf(base) > 1048576.0f)) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t s[16];
+                        tmem_ld16(s_addr + c * 16, s);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; e++) s[e] = __float_as_uint(__uint_as_float(s[e]) - (m == -INFINITY ? 0.0f : m));
+                        tmem_st16(s_addr + c * 16, s);
+                    }
+                    tmem_st_wait();
+                    tmem_ld32(s_addr, s0);
+                    tmem_ld_wait();
+                    if (edge) hide(0, s0);
+                    base = 0.0f;
+                }
+                const uint64_t scale22 = f2_pack(scale2, scale2), base2 = f2_pack(base, base);
                 uint64_t sum2[2] = {0ull, 0ull};
                 // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
                 // rounding of the result; l sums them unrounded
