@@ -453,7 +453,8 @@ TVQ_API int tvq_dev_paged_append(int type, int src_type, const void* k, const vo
  * see it (positions up to 127 before it: a tile's masked weights are zeros,
  * and 0 x inf is NaN).  Products are summed in f32; the softmax's
  * weights are rounded to `type` before they meet V (relative 2^-11 / 2^-8
- * each), its statistics stay f32.  The same call gives the same bits.
+ * each; F16 ones not finer than 2^-40 of the row's largest each where max_q *
+ * q_heads / kv heads <= 16, else 2^-32), its statistics stay f32.  The same call gives the same bits.
  * ws: at least tvq_paged_attention_workspace bytes, 256-byte aligned, used by
  * one call at a time; nothing in it has to last from call to call. */
 TVQ_API int tvq_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t n_seq,

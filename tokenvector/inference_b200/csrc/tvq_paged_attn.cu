@@ -72,6 +72,16 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// The softmax's weights meet V in its type, as multiples of 2^-24 at the
+// smallest in float16.  A factor 2^UP, which the sum l carries as well, keeps
+// the largest (1, or the tile kernel's 2^8) just within the type's 65504, so
+// that a weight is whole down to 2^(-14 - UP) of the largest and counts down to
+// 2^(-25 - UP): many keys beside one that has nearly all the weight are not
+// lost.  It costs nothing, the exponent's offset being subtracted in any case.
+// (bfloat16 has float's range.)
+template <typename T, int LARGEST>  // log2 of the largest weight
+constexpr int UP = std::is_same<T, __half>::value ? 15 - LARGEST : 0;
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
@@ -430,6 +440,7 @@ __global__ void __launch_bounds__(NTHR, 1)
 
     // ---------------------------------------------------- consumers
     const float scale2 = a.scale * 1.4426950408889634f;
+    constexpr float up = UP<T, 0>, down = 1.0f / (1 << UP<T, 0>);
     const int g = lane >> 2, quad = lane & 3;
     int stage = 0, phase = 0;
     bool ok = true;
@@ -506,8 +517,9 @@ __global__ void __launch_bounds__(NTHR, 1)
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float m2 = fmaxf(m[hf], top);
-                const float base = m2 == -INFINITY ? 0.0f : m2;
-                const float f = ex2(m[hf] - base);
+                // (rounded up: not even the rounding of huge scores makes a weight larger than 2^up)
+                const float to = m2 == -INFINITY ? 0.0f : m2, base = __fadd_ru(to, -up);
+                const float f = ex2(m[hf] - to);
                 m[hf] = m2;
                 float sum = 0.0f;
 #pragma unroll
@@ -516,7 +528,7 @@ __global__ void __launch_bounds__(NTHR, 1)
                     sum += x[e];
                 }
                 l[hf] = l[hf] * f + sum;
-                // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
+                // the weights meet V in its own type (see UP): 2^-11 (f16) or 2^-8 (bf16) of each, as the
                 // rounding of the result; l sums them unrounded
 #pragma unroll
                 for (int n = 0; n < KT / 16; n++) {
@@ -574,16 +586,16 @@ __global__ void __launch_bounds__(NTHR, 1)
                     if (n * 8 < a.c.dim)
                         *reinterpret_cast<uint32_t*>(out + n * 8) = pack2<T>(o[n][hf * 2] * inv, o[n][hf * 2 + 1] * inv);
                 if (quad == 0 && a.lse)
-                    a.lse[at[hf]] = sum == 0.0f ? -INFINITY : (m[hf] + log2f(sum)) * 0.6931471805599453f;
+                    a.lse[at[hf]] = sum == 0.0f ? -INFINITY : (m[hf] + log2f(sum * down)) * 0.6931471805599453f;
             } else {
                 float* out = reinterpret_cast<float*>(part) + r * DP + quad * 2;
 #pragma unroll
                 for (int n = 0; n < DP / 8; n++)
                     if (n * 8 < a.c.dim)
-                        *reinterpret_cast<float2*>(out + n * 8) = make_float2(o[n][hf * 2], o[n][hf * 2 + 1]);
+                        *reinterpret_cast<float2*>(out + n * 8) = make_float2(o[n][hf * 2] * down, o[n][hf * 2 + 1] * down);
                 if (quad == 0)
                     *reinterpret_cast<float2*>(part + (static_cast<int64_t>(plan.rows_cap) * DP * 4 + r * 8)) =
-                        make_float2(m[hf], sum);
+                        make_float2(m[hf], sum * down);
             }
         }
     }
@@ -711,7 +723,7 @@ __global__ void __launch_bounds__(JW * 32, 6) attn_join_kernel(const PagedAttnAr
 //                its instructions waited 1.4 cycles each for one another)
 // O stays relative to the row's first maximum until the running one exceeds it
 // by 2^8 (then O and l are scaled by the softmax warps): weights stay below
-// 2^8, exact enough in either 16-bit type, and nearly no tile is scaled twice.
+// 2^8, within either 16-bit type (see UP), and nearly no tile is scaled twice.
 // The weights of the first 32 keys of each thread are handed over by themselves,
 // so that half of PV runs while the other weights are made (414 -> 403 us below).
 // A commit of S_t(j) covers PV_t(j-1), issued before it, so scaling O needs no
@@ -1300,6 +1312,7 @@ __global__ void __launch_bounds__(TTHR, 1)
         const float* x_b = reinterpret_cast<float*>(sm + C::OFF_X) + 2 * 128 + row;  // tile B's, at a unit's end
         const uint32_t pair_bar = 1 + t * 4 + wl;  // of the two warps that share 32 rows
         const float scale2 = plan.scale2;
+        constexpr float up = UP<T, 8>, down = 1.0f / (1 << UP<T, 8>);
         const int ri = row / group, gi = row - ri * group;  // this row's token of the tile, its head of the group
         int ns = 0, no = 0, nd = 0;
         // (both warps of a pair go on, or neither: they meet at barriers)
@@ -1373,9 +1386,9 @@ __global__ void __launch_bounds__(TTHR, 1)
                     if (grow) m = tile;
                 }
                 if (m == -INFINITY) m = tile;
-                // One FMA makes the exponent scale2 s - scale2 m.  Where the bits of scale2 m end above 2^-4 its
+                // One FMA makes the exponent scale2 s - scale2 m + up.  Where the bits of scale2 m end above 2^-4 its
                 // rounding is off by whole powers of two: there m is subtracted from the scores first, where they are.
-                float base = m == -INFINITY ? 0.0f : -m * scale2;
+                float base = m == -INFINITY ? up : up - m * scale2;
                 if (__any_sync(0xffffffffu, fabsf(base) > 1048576.0f)) {
 #pragma unroll 1
                     for (int c = 0; c < 4; c++) {
@@ -1390,11 +1403,11 @@ __global__ void __launch_bounds__(TTHR, 1)
                     tmem_ld32(s_addr, s0);
                     tmem_ld_wait();
                     if (edge) hide(0, s0);
-                    base = 0.0f;
+                    base = up;
                 }
                 const uint64_t scale22 = f2_pack(scale2, scale2), base2 = f2_pack(base, base);
                 uint64_t sum2[2] = {0ull, 0ull};
-                // the weights meet V in its own type: 2^-11 (f16) or 2^-8 (bf16) of each, as the
+                // the weights meet V in its own type (see UP): 2^-11 (f16) or 2^-8 (bf16) of each, as the
                 // rounding of the result; l sums them unrounded
                 auto weigh = [&](int c, const uint32_t (&s)[32]) {  // (their columns lie within the scores read so far)
                     uint32_t p[16];
@@ -1461,7 +1474,7 @@ __global__ void __launch_bounds__(TTHR, 1)
             }
             const bool both = dup && w.lo[1] < w.hi[1];
             if (lo < hi && !(dup && t == 1)) {
-                const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : down;
                 const float ga = fa * inv, gb = fb * inv;
                 const int odd = lane & 1;
                 const int64_t own = valid ? at : -1, other = __shfl_xor_sync(0xffffffffu, own, 1);
@@ -1504,9 +1517,9 @@ __global__ void __launch_bounds__(TTHR, 1)
                 tc_fence_before();
             }
             if (half == 0 && !(dup && t == 1)) {
-                if (valid && whole && a.lse) a.lse[at] = l == 0.0f ? -INFINITY : (mt + log2f(l)) * 0.6931471805599453f;
+                if (valid && whole && a.lse) a.lse[at] = l == 0.0f ? -INFINITY : (mt + log2f(l * down)) * 0.6931471805599453f;
                 if (valid && !whole)  // (a row tile without keys in the piece: m -inf)
-                    *reinterpret_cast<float2*>(part + 2 * TM * DP * 4 + (t * TM + row) * 8) = make_float2(mt, l);
+                    *reinterpret_cast<float2*>(part + 2 * TM * DP * 4 + (t * TM + row) * 8) = make_float2(mt, l * down);
             }
             if (dup && t == 0) {
                 __syncwarp();
