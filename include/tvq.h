@@ -406,10 +406,11 @@ TVQ_API int tvq_matmul_int4_grouped(const float* A, const uint8_t* packed_w, con
 
 /* ================================================================ decoding
  * A paged cache of keys and values, the attention of new tokens over it, beam
- * search's choice of tokens and the reordering of the beams' caches.  No
- * counterpart in the reference, whose attention recomputes every key on every
- * call (gpt2_attention, tv/training/gpt2_ref.tkv:360-395).  Device buffers,
- * asynchronous on `stream`; lengths, tables and parents are read on the
+ * search's choice of tokens and the reordering of the beams' caches.  The
+ * reference has a cache, a paged pool and a beam search as CPU code
+ * (tv/runtime/kv_cache.tkv, tv/runtime/paged_kv.tkv, tv/text/); these entry
+ * points mirror none of their interfaces.  Device buffers, asynchronous on
+ * `stream`; lengths, tables and parents are read on the
  * device, so a decoding loop needs no host round trip.
  *
  * The cache of one layer is pages of `page` tokens: shape (host) = {pages,
@@ -448,13 +449,14 @@ TVQ_API int tvq_dev_paged_append(int type, int src_type, const void* k, const vo
  * heads share a kv head.
  * What lies in a page behind a sequence's end has no influence, and pages
  * that lie before the window of the sequence's first new row are not read
- * (their table entries may be anything).  A NaN or
- * infinity in a value of the sequence itself may also reach rows that do not
- * see it (positions up to 127 before it: a tile's masked weights are zeros,
- * and 0 x inf is NaN).  Products are summed in f32; the softmax's
- * weights are rounded to `type` before they meet V (relative 2^-11 / 2^-8
- * each; F16 ones not finer than 2^-40 of the row's largest each where max_q *
- * q_heads / kv heads <= 16, else 2^-32), its statistics stay f32.  The same call gives the same bits.
+ * (their table entries may be anything).  A NaN or infinity in a value of the
+ * sequence itself may also reach rows that do not see it (up to 254 positions
+ * before it, or as far behind the window that it has left: a tile's masked
+ * weights are zeros, and 0 x inf is NaN).  Products are summed in f32; the
+ * softmax's weights are rounded to `type` before they meet V (relative 2^-11 /
+ * 2^-8 each; F16 ones not finer than 2^-40 of the row's largest each where
+ * max_q * q_heads / kv heads <= 16, else 2^-32), its statistics stay f32.  The
+ * same call gives the same bits.
  * ws: at least tvq_paged_attention_workspace bytes, 256-byte aligned, used by
  * one call at a time; nothing in it has to last from call to call. */
 TVQ_API int tvq_paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t n_seq,

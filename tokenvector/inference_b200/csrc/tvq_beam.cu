@@ -57,8 +57,8 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 // best keys, best first.  Each logit is read once; a slice's steps are short
 // and follow one another (5026 f32 logits ~4 us with six CTAs on an SM, issue
 // slots 56 % busy), so a pass takes what one logit needs and the rest is paid
-// once a slice.  Measured with the merge: 256 rows of 50257 f32 25 us, 1024
-// rows 52 us (3.9 TB/s), 4 rows 9.8 us.  Six CTAs an SM go over the slices,
+// once a slice.  Measured with the merge: 256 rows of 50257 f32 22 us (f16 21:
+// it is not the bytes), 1024 rows 52 us (4.0 TB/s), 4 rows 8.6 us.  Six CTAs an SM go over the slices,
 // with a 32 KB buffer each that one bulk copy fills as soon as the slice before
 // has been looked through; between them there is always some at work.
 //   pass 1  the best value of every group of 4 threads (2 for keep > 32)
@@ -583,7 +583,7 @@ __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
 // rows copy, every layer, keys and values.  Bound: memory.  A thread writes one
 // entry of the tables or none, then CTAs go over (copy, layer, k or v); a
 // thread has eight 16-byte pieces on their way.  Measured with the kernel
-// before: 256 rows of 12 layers, 142 MB: 38 us, the copy 2 us a layer of it
+// before: 256 rows of 12 layers, 142 MB: 35 us, the copy 2 us a layer of it
 // (5.9 TB/s).
 constexpr int CT = 128, CU = 8;
 __global__ void __launch_bounds__(CT) reorder_copy_kernel(const BeamReorderArgs a, const RowPlan* rows,

@@ -61,8 +61,8 @@ __device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seq, int row)
 // ---------------------------------------------------------------- append
 // Bound: memory (each value is read once and written once).  One thread per
 // 8 values of one row.  Measured: 7 prompts of up to 3001 tokens, 8 heads of 128
-// and 32 of q, f32 to bf16 (499 MB): 74.5 us, 6.7 TB/s; a token of each of 64
-// beams 4.6 us.
+// and 32 of q, f32 to bf16 (499 MB): 72.9 us, 6.8 TB/s; a token of each of 64
+// beams 3.3 us.
 template <typename T, typename S>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int* err) {
     griddep_wait();

@@ -32,11 +32,11 @@
 //    bytes take ~330, so the wider tcgen05 tile (128 rows) would buy nothing.
 //  - a pair that lies in one piece is written at once; the parts of the others
 //    go to the workspace in f32, and attn_join_kernel joins them in order.
-// Measured: 24 sequences of up to 24000 tokens, 32 heads on 8 of 128: 224 us,
-// 6.2 TB/s, 94 % of a copy's rate.  48 sequences of up to 1024, 25 heads of 64,
-// whose tokens have their heads side by side: 46 us, of which ~10 are the start
-// and the join, and 128-byte pieces get 5.0 TB/s (2 KB ones 5.8).  One token
-// of one sequence of 700: 9.6 us, all latency.
+// Measured: 24 sequences of up to 24000 tokens, 32 heads on 8 of 128: 223 us,
+// 6.2 TB/s, 95 % of a copy's rate.  48 sequences of up to 1024, 25 heads of 64,
+// whose tokens have their heads side by side: 45 us, of which ~10 are the start
+// and the join, and 128-byte pieces get 4.9 TB/s (2 KB ones 5.8).  One token
+// of one sequence of 700: 8.4 us, all latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -738,9 +738,10 @@ __global__ void __launch_bounds__(JW * 32, 6) attn_join_kernel(const PagedAttnAr
 // issuer that takes whichever tile is ready, or one that starts a unit's first
 // S before the last PV of the unit before: their code comes between the
 // products, which cost the long chunk 25 % and 4 %.)
-// Measured: a chunk of 4096 tokens behind 16384, 16 heads on 4 of 128: 403 us,
-// 1194 TFLOP/s, 73 % of a large product's rate.  Nine prompts of up to 1023,
-// 12 heads of 64: 50 us, where a unit's end and the next one's first tile take
+// Measured: a chunk of 4096 tokens behind 16384, 16 heads on 4 of 128: 404 us,
+// 1191 TFLOP/s, 72 % of a large product's rate at full clock; called again and
+// again, under the power limit, 470 us, 1023 TFLOP/s, 73 % of what the product
+// sustains.  Nine prompts of up to 1023, 12 heads of 64: 51 us, where a unit's end and the next one's first tile take
 // ~4 us beside its few tiles, and the start ~6.
 constexpr int TM = 128, TKEYS = 128;
 constexpr int TTHR = 640;

@@ -6,7 +6,8 @@ with static activation scales, erf GELU, f32 residual stream, tied f32 LM
 head), called layer by layer on device buffers, with the attention replaced by
 `paged_append` and `paged_attention` over a float16 cache; `beam_select` picks
 each step's tokens and `beam_reorder` moves the beams' caches after them.
-Nothing of a step goes through the host.
+Nothing of a step goes through the host, except that with `eos` every eighth
+step asks whether all beams have ended.
 """
 from __future__ import annotations
 
