@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("kind", ["float32", "bfloat16"])
 @pytest.mark.parametrize("batch,beams,keep,vocab", [
-    (1, 16, 16, 50257), (2, 16, 64, 50257), (1, 8, 16, 128256), (1, 64, 64, 50257), (1, 64, 1, 131072), (1, 3, 64, 1 << 20)])
+    (1, 16, 16, 50257), (2, 16, 64, 50257), (1, 8, 16, 120001), (1, 64, 64, 50257), (1, 64, 1, 131072), (1, 3, 64, 1 << 20)])
 def test_choice_of_many_lists(batch, beams, keep, vocab, kind):
     import torch
     gen = torch.Generator(device="cuda").manual_seed(beams + vocab)

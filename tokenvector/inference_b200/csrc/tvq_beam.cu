@@ -455,10 +455,12 @@ __device__ __forceinline__ void cluster_sync() {
 // KB; what takes the time is the chain of reads that depend on one another, and
 // the atomics of one SM (one address a cycle), so a cluster of eight CTAs does
 // large ones, and one CTA small ones, where a barrier across the cluster costs
-// more (the rule and its figures are at the launch); both in three phases.  (The new tables themselves are written by the next kernel.)  full[page], part[page]:
-// how often the old tables hold it as a full page and as a part-filled one; owner[page]: the lowest new
-// row whose tail it is.  A page that some row holds as a full one is nobody's to go on in, also where
-// another row ends in it (rows of different lengths that share a prefix).
+// more (the rule and its figures are at the launch); both in three phases.
+// (The new tables themselves are written by the next kernel.)  full[page],
+// part[page]: how often the old tables hold it as a full page and as a
+// part-filled one; owner[page]: the lowest new row whose tail it is.  A page
+// that some row holds as a full one is nobody's to go on in, also where another
+// row ends in it (rows of different lengths that share a prefix).
 template <int RC>
 __global__ void __cluster_dims__(RC, 1, 1) __launch_bounds__(RT)
     reorder_tables_kernel(const BeamReorderArgs a, int* full, int* part, int* owner, int* freelist, RowPlan* rows,
@@ -719,9 +721,9 @@ int launch_beam_reorder(const BeamReorderArgs& a, cudaStream_t st) {
     int* freelist = reinterpret_cast<int*>(take(a.new_rows * 4ll));
     RowPlan* rows = reinterpret_cast<RowPlan*>(take(a.new_rows * 16ll));
     PageCopy* copies = reinterpret_cast<PageCopy*>(take(a.new_rows * 12ll));
-    // One CTA or the cluster, both kernels of a reorder with hardly anything to copy, one CTA and cluster: by entries of
-    // the table 92: 8.0 and 8.3 us, 736: 9.4 and 9.7, 1472: 9.7 and 9.9, 2944: 10.6 and 10.4, 5888: 13.5 and 11.2,
-    // 20288: 24.5 and 12.6; by pages (16 rows) 1000: 9.3 and 9.3, 2000: 9.9 and 9.5, 8000: 12.4 and 10.4, 64000: 33 and 11.6.
+    // One CTA and the cluster, both kernels of a reorder with hardly anything to copy: by entries of the table 92: 8.0
+    // and 8.3 us, 736: 9.4 and 9.7, 1472: 9.7 and 9.9, 2944: 10.6 and 10.4, 5888: 13.5 and 11.2, 20288: 24.5 and 12.6;
+    // by pages (16 rows) 1000: 9.3 and 9.3, 2000: 9.9 and 9.5, 8000: 12.4 and 10.4, 64000: 33 and 11.6.
     const bool small = static_cast<int64_t>(std::max(a.rows, a.new_rows)) * a.cols <= 2 * RT && a.n_pages <= RT;
     rc = launch_pdl(small ? reorder_tables_kernel<1> : reorder_tables_kernel<8>, dim3(small ? 1 : 8), dim3(RT), 0, st, a,
                     full, part, owner, freelist, rows, copies, n_copies, ds->d_error);

@@ -32,7 +32,8 @@ def paged_attention(q, k_pages, v_pages, table, ctx_len, cu=None, *, max_q=None,
     kv_heads).  window > 0 limits a row to the last `window` keys, its own
     among them.  scale defaults to head_dim ** -0.5.  max_q: the most new rows
     of one sequence (a host number; the number of rows if not given, which is
-    right but chooses the kernel for long chunks).  Returns out (written to
+    right but chooses the kernel for long chunks; rows of a sequence behind its
+    first max_q are left out).  Returns out (written to
     `out` if given: contiguous, q's shape and type), or (out, lse) with lse
     float32 [rows, heads], the natural logarithm of the softmax's
     denominators.  A row without keys gives 0 and -inf."""
